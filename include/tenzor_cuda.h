@@ -343,6 +343,27 @@ int tz_ew_unary_chain(tz_ctx_t ctx, const float* x, float* out, int64_t n, const
 /* FusedReduceKernel, codegen.zig:151-205: *out (device) = reduce(pre_ops(x)). */
 int tz_reduce(tz_ctx_t ctx, int reduce_op, const int* pre_ops, int n_pre, const float* x,
               int64_t n, float* out, tz_stream_t stream);
+/* ---- gated feed-forward block (device pointers, async on `stream`) --------------------------
+ * h = act(x Wg^T) * (x Wu^T): both projections, the activation and the product in one kernel, and its
+ * gradient.  x [t, d] with row stride ldx, w_gate and w_up [f, d] (PyTorch [out, in]), h [t, f]; all of
+ * the 16-bit type `dtype` (tz_gemm_prec: TZ_PREC_F16 or TZ_PREC_BF16), 16-byte aligned; d, f and the row
+ * strides multiples of 8, any t >= 0.  act: TZ_OP_SILU, TZ_OP_GELU (tanh form), TZ_OP_GELU_ERF,
+ * TZ_OP_RELU or TZ_OP_SIGMOID.  Products accumulate in f32, activation and product are f32, and h is
+ * rounded once. */
+int tz_gated_linear(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate, const void* w_up, void* h,
+                    int64_t t, int d, int f, int act, int dtype, tz_stream_t stream);
+/* Bytes of device workspace one tz_gated_linear_backward call of these sizes needs. */
+int tz_gated_linear_backward_workspace(tz_ctx_t ctx, int64_t t, int d, int f, size_t* bytes);
+/* dx [t, d], dw_gate and dw_up [f, d] from dh [t, f] (row stride lddh).  Nothing of the forward pass is
+ * kept: gate and up are computed again in f32.  Their gradients are rounded once to `dtype` as operands of
+ * the next products (an f16 value beyond 65504 there becomes an infinity); every sum is f32, and the order
+ * of summation depends on the sizes alone.  The caller owns the workspace (16-byte aligned) until the
+ * stream has passed the call.  t = 0 zeroes the weights' gradients. */
+int tz_gated_linear_backward(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate, const void* w_up,
+                             const void* dh, int64_t lddh, void* dx, void* dw_gate, void* dw_up, void* workspace,
+                             size_t workspace_bytes, int64_t t, int d, int f, int act, int dtype,
+                             tz_stream_t stream);
+
 /* ---- N-D tensor ops of the `.eval()` executor and the ONNX op map ---------------------------
  * Device pointers, asynchronous on `stream`, f32 unless noted. */
 /* Batched matmul with broadcast batch dimensions (evalBatchedMatmul, executor.zig:199-325, and

@@ -40,6 +40,7 @@ EXPORTS = [
     "tz_tenzor_close", "tz_tenzor_count", "tz_tenzor_entry_at", "tz_tenzor_find", "tz_tenzor_metadata",
     "tz_lenet_load_tenzor", "tz_arctic_load_tenzor", "tz_ew_program_run_nd", "tz_batched_matmul",
     "tz_matmul_f32x3", "tz_reduce_axis", "tz_softmax_axis", "tz_permute", "tz_cast", "tz_concat",
+    "tz_gated_linear", "tz_gated_linear_backward", "tz_gated_linear_backward_workspace",
 ]
 
 
@@ -176,6 +177,9 @@ def _declare(L):
         "tz_permute": [P, P, P, i, i, P, P, P],
         "tz_cast": [P, P, i, P, i, i64, P],
         "tz_concat": [P, P, P, i, i64, i64, i, P, P],
+        "tz_gated_linear": [P, P, i64, P, P, P, i64, i, i, i, i, P],
+        "tz_gated_linear_backward_workspace": [P, i64, i, i, C.POINTER(u)],
+        "tz_gated_linear_backward": [P, P, i64, P, P, P, i64, P, P, P, P, u, i64, i, i, i, i, P],
     }
     for name, args in sig.items():
         f = getattr(L, name)

@@ -1,0 +1,657 @@
+// tz_gated.cu -- the gated feed-forward block in 16 bits, forward and backward, on tcgen05.
+//
+//   forward    g = x Wg^T, u = x Wu^T,  h = act(g) * u                    x [T, D], Wg and Wu [F, D], h [T, F]
+//   backward   dg = dh * u * act'(g),  du = dh * act(g)                   g and u are computed again
+//              dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
+//
+// One persistent kernel template with four forms (what differs is the operands' layout and the epilogue):
+//   FWD  both projections of a tile in one accumulator: its B tile is BN/2 rows of Wg over BN/2 rows of Wu, so
+//        one MMA makes the gate and the up columns of the same outputs; the epilogue multiplies them
+//   BWD  the same products; the epilogue makes dg and du (16 bits) from them and dh, all in f32 before the
+//        one rounding that the tensor core needs for the next products' operands
+//   DX   [dg | du] [Wg ; Wu]: one accumulation over both halves; the weights are read MN-major in place
+//   DW   dg^T x and du^T x: both operands MN-major in place (the sum runs over tokens); where the tiles do not
+//        fill the GPU the tokens are split and the f32 partial sums added in a fixed order by a second kernel
+//
+// Per CTA (64 + 32 * EPI warps): warp 0 TMA producer, warp 1 allocates TMEM and issues the MMAs, the others
+// read the accumulators (two buffers: the epilogue of a tile runs under the next tile's MMAs) and store boxes
+// of 32 x 32 outputs through swizzled shared memory and TMA, which clips ragged edges.  TMA fills reads
+// outside the operands with zeros, so any T works; D and F are multiples of 8 (16-byte rows).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "tz_act.cuh"
+#include "tz_internal.h"
+#include "tz_pair.cuh"
+
+namespace tz {
+namespace {
+
+enum { MM_FWD = 0, MM_BWD = 1, MM_DX = 2, MM_DW = 3 };
+
+struct MmParams {
+    int m_tiles, n_tiles;  // tiles of 128 * CG rows x BN columns (FWD / BWD: BN / 2 output columns)
+    int which;             // DW: 2 (dWg and dWu), else 1
+    int splits;            // of the K blocks; > 1: f32 partial sums
+    int kblocks;           // K blocks of 64, both halves for DX
+    int half;              // DX: K blocks of one half
+    int kper;              // K blocks per split
+    int m_pad;             // rows of one partial sum
+    int rows, cols;        // BWD: of dh
+    const void* dh;
+    long long ldh;
+    int act;
+};
+
+template <int CG, int BN, int MODE>
+struct MmCfg {
+    static constexpr bool kDual = MODE == MM_FWD || MODE == MM_BWD;
+    static constexpr bool kAmn = MODE == MM_DW;
+    static constexpr bool kBmn = MODE == MM_DX || MODE == MM_DW;
+    static constexpr int EPI = 8;
+    static constexpr int THREADS = 64 + 32 * EPI;
+    static constexpr int BNC = BN / CG;  // B rows (or columns) in one CTA
+    static constexpr int A_BYTES = 128 * 128;
+    static constexpr int STAGE = A_BYTES + BNC * 128;
+    static constexpr int STAGING = EPI * 4096;
+    static constexpr int BUDGET = 227 * 1024 - 1024 - 512 - STAGING;
+    static constexpr int STAGES = BUDGET / STAGE > 8 ? 8 : BUDGET / STAGE;
+    static constexpr int SMEM = STAGES * STAGE + STAGING + 512 + 1024;
+    static_assert(!kBmn || BNC % 64 == 0, "MN-major B comes in blocks of 64");
+};
+
+// act over 32 gate / up pairs -> packed 16-bit outputs.
+template <int ACT, bool BF>
+__device__ __forceinline__ void fwd_math(const uint32_t (&g)[32], const uint32_t (&u)[32], uint32_t (&o)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        float d;
+        const float a = gated_act<ACT, false>(__uint_as_float(g[2 * j]), d) * __uint_as_float(u[2 * j]);
+        const float b = gated_act<ACT, false>(__uint_as_float(g[2 * j + 1]), d) * __uint_as_float(u[2 * j + 1]);
+        o[j] = tzp::pack16x2<BF>(a, b);
+    }
+}
+template <int ACT, bool BF>
+__device__ __forceinline__ void bwd_math(const uint32_t (&g)[32], const uint32_t (&u)[32], const uint32_t (&dh)[16],
+                                         uint32_t (&dg)[16], uint32_t (&du)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        float2 h;
+        if constexpr (BF)
+            h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&dh[j]));
+        else
+            h = __half22float2(*reinterpret_cast<const __half2*>(&dh[j]));
+        float d0, d1;
+        const float a0 = gated_act<ACT, true>(__uint_as_float(g[2 * j]), d0);
+        const float a1 = gated_act<ACT, true>(__uint_as_float(g[2 * j + 1]), d1);
+        dg[j] = tzp::pack16x2<BF>(h.x * __uint_as_float(u[2 * j]) * d0, h.y * __uint_as_float(u[2 * j + 1]) * d1);
+        du[j] = tzp::pack16x2<BF>(h.x * a0, h.y * a1);
+    }
+}
+
+#define TZ_ACT_SWITCH(act, CALL)                          \
+    switch (act) {                                        \
+        case TZ_OP_SILU: CALL(TZ_OP_SILU); break;         \
+        case TZ_OP_GELU: CALL(TZ_OP_GELU); break;         \
+        case TZ_OP_GELU_ERF: CALL(TZ_OP_GELU_ERF); break; \
+        case TZ_OP_RELU: CALL(TZ_OP_RELU); break;         \
+        default: CALL(TZ_OP_SIGMOID); break;              \
+    }
+
+// 32 rows (one per lane) x 64 bytes into a 2 KB box with the 64-byte swizzle.
+__device__ __forceinline__ void stage64(uint32_t buf, int lane, const uint32_t (&o)[16]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        tzp::st_shared_v4(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+}
+// 32 rows x 128 bytes into a 4 KB box with the 128-byte swizzle.
+__device__ __forceinline__ void stage128(uint32_t buf, int lane, const uint32_t (&v)[32]) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        tzp::st_shared_v4(buf + lane * 128 + ((c ^ (lane & 7)) << 4), v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+}
+
+template <int CG, int BN, int MODE, bool BF, bool PART>
+__global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
+    gated_mm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
+                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+                    const __grid_constant__ CUtensorMap tmO0, const __grid_constant__ CUtensorMap tmO1, const MmParams p,
+                    int* status) {
+    using C = MmCfg<CG, BN, MODE>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = tzp::smem_u32(smem_raw);
+    uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+    uint8_t* staging = smem + STAGES * C::STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? tzp::cluster_ctarank() : 0u;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tzp::mbar_init(&full[s], 1);
+            tzp::mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            tzp::mbar_init(&tfull[a], 1);
+            tzp::mbar_init(&tempty[a], C::EPI * CG);
+        }
+        tzp::mbar_init(drain, 1);
+        *abort_flag = 0;
+        tzp::fence_mbar_init();
+        tzp::tma_prefetch_desc(&tmA0);
+        tzp::tma_prefetch_desc(&tmB0);
+    }
+    if (warp == 1) tzp::pair_tmem_alloc<CG>(tmem_slot, 2 * BN);
+    tzp::tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) tzp::cluster_sync();  // both CTAs' barriers exist before either signals them
+    tzp::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    tzp::pdl_trigger();
+    tzp::pdl_wait();
+
+    // Tile t of this launch: a group of 8 row blocks walks all column blocks before the next group starts, so
+    // that the CTAs running at one time share both operands in L2.
+    const int per = p.m_tiles * p.n_tiles;
+    const int num_tiles = per * p.which * p.splits;
+    struct Tile {
+        int m, n, w, s, kb0, kb1;
+    };
+    auto tile_of = [&](int t) {
+        Tile r;
+        r.s = t / (per * p.which);
+        t -= r.s * per * p.which;
+        r.w = t / per;
+        t -= r.w * per;
+        constexpr int GM = 8;
+        const int grp = t / (GM * p.n_tiles);
+        const int gm = min(GM, p.m_tiles - grp * GM);
+        t -= grp * GM * p.n_tiles;
+        r.m = grp * GM + t % gm;
+        r.n = t / gm;
+        r.kb0 = r.s * p.kper;
+        r.kb1 = min(p.kblocks, r.kb0 + p.kper);
+        return r;
+    };
+    const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---- TMA producer ----
+            int stage = 0;
+            uint32_t phase = 0, armed = 0, armed_par = 0;
+            bool ok = true;
+            for (int t = t0; ok && t < num_tiles; t += tstep) {
+                const Tile q = tile_of(t);
+                const int m0 = (q.m * CG + static_cast<int>(rank)) * 128;
+                for (int kb = q.kb0; kb < q.kb1; ++kb) {
+                    if (!tzp::pair_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) {
+                        tzp::mbar_arrive_expect_tx(&full[stage], CG * C::STAGE);
+                        armed |= 1u << stage;
+                        armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
+                    }
+                    const uint32_t bar = CG == 2 ? tzp::mapa(&full[stage], 0) : tzp::smem_u32(&full[stage]);
+                    const uint32_t sa = tzp::smem_u32(smem + stage * C::STAGE);
+                    const uint32_t sb = sa + C::A_BYTES;
+                    if constexpr (MODE == MM_DW) {
+                        const CUtensorMap* ta = q.w ? &tmA1 : &tmA0;
+                        tzp::pair_load_2d<CG>(sa, ta, m0, kb * 64, bar);
+                        tzp::pair_load_2d<CG>(sa + 8192, ta, m0 + 64, kb * 64, bar);
+#pragma unroll
+                        for (int j = 0; j < C::BNC / 64; ++j)
+                            tzp::pair_load_2d<CG>(sb + j * 8192, &tmB0, q.n * BN + static_cast<int>(rank) * C::BNC + 64 * j, kb * 64, bar);
+                    } else if constexpr (MODE == MM_DX) {
+                        const bool up = kb >= p.half;
+                        const int k = (up ? kb - p.half : kb) * 64;
+                        tzp::pair_load_2d<CG>(sa, up ? &tmA1 : &tmA0, k, m0, bar);
+#pragma unroll
+                        for (int j = 0; j < C::BNC / 64; ++j)
+                            tzp::pair_load_2d<CG>(sb + j * 8192, up ? &tmB1 : &tmB0, q.n * BN + static_cast<int>(rank) * C::BNC + 64 * j, k, bar);
+                    } else {
+                        tzp::pair_load_2d<CG>(sa, &tmA0, kb * 64, m0, bar);
+                        if constexpr (CG == 2) {
+                            tzp::pair_load_2d<CG>(sb, rank ? &tmB1 : &tmB0, kb * 64, q.n * (BN / 2), bar);
+                        } else {
+                            tzp::pair_load_2d<CG>(sb, &tmB0, kb * 64, q.n * (BN / 2), bar);
+                            tzp::pair_load_2d<CG>(sb + (BN / 2) * 128, &tmB1, kb * 64, q.n * (BN / 2), bar);
+                        }
+                    }
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            // Every copy has landed before the CTA can exit (bounded; the pair's copies all count on the leader).
+            for (int s = 0; s < STAGES; ++s)
+                if (armed & (1u << s)) tzp::pair_wait<CG>(&full[s], (armed_par >> s) & 1u, status, nullptr);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            // ---- MMA issuer ----
+            constexpr uint32_t idesc = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, BN) | (C::kAmn ? 1u << 15 : 0u) | (C::kBmn ? 1u << 16 : 0u);
+            constexpr uint32_t kAstep = C::kAmn ? 2048u >> 4 : 2u, kBstep = C::kBmn ? 2048u >> 4 : 2u;
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int t = t0; ok && t < num_tiles; t += tstep) {
+                const Tile q = tile_of(t);
+                if (!tzp::pair_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
+                tzp::tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                for (int kb = q.kb0; kb < q.kb1; ++kb) {
+                    if (!tzp::pair_wait<CG>(&full[stage], phase, status, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tzp::tc_fence_after();
+                    const uint32_t sa = tzp::smem_u32(smem + stage * C::STAGE);
+                    const uint64_t ad = C::kAmn ? tzp::sdesc_mn128(sa, 8192) : tzp::sdesc_k128(sa);
+                    const uint64_t bd = C::kBmn ? tzp::sdesc_mn128(sa + C::A_BYTES, 8192) : tzp::sdesc_k128(sa + C::A_BYTES);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tzp::pair_mma_f16<CG>(d, ad + kAstep * k, bd + kBstep * k, idesc, (kb > q.kb0 || k > 0) ? 1u : 0u);
+                    tzp::pair_commit<CG>(&empty[stage]);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                tzp::pair_commit<CG>(&tfull[acc]);
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+            // Every MMA issued has completed before TMEM is released.
+            tzp::pair_commit<CG>(drain);
+            tzp::pair_wait<CG>(drain, 0, status, nullptr);
+        }
+    } else {
+        // ---- epilogue: warp reads TMEM lane quarter (warp % 4) and half of the columns ----
+        const int e = warp - 2, q4 = warp & 3, hf = e >> 2;
+        const uint32_t box = tzp::smem_u32(staging) + static_cast<uint32_t>(e * 4096);
+        uint8_t* boxp = staging + e * 4096;
+        int acc = 0, nb = 0;
+        uint32_t acc_phase = 0;
+        for (int t = t0; t < num_tiles; t += tstep) {
+            const Tile q = tile_of(t);
+            if (!tzp::pair_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
+            tzp::tc_fence_after();
+            const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN);
+            const int row0 = (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32;
+            if constexpr (C::kDual) {
+                constexpr int CH = BN / 128;  // 32-column chunks of this warp: half of the BN / 2 outputs
+#pragma unroll 1
+                for (int c = 0; c < CH; ++c) {
+                    const int cc = (hf * CH + c) * 32;
+                    const int col0 = q.n * (BN / 2) + cc;
+                    if (col0 >= p.cols) break;
+                    uint32_t dh[16];
+                    if constexpr (MODE == MM_BWD) {
+                        const bool rok = row0 + lane < p.rows;
+                        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.dh) + (row0 + lane) * p.ldh + col0);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint4 v = make_uint4(0, 0, 0, 0);
+                            if (rok && col0 + 8 * j < p.cols) v = __ldg(src + j);
+                            dh[4 * j] = v.x, dh[4 * j + 1] = v.y, dh[4 * j + 2] = v.z, dh[4 * j + 3] = v.w;
+                        }
+                    }
+                    uint32_t g[32], u[32];
+                    tzp::tmem_ld32(td + cc, g);
+                    tzp::tmem_ld32(td + BN / 2 + cc, u);
+                    tzp::tmem_ld_wait();
+                    if constexpr (MODE == MM_FWD) {
+                        uint32_t o[16];
+#define TZ_FWD(A) fwd_math<A, BF>(g, u, o)
+                        TZ_ACT_SWITCH(p.act, TZ_FWD)
+#undef TZ_FWD
+                        if (lane == 0) tzp::bulk_wait_read<1>();  // the store that used this box has read it
+                        __syncwarp();
+                        stage64(box + nb * 2048, lane, o);
+                        tzp::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tzp::tma_store_2d(&tmO0, boxp + nb * 2048, col0, row0);
+                            tzp::bulk_commit();
+                        }
+                        nb ^= 1;
+                    } else {
+                        uint32_t dg[16], du[16];
+#define TZ_BWD(A) bwd_math<A, BF>(g, u, dh, dg, du)
+                        TZ_ACT_SWITCH(p.act, TZ_BWD)
+#undef TZ_BWD
+                        if (lane == 0) tzp::bulk_wait_read<0>();
+                        __syncwarp();
+                        stage64(box, lane, dg);
+                        stage64(box + 2048, lane, du);
+                        tzp::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tzp::tma_store_2d(&tmO0, boxp, col0, row0);
+                            tzp::tma_store_2d(&tmO1, boxp + 2048, col0, row0);
+                            tzp::bulk_commit();
+                        }
+                    }
+                }
+            } else {
+                constexpr int CH = BN / 64;
+#pragma unroll 1
+                for (int c = 0; c < CH; ++c) {
+                    const int cc = (hf * CH + c) * 32;
+                    const int col0 = q.n * BN + cc;
+                    if (col0 >= p.cols) break;
+                    uint32_t v[32];
+                    tzp::tmem_ld32(td + cc, v);
+                    tzp::tmem_ld_wait();
+                    if constexpr (PART) {
+                        if (lane == 0) tzp::bulk_wait_read<0>();
+                        __syncwarp();
+                        stage128(box, lane, v);
+                        tzp::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tzp::tma_store_2d(&tmO0, boxp, col0, (q.s * p.which + q.w) * p.m_pad + row0);
+                            tzp::bulk_commit();
+                        }
+                    } else {
+                        uint32_t o[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = tzp::pack16x2<BF>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                        if (lane == 0) tzp::bulk_wait_read<1>();
+                        __syncwarp();
+                        stage64(box + nb * 2048, lane, o);
+                        tzp::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tzp::tma_store_2d(q.w ? &tmO1 : &tmO0, boxp + nb * 2048, col0, row0);
+                            tzp::bulk_commit();
+                        }
+                        nb ^= 1;
+                    }
+                }
+            }
+            tzp::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2)
+                    tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
+                else
+                    tzp::mbar_arrive(&tempty[acc]);
+            }
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        if (lane == 0) tzp::bulk_wait_all();
+    }
+
+    tzp::tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) tzp::cluster_sync();  // no CTA leaves while the other may still signal it
+    if (warp == 1) {
+        __syncwarp();
+        tzp::tc_fence_after();
+        tzp::pair_tmem_dealloc<CG>(tmem_base, 2 * BN);
+    }
+}
+
+// Sums the partial products [splits][which][m_pad][cols] in order and rounds to 16 bits.
+template <bool BF>
+__global__ void sum_parts_kernel(const float* part, void* out0, void* out1, int which, int splits, int m_pad, int rows, int cols) {
+    tzp::pdl_trigger();
+    tzp::pdl_wait();
+    const long long n8 = static_cast<long long>(rows) * cols / 8;
+    const long long plane = static_cast<long long>(m_pad) * cols;
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n8 * which; i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int w = i >= n8;
+        const long long o = (i - (w ? n8 : 0)) * 8;
+        float s[8] = {};
+        for (int k = 0; k < splits; ++k) {
+            const float4* src = reinterpret_cast<const float4*>(part + (static_cast<long long>(k) * which + w) * plane + o);
+            const float4 a = __ldcs(src), b = __ldcs(src + 1);
+            s[0] += a.x, s[1] += a.y, s[2] += a.z, s[3] += a.w, s[4] += b.x, s[5] += b.y, s[6] += b.z, s[7] += b.w;
+        }
+        uint4 r = make_uint4(tzp::pack16x2<BF>(s[0], s[1]), tzp::pack16x2<BF>(s[2], s[3]), tzp::pack16x2<BF>(s[4], s[5]), tzp::pack16x2<BF>(s[6], s[7]));
+        reinterpret_cast<uint4*>(w ? out1 : out0)[o / 8] = r;
+    }
+}
+
+// One operand or output of a product: row-major, 16 bits.
+struct Mat {
+    const void* p;
+    int64_t rows, cols, ld;
+};
+
+template <bool BF>
+int map16(CUtensorMap* m, const Mat& a, int box_cols, int box_rows, CUtensorMapSwizzle swz) {
+    return encode_tmap_2d_swz(m, BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.p, a.cols, a.rows,
+                              a.ld * 2, box_cols, box_rows, swz);
+}
+
+template <int CG, int BN, int MODE, bool BF, bool PART>
+int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, const Mat& o0, const Mat& o1, MmParams p,
+              float* part, cudaStream_t s) {
+    using C = MmCfg<CG, BN, MODE>;
+    auto kern = gated_mm_kernel<CG, BN, MODE, BF, PART>;
+    static std::atomic<unsigned> done{0};
+    int rc = ensure_smem(kern, C::SMEM, done);
+    if (rc) return rc;
+    CUtensorMap ma0, ma1, mb0, mb1, mo0, mo1;
+    const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B;
+    const int arows = C::kAmn ? 64 : 128, brows = C::kBmn ? 64 : (C::kDual ? BN / 2 : C::BNC);
+    if ((rc = map16<BF>(&ma0, a0, 64, arows, S128)) || (rc = map16<BF>(&ma1, a1, 64, arows, S128)) ||
+        (rc = map16<BF>(&mb0, b0, 64, brows, S128)) || (rc = map16<BF>(&mb1, b1, 64, brows, S128)))
+        return rc;
+    if (PART) {
+        rc = encode_tmap_2d_swz(&mo0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, o0.cols,
+                                static_cast<uint64_t>(p.splits) * p.which * p.m_pad, o0.cols * 4, 32, 32, S128);
+        mo1 = mo0;
+    } else {
+        rc = map16<BF>(&mo0, o0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+        if (!rc) rc = map16<BF>(&mo1, o1, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+    }
+    if (rc) return rc;
+    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * p.which * p.splits;
+    const int groups = (ctx->sm_count - ctx->sm_reserve) / CG;
+    const int grid = static_cast<int>(tiles < groups ? tiles : groups) * CG;
+    TZ_CHECK(grid > 0, TZ_EINVAL, "gated kernels need %d free SMs", CG);
+    return launch_cluster(kern, CG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma0, ma1, mb0, mb1, mo0, mo1, p, ctx->d_status);
+}
+
+constexpr int kCG = 1, kBN = 256;
+
+int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+// Splits of the K blocks so that the tiles fill the GPU, each with at least 8 K blocks.
+int pick_splits(tz_ctx_t ctx, int64_t tiles, int kblocks) {
+    const int groups = (ctx->sm_count - ctx->sm_reserve) / kCG;
+    int s = static_cast<int>(groups / (tiles < 1 ? 1 : tiles));
+    if (s > kblocks / 8) s = kblocks / 8;
+    if (s > 16) s = 16;
+    if (s <= 1) return 1;
+    return ceil_div(kblocks, ceil_div(kblocks, s));  // no split without K blocks
+}
+
+struct BwdPlan {
+    size_t dgdu, part_dx, part_dw;  // bytes
+    int s_dx, s_dw;
+};
+BwdPlan plan_bwd(tz_ctx_t ctx, int64_t T, int64_t D, int64_t F) {
+    BwdPlan b{};
+    auto a256 = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
+    b.dgdu = a256(static_cast<size_t>(T) * F * 2);
+    const int mt = ceil_div(T, 128 * kCG), nt = ceil_div(D, kBN), ft = ceil_div(F, 128 * kCG);
+    b.s_dx = pick_splits(ctx, static_cast<int64_t>(mt) * nt, 2 * ceil_div(F, 64));
+    b.s_dw = pick_splits(ctx, 2ll * ft * nt, ceil_div(T, 64));
+    if (b.s_dx > 1) b.part_dx = a256(static_cast<size_t>(b.s_dx) * mt * 128 * kCG * D * 4);
+    if (b.s_dw > 1) b.part_dw = a256(static_cast<size_t>(b.s_dw) * 2 * ft * 128 * kCG * D * 4);
+    return b;
+}
+
+template <bool BF>
+int sum_parts(tz_ctx_t ctx, const float* part, void* o0, void* o1, int which, int splits, int m_pad, int rows, int cols, cudaStream_t s) {
+    const long long n8 = static_cast<long long>(rows) * cols / 8 * which;
+    const int blocks = static_cast<int>(n8 / 256 + 1 < ctx->sm_count * 8 ? n8 / 256 + 1 : ctx->sm_count * 8);
+    return launch_kernel(sum_parts_kernel<BF>, dim3(blocks), dim3(256), 0, s, true, part, o0, o1, which, splits, m_pad, rows, cols);
+}
+
+template <bool BF>
+int forward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& h, int act, cudaStream_t s) {
+    MmParams p{};
+    p.m_tiles = ceil_div(x.rows, 128 * kCG);
+    p.n_tiles = ceil_div(h.cols, kBN / 2);
+    p.which = p.splits = 1;
+    p.kblocks = p.kper = ceil_div(x.cols, 64);
+    p.rows = static_cast<int>(h.rows);
+    p.cols = static_cast<int>(h.cols);
+    p.act = act;
+    return launch_mm<kCG, kBN, MM_FWD, BF, false>(ctx, x, x, wg, wu, h, h, p, nullptr, s);
+}
+
+template <bool BF>
+int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& dh, const Mat& dx, const Mat& dwg, const Mat& dwu,
+             int act, char* ws, cudaStream_t s) {
+    const int64_t T = x.rows, D = x.cols, F = dh.cols;
+    const BwdPlan b = plan_bwd(ctx, T, D, F);
+    const Mat dg{ws, T, F, F}, du{ws + b.dgdu, T, F, F};
+    float* part_dx = reinterpret_cast<float*>(ws + 2 * b.dgdu);
+    float* part_dw = reinterpret_cast<float*>(ws + 2 * b.dgdu + b.part_dx);
+    MmParams p{};
+    p.m_tiles = ceil_div(T, 128 * kCG);
+    p.n_tiles = ceil_div(F, kBN / 2);
+    p.which = p.splits = 1;
+    p.kblocks = p.kper = ceil_div(D, 64);
+    p.rows = static_cast<int>(T);
+    p.cols = static_cast<int>(F);
+    p.dh = dh.p;
+    p.ldh = dh.ld;
+    p.act = act;
+    int rc = launch_mm<kCG, kBN, MM_BWD, BF, false>(ctx, x, x, wg, wu, dg, du, p, nullptr, s);
+    if (rc) return rc;
+
+    MmParams q{};
+    q.m_tiles = ceil_div(T, 128 * kCG);
+    q.n_tiles = ceil_div(D, kBN);
+    q.which = 1;
+    q.splits = b.s_dx;
+    q.half = ceil_div(F, 64);
+    q.kblocks = 2 * q.half;
+    q.kper = ceil_div(q.kblocks, q.splits);
+    q.m_pad = q.m_tiles * 128 * kCG;
+    q.rows = static_cast<int>(T);
+    q.cols = static_cast<int>(D);
+    if (q.splits > 1) {
+        rc = launch_mm<kCG, kBN, MM_DX, BF, true>(ctx, dg, du, wg, wu, dx, dx, q, part_dx, s);
+        if (!rc) rc = sum_parts<BF>(ctx, part_dx, const_cast<void*>(dx.p), nullptr, 1, q.splits, q.m_pad, q.rows, q.cols, s);
+    } else {
+        rc = launch_mm<kCG, kBN, MM_DX, BF, false>(ctx, dg, du, wg, wu, dx, dx, q, nullptr, s);
+    }
+    if (rc) return rc;
+
+    MmParams r{};
+    r.m_tiles = ceil_div(F, 128 * kCG);
+    r.n_tiles = ceil_div(D, kBN);
+    r.which = 2;
+    r.splits = b.s_dw;
+    r.kblocks = ceil_div(T, 64);
+    r.kper = ceil_div(r.kblocks, r.splits);
+    r.m_pad = r.m_tiles * 128 * kCG;
+    r.rows = static_cast<int>(F);
+    r.cols = static_cast<int>(D);
+    if (r.splits > 1) {
+        rc = launch_mm<kCG, kBN, MM_DW, BF, true>(ctx, dg, du, x, x, dwg, dwu, r, part_dw, s);
+        if (!rc) rc = sum_parts<BF>(ctx, part_dw, const_cast<void*>(dwg.p), const_cast<void*>(dwu.p), 2, r.splits, r.m_pad, r.rows, r.cols, s);
+        return rc;
+    }
+    return launch_mm<kCG, kBN, MM_DW, BF, false>(ctx, dg, du, x, x, dwg, dwu, r, nullptr, s);
+}
+
+bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check_shape(const char* fn, int64_t T, int D, int F, int dtype, int act) {
+    TZ_CHECK(dtype == TZ_PREC_F16 || dtype == TZ_PREC_BF16, TZ_EINVAL, "%s: dtype %d is neither f16 nor bf16", fn, dtype);
+    TZ_CHECK(gated_act_ok(act), TZ_EINVAL, "%s: activation %d is not silu, gelu, gelu_erf, relu or sigmoid", fn, act);
+    TZ_CHECK(T >= 0 && T <= (1 << 30) && D > 0 && F > 0 && D <= (1 << 24) && F <= (1 << 24), TZ_EINVAL, "%s: bad sizes T=%lld D=%d F=%d", fn,
+             static_cast<long long>(T), D, F);
+    TZ_CHECK(D % 8 == 0 && F % 8 == 0, TZ_EINVAL, "%s: D and F must be multiples of 8 (D=%d F=%d)", fn, D, F);
+    return TZ_OK;
+}
+
+}  // namespace
+}  // namespace tz
+
+using namespace tz;
+
+extern "C" {
+
+int tz_gated_linear(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate, const void* w_up, void* h, int64_t t, int d, int f,
+                    int act, int dtype, tz_stream_t stream) {
+    TZ_CHECK(ctx, TZ_EINVAL, "tz_gated_linear: null context");
+    int rc = check_shape("tz_gated_linear", t, d, f, dtype, act);
+    if (rc) return rc;
+    if (t == 0) return TZ_OK;
+    TZ_CHECK(x && w_gate && w_up && h, TZ_EINVAL, "tz_gated_linear: null pointer");
+    TZ_CHECK(ldx >= d && ldx % 8 == 0, TZ_EINVAL, "tz_gated_linear: row stride %lld of x (at least D, a multiple of 8)", static_cast<long long>(ldx));
+    TZ_CHECK(al16(x) && al16(w_gate) && al16(w_up) && al16(h), TZ_EINVAL, "tz_gated_linear: pointers must be 16-byte aligned");
+    cudaStream_t s = pick_stream(ctx, stream);
+    const Mat mx{x, t, d, ldx}, mg{w_gate, f, d, d}, mu{w_up, f, d, d}, mh{h, t, f, f};
+    return dtype == TZ_PREC_BF16 ? forward<true>(ctx, mx, mg, mu, mh, act, s) : forward<false>(ctx, mx, mg, mu, mh, act, s);
+}
+
+int tz_gated_linear_backward_workspace(tz_ctx_t ctx, int64_t t, int d, int f, size_t* bytes) {
+    TZ_CHECK(ctx && bytes, TZ_EINVAL, "tz_gated_linear_backward_workspace: null argument");
+    int rc = check_shape("tz_gated_linear_backward_workspace", t, d, f, TZ_PREC_F16, TZ_OP_SILU);
+    if (rc) return rc;
+    const BwdPlan b = plan_bwd(ctx, t, d, f);
+    *bytes = 2 * b.dgdu + b.part_dx + b.part_dw;
+    return TZ_OK;
+}
+
+int tz_gated_linear_backward(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* dh, int64_t lddh,
+                             void* dx, void* dw_gate, void* dw_up, void* workspace, size_t workspace_bytes, int64_t t, int d, int f,
+                             int act, int dtype, tz_stream_t stream) {
+    TZ_CHECK(ctx, TZ_EINVAL, "tz_gated_linear_backward: null context");
+    int rc = check_shape("tz_gated_linear_backward", t, d, f, dtype, act);
+    if (rc) return rc;
+    TZ_CHECK(w_gate && w_up && dw_gate && dw_up && (t == 0 || (x && dh && dx && workspace)), TZ_EINVAL, "tz_gated_linear_backward: null pointer");
+    cudaStream_t s = pick_stream(ctx, stream);
+    if (t == 0) {  // an empty sum
+        TZ_CUDA(cudaMemsetAsync(dw_gate, 0, static_cast<size_t>(d) * f * 2, s));
+        TZ_CUDA(cudaMemsetAsync(dw_up, 0, static_cast<size_t>(d) * f * 2, s));
+        return TZ_OK;
+    }
+    TZ_CHECK(ldx >= d && ldx % 8 == 0 && lddh >= f && lddh % 8 == 0, TZ_EINVAL,
+             "tz_gated_linear_backward: row strides %lld of x and %lld of dh (at least the width, multiples of 8)", static_cast<long long>(ldx),
+             static_cast<long long>(lddh));
+    TZ_CHECK(al16(x) && al16(w_gate) && al16(w_up) && al16(dh) && al16(dx) && al16(dw_gate) && al16(dw_up) && al16(workspace), TZ_EINVAL,
+             "tz_gated_linear_backward: pointers must be 16-byte aligned");
+    size_t need = 0;
+    if ((rc = tz_gated_linear_backward_workspace(ctx, t, d, f, &need))) return rc;
+    TZ_CHECK(workspace_bytes >= need, TZ_EINVAL, "tz_gated_linear_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    const Mat mx{x, t, d, ldx}, mg{w_gate, f, d, d}, mu{w_up, f, d, d}, mdh{dh, t, f, lddh}, mdx{dx, t, d, d}, mwg{dw_gate, f, d, d},
+        mwu{dw_up, f, d, d};
+    char* ws = static_cast<char*>(workspace);
+    return dtype == TZ_PREC_BF16 ? backward<true>(ctx, mx, mg, mu, mdh, mdx, mwg, mwu, act, ws, s)
+                                 : backward<false>(ctx, mx, mg, mu, mdh, mdx, mwg, mwu, act, ws, s);
+}
+
+}  // extern "C"

@@ -8,6 +8,7 @@ every computation runs in libtenzor_cuda.so).  Names follow the reference kernel
   matmul_epilogue       codegen.zig:78-147            ew_add_mul_exp      executor.zig:114-197
   ew_unary_chain        codegen.zig:15-74             reduce              codegen.zig:151-205
   gather_rows           gather.zig:15-57
+Gated feed-forward block (no counterpart in the reference): gated_linear, gated_linear_backward.
 N-D forms (executor.zig / onnx/executor.zig): batched_matmul, matmul_f32x3, reduce_axis, softmax_axis,
 permute, cast, concat.
 """
@@ -280,3 +281,78 @@ def concat(ctx: Context, xs, axis: int):
     L.check(L.lib().tz_concat(ctx.handle, C.addressof(ptrs), C.addressof(ln), len(xs), outer, inner,
                               xs[0].element_size(), _p(out), _stream()))
     return out
+
+
+# ---- gated feed-forward block ----------------------------------------------------------------------
+GATED_ACTS = ("silu", "gelu", "gelu_erf", "relu", "sigmoid")
+_DT16 = {torch.float16: 0, torch.bfloat16: 1}  # tz_gemm_prec
+
+
+def _dtype16(fn, t):
+    d = _DT16.get(t.dtype)
+    if d is None:
+        raise TypeError(f"{fn}: float16 or bfloat16 tensors, got {t.dtype}")
+    return d
+
+
+def _act_code(fn, act):
+    if act not in GATED_ACTS:
+        raise ValueError(f"{fn}: activation {act!r} is not one of {GATED_ACTS}")
+    return L.OP[act]
+
+
+def _rows16(fn, name, t, shape, dtype):
+    """Row stride of a 2-D device tensor of `shape` whose rows are contiguous."""
+    if not t.is_cuda or t.dtype != dtype or t.shape != shape or (t.stride(1) != 1 and shape[1] > 1):
+        raise ValueError(f"{fn}: {name} must be a CUDA {dtype} tensor of shape {tuple(shape)} with contiguous rows, "
+                         f"got {t.dtype} {tuple(t.shape)} stride {t.stride()} on {t.device}")
+    return t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def _full16(fn, name, t, shape, dtype):
+    if not t.is_cuda or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{fn}: {name} must be a contiguous CUDA {dtype} tensor of shape {tuple(shape)}, "
+                         f"got {t.dtype} {tuple(t.shape)} stride {t.stride()} on {t.device}")
+    return t
+
+
+def gated_linear(ctx: Context, x, w_gate, w_up, act: str = "silu", out=None):
+    """act(x @ w_gate.T) * (x @ w_up.T) in one kernel: x [T, D] (rows may be strided), w_gate and w_up [F, D],
+    all float16 or all bfloat16, D and F multiples of 8; returns [T, F].  act: one of GATED_ACTS."""
+    dt = _dtype16("gated_linear", x)
+    if x.dim() != 2 or w_gate.dim() != 2:
+        raise ValueError(f"gated_linear: x [T, D] and weights [F, D], got {tuple(x.shape)} and {tuple(w_gate.shape)}")
+    T, D = x.shape
+    F = w_gate.shape[0]
+    ldx = _rows16("gated_linear", "x", x, (T, D), x.dtype)
+    _full16("gated_linear", "w_gate", w_gate, (F, D), x.dtype)
+    _full16("gated_linear", "w_up", w_up, (F, D), x.dtype)
+    if out is None:
+        out = torch.empty((T, F), device=x.device, dtype=x.dtype)
+    else:
+        _full16("gated_linear", "out", out, (T, F), x.dtype)
+    L.check(L.lib().tz_gated_linear(ctx.handle, _p(x), ldx, _p(w_gate), _p(w_up), _p(out), T, D, F,
+                                    _act_code("gated_linear", act), dt, _stream()))
+    return out
+
+
+def gated_linear_backward(ctx: Context, x, w_gate, w_up, dh, act: str = "silu"):
+    """(dx, dw_gate, dw_up) of gated_linear for the output's gradient dh [T, F]."""
+    dt = _dtype16("gated_linear_backward", x)
+    if x.dim() != 2 or w_gate.dim() != 2:
+        raise ValueError(f"gated_linear_backward: x [T, D] and weights [F, D], got {tuple(x.shape)} and "
+                         f"{tuple(w_gate.shape)}")
+    T, D = x.shape
+    F = w_gate.shape[0]
+    ldx = _rows16("gated_linear_backward", "x", x, (T, D), x.dtype)
+    lddh = _rows16("gated_linear_backward", "dh", dh, (T, F), x.dtype)
+    _full16("gated_linear_backward", "w_gate", w_gate, (F, D), x.dtype)
+    _full16("gated_linear_backward", "w_up", w_up, (F, D), x.dtype)
+    code = _act_code("gated_linear_backward", act)
+    need = C.c_size_t()
+    L.check(L.lib().tz_gated_linear_backward_workspace(ctx.handle, T, D, F, C.byref(need)))
+    ws = torch.empty(max(need.value, 1), device=x.device, dtype=torch.uint8)
+    dx, dwg, dwu = torch.empty((T, D), device=x.device, dtype=x.dtype), torch.empty_like(w_gate), torch.empty_like(w_up)
+    L.check(L.lib().tz_gated_linear_backward(ctx.handle, _p(x), ldx, _p(w_gate), _p(w_up), _p(dh), lddh, _p(dx), _p(dwg),
+                                             _p(dwu), _p(ws), need.value, T, D, F, code, dt, _stream()))
+    return dx, dwg, dwu

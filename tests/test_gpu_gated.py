@@ -1,0 +1,255 @@
+"""Gated feed-forward block (forward and backward) against plain 64-bit formulas.
+
+Tolerances, elementwise and derived from the arithmetic:
+  U       unit roundoff of the 16-bit type (2^-8 bf16, 2^-11 f16), TINY half its smallest subnormal
+  S(n)    a sum of n products in f32 on the tensor core: one rounding or truncation (2^-23) per 16 products
+          and one per partial sum, relative to the sum of the absolute products: (n / 16 + 20) 2^-23
+  ACT     the fast exponential and reciprocal: 2^-19 of the value's scale
+"""
+import ctypes as C
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f16": torch.float16, "bf16": torch.bfloat16}
+U = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f16": 2.0 ** -25, "bf16": 2.0 ** -134}
+ACTS = ["silu", "gelu", "gelu_erf", "relu", "sigmoid"]
+ACT = 2.0 ** -19
+
+
+def act64(name, g):
+    fn = torch.nn.functional
+    return {"silu": fn.silu, "gelu": lambda z: fn.gelu(z, approximate="tanh"), "gelu_erf": fn.gelu, "relu": fn.relu,
+            "sigmoid": torch.sigmoid}[name](g)
+
+
+def S(n):
+    return (n / 16 + 20) * 2.0 ** -23
+
+
+def make(T, D, F, dt, seed=0, wscale=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def r(*s, std=1.0):
+        return (torch.randn(*s, generator=gen, device="cuda") * std).to(DT[dt])
+
+    return r(T, D), r(F, D, std=wscale * D ** -0.5), r(F, D, std=wscale * D ** -0.5), r(T, F, std=0.1)
+
+
+def reference(x, wg, wu, dh, act):
+    """h and the gradients in 64 bits, and the bounds of h, dx, dwg, dwu."""
+    dt = {v: k for k, v in DT.items()}[x.dtype]
+    u16, tiny = U[dt], TINY[dt]
+    x, wg, wu, dh = x.double(), wg.double(), wu.double(), dh.double()
+    g = (x @ wg.t()).requires_grad_(True)
+    u = (x @ wu.t()).requires_grad_(True)
+    a = act64(act, g)
+    h = a * u
+    dg, du = torch.autograd.grad(h, (g, u), dh)
+    (da,) = torch.autograd.grad(act64(act, g).sum(), g)
+    g, u, a, h = g.detach(), u.detach(), a.detach(), h.detach()
+    D, F, T = x.shape[1], wg.shape[0], x.shape[0]
+    eg, eu = S(D) * (x.abs() @ wg.abs().t()), S(D) * (x.abs() @ wu.abs().t())
+    scale = 1.0 + g.abs()
+    ea = 1.13 * eg + ACT * scale  # |act'| <= 1.13
+    th = u16 * h.abs() + (1 + u16) * (u.abs() * ea + a.abs() * eu + ea * eu) + tiny
+    # |act''| <= 1 except at relu's corner, where the sign of g is not certain
+    ed = (da.abs() + (g.abs() <= eg).double() + 1) * eg + ACT * scale
+    if act == "relu":
+        ed = torch.where(g.abs() <= eg, torch.ones_like(g), torch.zeros_like(g))
+    edg = dh.abs() * (u.abs() * ed + da.abs() * eu + ed * eu)
+    edg = edg + u16 * (dg.abs() + edg) + tiny
+    edu = dh.abs() * ea
+    edu = edu + u16 * (du.abs() + edu) + tiny
+    dx, dwg, dwu = dg @ wg + du @ wu, dg.t() @ x, du.t() @ x
+    sx = (dg.abs() + edg) @ wg.abs() + (du.abs() + edu) @ wu.abs()
+    tx = edg @ wg.abs() + edu @ wu.abs() + S(2 * F) * sx
+    tg = edg.t() @ x.abs() + S(T) * ((dg.abs() + edg).t() @ x.abs())
+    tu = edu.t() @ x.abs() + S(T) * ((du.abs() + edu).t() @ x.abs())
+    tx, tg, tu = (t + u16 * (v.abs() + t) + tiny for t, v in ((tx, dx), (tg, dwg), (tu, dwu)))
+    return (h, dx, dwg, dwu), (th, tx, tg, tu)
+
+
+def near(got, want, tol, what):
+    assert got.shape == want.shape, (got.shape, want.shape)
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((got.double() - want).abs().max()), float(tol.max()))
+
+
+def run(ctx, x, wg, wu, dh, act):
+    from tenzor_b200 import ops
+    h = ops.gated_linear(ctx, x, wg, wu, act)
+    dx, dwg, dwu = ops.gated_linear_backward(ctx, x, wg, wu, dh, act)
+    torch.cuda.synchronize()
+    ctx.check_status()
+    return h, dx, dwg, dwu
+
+
+def check(ctx, x, wg, wu, dh, act):
+    want, tol = reference(x, wg, wu, dh, act)
+    for g, w, t, n in zip(run(ctx, x, wg, wu, dh, act), want, tol, ("h", "dx", "dw_gate", "dw_up")):
+        near(g, w, t, n)
+
+
+SIZES = [(1, 8, 8), (1, 384, 1536), (2, 64, 72), (3, 2048, 264), (7, 72, 2000), (8, 384, 1536), (9, 40, 8), (16, 1024, 520),
+         (17, 136, 136), (31, 200, 96), (64, 384, 1000), (77, 384, 1000), (127, 128, 128), (128, 8, 264), (129, 64, 384),
+         (256, 256, 512), (300, 1000, 328), (513, 520, 776), (1000, 384, 1536), (4099, 128, 264)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("T,D,F", SIZES)
+def test_sizes(ctx, T, D, F, dt):
+    check(ctx, *make(T, D, F, dt, seed=T + D + F), "silu")
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T", [3, 150])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_activations(ctx, act, T, dt):
+    check(ctx, *make(T, 128, 200, dt, seed=T), act)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T", [4, 140])
+def test_large_gates_saturate(ctx, act, T):
+    """Gates of a few hundred: every activation and derivative reaches its limits without an infinity or NaN."""
+    x, wg, wu, dh = make(T, 64, 96, "bf16", seed=5, wscale=1.0)
+    for o in run(ctx, x, (wg.float() * 300).to(wg.dtype), wu, dh, act):
+        assert torch.isfinite(o).all()
+    if act in ("relu", "sigmoid"):
+        return
+    h = run(ctx, x, (wg.float() * 300).to(wg.dtype), wu, dh, act)[0]
+    g = x.double() @ (wg.float() * 300).to(wg.dtype).double().t()
+    u = x.double() @ wu.double().t()
+    sure = g.abs() > 60
+    want = torch.where(g > 0, g * u, torch.zeros_like(g))
+    assert ((h.double() - want).abs()[sure] <= 2.0 ** -7 * want.abs()[sure] + 1e-3).all()
+
+
+@pytest.mark.parametrize("T", [5, 200])
+def test_strided_rows(ctx, T):
+    x, wg, wu, dh = make(T, 128, 136, "bf16", seed=3)
+    xb = torch.full((T, 128 + 64), float("nan"), device="cuda", dtype=x.dtype)
+    db = torch.full((T, 136 + 8), float("nan"), device="cuda", dtype=x.dtype)
+    xb[:, 64:], db[:, :136] = x, dh
+    check(ctx, xb[:, 64:], wg, wu, db[:, :136], "gelu")
+
+
+@pytest.mark.parametrize("T", [6, 135])
+def test_weights_as_halves_of_one_matrix(ctx, T):
+    x, wg, wu, dh = make(T, 64, 80, "f16", seed=9)
+    w = torch.cat([wg, wu])
+    check(ctx, x, w[:80], w[80:], dh, "silu")
+
+
+@pytest.mark.parametrize("T", [7, 140])
+def test_bad_values_stay_in_their_rows(ctx, T):
+    """A NaN or infinite token spoils its own row of h and dx; the weights' gradients sum over tokens and show it."""
+    x, wg, wu, dh = make(T, 64, 72, "bf16", seed=4)
+    clean = run(ctx, x, wg, wu, dh, "silu")
+    x[2, 5] = float("nan")
+    x[4, 9] = float("inf")
+    h, dx, dwg, dwu = run(ctx, x, wg, wu, dh, "silu")
+    keep = [r for r in range(T) if r not in (2, 4)]
+    assert torch.equal(h[keep], clean[0][keep]) and torch.equal(dx[keep], clean[1][keep])
+    assert torch.isnan(h[2]).all() and torch.isnan(dx[2]).all() and not torch.isfinite(h[4]).any()
+    assert torch.isnan(dwg[:, 5]).all() and torch.isnan(dwu[:, 5]).all()
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_gradient_against_differences(ctx, act):
+    """<dx, v> and <dW, V> against central differences of the 64-bit forward formula."""
+    from tenzor_b200 import ops
+    x, wg, wu, dh = make(70, 72, 88, "f16", seed=21)
+    grads = ops.gated_linear_backward(ctx, x, wg, wu, dh, act)
+    _, (_, *tol) = reference(x, wg, wu, dh, act)
+    base = [t.double() for t in (x, wg, wu)]
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    eps = 1e-5
+
+    def loss(v):
+        return float((act64(act, v[0] @ v[1].t()) * (v[0] @ v[2].t()) * dh.double()).sum())
+
+    for i in range(3):
+        v = torch.randn(base[i].shape, generator=gen, device="cuda", dtype=torch.float64)
+        up, dn = list(base), list(base)
+        up[i], dn[i] = base[i] + eps * v, base[i] - eps * v
+        diff = (loss(up) - loss(dn)) / (2 * eps)
+        bound = float((tol[i] * v.abs()).sum()) + 1e-4  # the differences' own error: eps^2 and 2^-52 / eps
+        if act == "relu":
+            bound += 0.02  # corners crossed within eps
+        assert abs(float((grads[i].double() * v).sum()) - diff) <= bound
+
+
+def test_repeats_are_bit_equal(ctx):
+    a = make(700, 136, 200, "bf16", seed=8)
+    one, two = run(ctx, *a, "gelu"), run(ctx, *a, "gelu")
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+
+
+def test_no_tokens(ctx):
+    from tenzor_b200 import ops
+    x, wg, wu, dh = make(4, 64, 72, "bf16")
+    assert ops.gated_linear(ctx, x[:0], wg, wu).shape == (0, 72)
+    dx, dwg, dwu = ops.gated_linear_backward(ctx, x[:0], wg, wu, dh[:0])
+    assert dx.shape == (0, 64) and not dwg.any() and not dwu.any()
+
+
+def test_other_stream_and_graph(ctx):
+    from tenzor_b200 import ops
+    x, wg, wu, dh = make(300, 128, 136, "f16", seed=6)
+    want = run(ctx, x, wg, wu, dh, "silu")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = (ops.gated_linear(ctx, x, wg, wu), *ops.gated_linear_backward(ctx, x, wg, wu, dh))
+    s.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = (ops.gated_linear(ctx, x, wg, wu), *ops.gated_linear_backward(ctx, x, wg, wu, dh))
+    for t in got:
+        t.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_refusals(ctx):
+    from tenzor_b200 import TenzorError, _lib, ops
+    x, wg, wu, dh = make(4, 64, 72, "bf16")
+    with pytest.raises(TypeError):
+        ops.gated_linear(ctx, x.float(), wg, wu)
+    with pytest.raises(ValueError):
+        ops.gated_linear(ctx, x, wg.half(), wu)
+    with pytest.raises(ValueError):
+        ops.gated_linear(ctx, x, wg, wu[:64])
+    with pytest.raises(ValueError):
+        ops.gated_linear(ctx, x, wg, wu, act="tanh")
+    with pytest.raises(ValueError):
+        ops.gated_linear(ctx, x, wg, wu, out=torch.empty(4, 64, device="cuda", dtype=x.dtype))
+    with pytest.raises(ValueError):
+        ops.gated_linear(ctx, x.t().contiguous().t(), wg, wu)
+    with pytest.raises(ValueError):
+        ops.gated_linear(ctx, x.cpu(), wg, wu)
+    with pytest.raises(ValueError):
+        ops.gated_linear_backward(ctx, x, wg, wu, dh[:2])
+    with pytest.raises(TenzorError) as e:  # a width that is no multiple of 8
+        ops.gated_linear(ctx, x[:, :60].contiguous(), wg[:, :60].contiguous(), wu[:, :60].contiguous())
+    assert e.value.code == _lib.TZ_EINVAL
+    wide = torch.zeros(4, 68, device="cuda", dtype=x.dtype)
+    with pytest.raises(TenzorError):  # a row stride that is no multiple of 8
+        ops.gated_linear(ctx, wide[:, :64], wg, wu)
+    odd = torch.zeros(4 * 64 + 1, device="cuda", dtype=x.dtype)[1:].view(4, 64)
+    with pytest.raises(TenzorError):  # an address that is no multiple of 16 bytes
+        ops.gated_linear(ctx, odd, wg, wu)
+    Lb, p = _lib.lib(), (lambda t: C.c_void_p(t.data_ptr()))
+    assert Lb.tz_gated_linear_backward(ctx.handle, p(x), 64, p(wg), p(wu), p(dh), 72, p(x), p(wg), p(wu), p(x), 1, 4, 64, 72,
+                                       _lib.OP["silu"], 1, None) == _lib.TZ_EINVAL
+    assert "workspace" in Lb.tz_get_last_error().decode()
+    assert Lb.tz_gated_linear(ctx.handle, p(x), 64, p(wg), p(wu), p(dh), 4, 64, 72, _lib.OP["exp"], 1, None) == _lib.TZ_EINVAL
+    assert Lb.tz_gated_linear(ctx.handle, p(x), 64, p(wg), p(wu), p(dh), 4, 64, 72, _lib.OP["silu"], 7, None) == _lib.TZ_EINVAL
+    assert Lb.tz_gated_linear(None, p(x), 64, p(wg), p(wu), p(dh), 4, 64, 72, _lib.OP["silu"], 1, None) == _lib.TZ_EINVAL
