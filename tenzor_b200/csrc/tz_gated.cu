@@ -477,7 +477,7 @@ int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const M
     return launch_cluster(kern, CG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma0, ma1, mb0, mb1, mo0, mo1, p, ctx->d_status);
 }
 
-constexpr int kCG = 1, kBN = 256;
+constexpr int kCG = 2, kBN = 256;
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
