@@ -364,6 +364,41 @@ int tz_gated_linear_backward(tz_ctx_t ctx, const void* x, int64_t ldx, const voi
                              size_t workspace_bytes, int64_t t, int d, int f, int act, int dtype,
                              tz_stream_t stream);
 
+/* ---- microscaled 4-bit floating point (device pointers, async on `stream`) -------------------
+ * MXFP4: 32 consecutive values of a row share a power-of-two scale (E8M0 code, 255 = NaN), each value is
+ * an E2M1 code (0 .5 1 1.5 2 3 4 6 and a sign).  The scale is 2^(floor(log2 max|x|) - 2); values round to
+ * nearest, ties to the even code, and saturate at 6; a block with a NaN or an infinity becomes NaN.
+ *   codes   [rows, cols / 2] bytes, the even column in the low half
+ *   scales  tz_mxfp4_scale_bytes(rows, cols) bytes: chunks of 512 bytes for 128 rows x 4 blocks, chunk
+ *           (r / 128, b / 4) at ((r / 128) * ceil(cols / 128) + b / 4) * 512, byte
+ *           (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 inside it; bytes of absent rows are not written
+ * cols is a multiple of 32, all pointers are 16-byte aligned, row strides keep rows 16-byte aligned.
+ * dtype, x_dtype, y_dtype: TZ_DT_F32, TZ_DT_F16 or TZ_DT_BF16. */
+int64_t tz_mxfp4_scale_bytes(int64_t rows, int cols);
+int tz_quantize_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, void* codes, void* scales,
+                      int64_t rows, int cols, tz_stream_t stream);
+int tz_dequantize_mxfp4(tz_ctx_t ctx, const void* codes, const void* scales, void* out, int dtype, int64_t rows,
+                        int cols, tz_stream_t stream);
+/* Two weight matrices [f, d] as the one operand [2f, d] of tz_gated_linear_mxfp4: 16 rows of w_gate, then
+ * 16 of w_up, and so on; f a multiple of 16. */
+int tz_pack_gated_mxfp4(tz_ctx_t ctx, const void* w_gate, const void* w_up, int dtype, void* codes, void* scales,
+                        int f, int d, tz_stream_t stream);
+/* y [m, n] = a [m, k] w [n, k]^T (+ bias [n], f32 or NULL) of two quantised matrices on the block-scaled
+ * tensor cores (kind::mxf4), f32 accumulation, one rounding to y_dtype; n a multiple of 8. */
+int tz_gemm_mxfp4(tz_ctx_t ctx, const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,
+                  const float* bias, void* y, int y_dtype, int64_t m, int k, int n, tz_stream_t stream);
+/* Device workspace of the two calls below (n = 2f for the gated one). */
+int tz_linear_mxfp4_workspace(tz_ctx_t ctx, int64_t m, int k, int n, size_t* bytes);
+/* y = quantised(x) w^T (+ bias): x [m, k] with row stride ldx is quantised in the call. */
+int tz_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, const void* w_codes, const void* w_scales,
+                    const float* bias, void* y, int y_dtype, void* workspace, size_t workspace_bytes, int64_t m,
+                    int k, int n, tz_stream_t stream);
+/* h [t, f] = act(q wg^T) * (q wu^T), q = quantised(x), weights from tz_pack_gated_mxfp4; x and h of the
+ * 16-bit type `dtype`; act as for tz_gated_linear. */
+int tz_gated_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, const void* w_codes,
+                          const void* w_scales, void* h, int act, void* workspace, size_t workspace_bytes, int64_t t,
+                          int d, int f, tz_stream_t stream);
+
 /* ---- N-D tensor ops of the `.eval()` executor and the ONNX op map ---------------------------
  * Device pointers, asynchronous on `stream`, f32 unless noted. */
 /* Batched matmul with broadcast batch dimensions (evalBatchedMatmul, executor.zig:199-325, and

@@ -41,6 +41,8 @@ EXPORTS = [
     "tz_lenet_load_tenzor", "tz_arctic_load_tenzor", "tz_ew_program_run_nd", "tz_batched_matmul",
     "tz_matmul_f32x3", "tz_reduce_axis", "tz_softmax_axis", "tz_permute", "tz_cast", "tz_concat",
     "tz_gated_linear", "tz_gated_linear_backward", "tz_gated_linear_backward_workspace",
+    "tz_mxfp4_scale_bytes", "tz_quantize_mxfp4", "tz_dequantize_mxfp4", "tz_pack_gated_mxfp4", "tz_gemm_mxfp4",
+    "tz_linear_mxfp4_workspace", "tz_linear_mxfp4", "tz_gated_linear_mxfp4",
 ]
 
 
@@ -179,12 +181,21 @@ def _declare(L):
         "tz_concat": [P, P, P, i, i64, i64, i, P, P],
         "tz_gated_linear": [P, P, i64, P, P, P, i64, i, i, i, i, P],
         "tz_gated_linear_backward_workspace": [P, i64, i, i, C.POINTER(u)],
+        "tz_quantize_mxfp4": [P, P, i64, i, P, P, i64, i, P],
+        "tz_dequantize_mxfp4": [P, P, P, P, i, i64, i, P],
+        "tz_pack_gated_mxfp4": [P, P, P, i, P, P, i, i, P],
+        "tz_gemm_mxfp4": [P, P, P, P, P, P, P, i, i64, i, i, P],
+        "tz_linear_mxfp4_workspace": [P, i64, i, i, C.POINTER(u)],
+        "tz_linear_mxfp4": [P, P, i64, i, P, P, P, P, i, P, u, i64, i, i, P],
+        "tz_gated_linear_mxfp4": [P, P, i64, i, P, P, P, i, P, u, i64, i, i, P],
         "tz_gated_linear_backward": [P, P, i64, P, P, P, i64, P, P, P, P, u, i64, i, i, i, i, P],
     }
     for name, args in sig.items():
         f = getattr(L, name)
         f.argtypes = args
         f.restype = C.c_int
+    L.tz_mxfp4_scale_bytes.argtypes = [i64, i]
+    L.tz_mxfp4_scale_bytes.restype = i64
     L.tz_doc_chunk_count.argtypes = [i64]
     L.tz_doc_chunk_count.restype = i64
     L.tz_tenzor_hash_name.argtypes = [C.c_char_p, u]

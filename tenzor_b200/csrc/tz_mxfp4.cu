@@ -1,0 +1,738 @@
+// tz_mxfp4.cu -- microscaled 4-bit floating point (the OCP MXFP4 format): quantiser, and the product of two
+// quantised matrices on the block-scaled tensor cores, plain or with the gated epilogue.
+//
+// Format: blocks of 32 consecutive values of a row share a scale 2^(code - 127) (E8M0, code 255 = NaN); an
+// element is E2M1: sign and 0 .5 1 1.5 2 3 4 6.  The scale is 2^(floor(log2 max|x|) - 2), so the largest
+// element lands in [4, 8); elements round to nearest, ties to the even code, and saturate at 6.  A block that
+// holds a NaN or an infinity gets the NaN scale.
+//
+// Memory: element codes [rows, cols / 2], two per byte, the even column in the low half.  Scale codes in
+// 512-byte chunks of 128 rows x 4 blocks, chunk (r / 128, b / 4) at ((r / 128) * ceil(cols / 128) + b / 4) * 512,
+// byte (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 inside it: the order in which the tensor core's scale
+// operand lies in TMEM (lane r % 32, column r / 32, four blocks per 32-bit word), so that one tcgen05.cp moves
+// a chunk from shared memory without a rearrangement.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "tz_act.cuh"
+#include "tz_internal.h"
+#include "tz_pair.cuh"
+
+namespace tz {
+namespace {
+
+constexpr int DT_F32 = TZ_DT_F32, DT_F16 = TZ_DT_F16, DT_BF16 = TZ_DT_BF16;
+
+__host__ __device__ __forceinline__ long long sf_chunk(long long row_block, int k_chunk, int k_chunks) {
+    return (row_block * k_chunks + k_chunk) * 512;
+}
+
+// ---- quantiser -------------------------------------------------------------------------------------
+template <int DT>
+struct Elem;
+template <>
+struct Elem<DT_F32> { using T = float; };
+template <>
+struct Elem<DT_F16> { using T = __half; };
+template <>
+struct Elem<DT_BF16> { using T = __nv_bfloat16; };
+
+// 8 consecutive values as f32.
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, long long i, float (&v)[8]) {
+    if constexpr (DT == DT_F32) {
+        const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+        const float4 a = __ldg(s), b = __ldg(s + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i));
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 f;
+            if constexpr (DT == DT_BF16)
+                f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+            else
+                f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        }
+    }
+}
+
+// Eight values to eight E2M1 codes (value j in bits 4j .. 4j+3).
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8], float inv) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv),
+          "f"(v[7] * inv));
+    return r;
+}
+
+// Quantises a block spread over 4 neighbouring lanes (8 values each); returns the codes, `sc` the scale code.
+__device__ __forceinline__ uint32_t quant_block(const float (&v)[8], uint32_t& sc) {
+    // The largest bit pattern of |x|: orders like the value, and an infinity or NaN stays on top.
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    const uint32_t e = top >> 23;  // floor(log2) + 127; 0 for subnormals, whose scale is the smallest anyway
+    sc = e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+    return e2m1x8(v, __uint_as_float((254u - (e == 255u ? 0u : sc)) << 23));
+}
+
+// One lane quantises 8 values at a time; 4 lanes make a block and 16 lanes the four scale codes of one word.
+// A warp takes 256 columns of a row per step.  Memory-bound: 2 (or 4) bytes read, 0.53 written per value.
+// Row r of x becomes row `map(r)` of the result: r, or with GROUP > 0 row (r / GROUP) * 2 GROUP + r % GROUP +
+// off, which interleaves two matrices in groups of GROUP rows.
+template <int DT, int GROUP>
+__global__ void __launch_bounds__(256) quantize_mxfp4_kernel(const void* x, long long ldx, uint8_t* codes, uint8_t* scales, long long rows,
+                                                             int cols, int off) {
+    tzp::pdl_trigger();
+    tzp::pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int k_chunks = (cols + 127) / 128;
+    const int steps = (cols + 255) / 256;
+    const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
+    const long long total = rows * steps;
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += warps) {
+        const long long r = i / steps;
+        const int c = static_cast<int>(i - r * steps) * 256 + lane * 8;
+        const bool in = c < cols;
+        float v[8] = {};
+        if (in) load8<DT>(x, r * ldx + c, v);
+        uint32_t sc;
+        const uint32_t q = quant_block(v, sc);
+        const long long ro = GROUP > 0 ? (r / GROUP) * (2 * GROUP) + r % GROUP + off : r;
+        if (in) *reinterpret_cast<uint32_t*>(codes + (ro * cols + c) / 2) = q;
+        // lanes 0, 4, 8, 12 of each half warp hold the word's four bytes (0 for blocks past the row's end)
+        uint32_t w = in ? sc << (8 * ((lane >> 2) & 3)) : 0u;
+        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
+        if (in && (lane & 15) == 0)
+            *reinterpret_cast<uint32_t*>(scales + sf_chunk(ro >> 7, c >> 7, k_chunks) + (ro & 31) * 16 + ((ro & 127) >> 5) * 4) = w;
+    }
+}
+
+// 2^(code - 127) in f32 (code 0 is the subnormal 2^-127, 255 a NaN).
+__device__ __forceinline__ float e8m0(uint32_t code) {
+    return __uint_as_float(code == 255u ? 0x7FC00000u : code == 0u ? 0x00400000u : code << 23);
+}
+
+// Two E2M1 codes (low nibble first) as f32.
+__device__ __forceinline__ float2 e2m1x2(uint32_t byte) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 t, u;\n\t.reg .b16 s;\n\tcvt.u16.u32 s, %1;\n\tmov.b16 {t, u}, s;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(byte));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) dequantize_mxfp4_kernel(const uint8_t* codes, const uint8_t* scales, void* out, long long rows, int cols) {
+    tzp::pdl_trigger();
+    tzp::pdl_wait();
+    const int k_chunks = (cols + 127) / 128;
+    const long long n8 = rows * (cols / 8);
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n8; i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const long long r = i / (cols / 8);
+        const int c = static_cast<int>(i - r * (cols / 8)) * 8;
+        const uint32_t q = __ldg(reinterpret_cast<const uint32_t*>(codes) + i);
+        const float s = e8m0(__ldg(scales + sf_chunk(r >> 7, c >> 7, k_chunks) + (r & 31) * 16 + ((r & 127) >> 5) * 4 + ((c >> 5) & 3)));
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = e2m1x2((q >> (8 * j)) & 255u);
+            v[2 * j] = f.x * s, v[2 * j + 1] = f.y * s;
+        }
+        if constexpr (DT == DT_F32) {
+            float4* o = reinterpret_cast<float4*>(out) + 2 * i;
+            o[0] = make_float4(v[0], v[1], v[2], v[3]);
+            o[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            constexpr bool BF = DT == DT_BF16;
+            reinterpret_cast<uint4*>(out)[i] = make_uint4(tzp::pack16x2<BF>(v[0], v[1]), tzp::pack16x2<BF>(v[2], v[3]),
+                                                          tzp::pack16x2<BF>(v[4], v[5]), tzp::pack16x2<BF>(v[6], v[7]));
+        }
+    }
+}
+
+// ---- block-scaled product --------------------------------------------------------------------------
+// y = q(x) q(W)^T (+ bias), or with GATED the gated form of interleaved weights: W rows come as 16 gate rows,
+// 16 up rows, and so on, so a 32-column chunk of the accumulator holds the gate and the up values of 16 outputs.
+//
+// The structure of the 16-bit gated kernel (persistent, TMA producer, MMA issuer, 8 epilogue warps, two
+// accumulators, CTA pairs).  A K block is 128 bytes = 256 values: four MMAs of 64.  Its scales arrive by bulk
+// copies (2 chunks for the CTA's 128 rows of A, up to 4 for the columns' rows of W: both CTAs of a pair keep
+// all of them) and go to TMEM by tcgen05.cp, each stage to its own 24 columns: a stage's scales are only
+// replaced once its MMAs have completed.  BN = 192 leaves TMEM for that: 2 x 192 + 24 x stages <= 512 columns.
+constexpr int GROUP = 16;
+
+struct MxParams {
+    int m_tiles, n_tiles;
+    int rows, n;        // of the output before the gate
+    int k_chunks;       // scale chunks per row block
+    int k;              // values
+    int a_blocks, b_blocks;  // 128-row blocks of the scales
+    const uint8_t* sfa;
+    const uint8_t* sfb;
+    const float* bias;
+    int act;
+};
+
+template <int CG>
+struct MxCfg {
+    static constexpr int BN = 192;
+    static constexpr int EPI = 8;
+    static constexpr int THREADS = 64 + 32 * EPI;
+    static constexpr int BNC = BN / CG;
+    static constexpr int A_BYTES = 128 * 128;
+    static constexpr int B_BYTES = BNC * 128;
+    static constexpr int SF_BYTES = 3072;  // A: 2 chunks; B: 2 row blocks x 2 chunks
+    static constexpr int STAGE = A_BYTES + B_BYTES + SF_BYTES;
+    static constexpr int STAGING = EPI * 4096;
+    static constexpr int STAGES = CG == 2 ? 5 : 4;
+    static constexpr int SF_COLS = 24;
+    static constexpr int SF0 = 2 * BN;
+    static constexpr int SMEM = STAGES * STAGE + STAGING + 512 + 1024;
+    static_assert(SF0 + STAGES * SF_COLS <= 512, "TMEM");
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+    static_assert(STAGE % 1024 == 0, "swizzle atoms");
+};
+
+// kind::mxf4 instruction descriptor: E2M1 operands (1), E8M0 scales (bit 23), K-major, scale ids of A and B.
+__host__ __device__ constexpr uint32_t mx_idesc(uint32_t M, uint32_t N, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | ((M >> 4) << 24) | (sf_id << 29);
+}
+
+template <int CG>
+__device__ __forceinline__ void mx_mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+
+// One 512-byte scale chunk (32 rows of 16 bytes) to 4 TMEM columns, repeated in the four lane quarters.
+template <int CG>
+__device__ __forceinline__ void sf_copy(uint32_t taddr, uint32_t smem_addr) {
+    uint64_t d = 0;  // no swizzle: 8-row groups 128 bytes apart
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(128 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+// Bulk copy into this CTA's shared memory, counted on the barrier at cluster address `bar`.
+__device__ __forceinline__ void bulk_load_bar(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+template <int CG, int OUT, bool GATED>
+__global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
+    mxfp4_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO,
+                    const MxParams p, int* status) {
+    using C = MxCfg<CG>;
+    constexpr int STAGES = C::STAGES, BN = C::BN;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = tzp::smem_u32(smem_raw);
+    uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+    uint8_t* staging = smem + STAGES * C::STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? tzp::cluster_ctarank() : 0u;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tzp::mbar_init(&full[s], 1);
+            tzp::mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            tzp::mbar_init(&tfull[a], 1);
+            tzp::mbar_init(&tempty[a], C::EPI * CG);
+        }
+        tzp::mbar_init(drain, 1);
+        *abort_flag = 0;
+        tzp::fence_mbar_init();
+        tzp::tma_prefetch_desc(&tmA);
+        tzp::tma_prefetch_desc(&tmB);
+    }
+    if (warp == 1) tzp::pair_tmem_alloc<CG>(tmem_slot, 512);
+    tzp::tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) tzp::cluster_sync();
+    tzp::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    tzp::pdl_trigger();
+    tzp::pdl_wait();
+
+    const int num_tiles = p.m_tiles * p.n_tiles;
+    const int kblocks = (p.k + 255) / 256;
+    auto tile_of = [&](int t, int& m, int& n) {  // groups of 8 row blocks walk the column blocks together
+        constexpr int GM = 8;
+        const int grp = t / (GM * p.n_tiles);
+        const int gm = min(GM, p.m_tiles - grp * GM);
+        t -= grp * GM * p.n_tiles;
+        m = grp * GM + t % gm;
+        n = t / gm;
+    };
+    const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---- TMA producer ----
+            int stage = 0;
+            uint32_t phase = 0, armed = 0, armed_par = 0;
+            bool ok = true;
+            for (int t = t0; ok && t < num_tiles; t += tstep) {
+                int m, n;
+                tile_of(t, m, n);
+                const int mb = m * CG + static_cast<int>(rank);
+                const int nb = n * BN / 128;
+                const uint8_t* sa_g = p.sfa + sf_chunk(min(mb, p.a_blocks - 1), 0, p.k_chunks);
+                const uint8_t* sb_g0 = p.sfb + sf_chunk(nb, 0, p.k_chunks);
+                const uint8_t* sb_g1 = p.sfb + sf_chunk(min(nb + 1, p.b_blocks - 1), 0, p.k_chunks);
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!tzp::pair_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t sfb = 2 * kb + 1 < p.k_chunks ? 1024u : 512u;  // the last K block may hold one chunk
+                    if (rank == 0) {
+                        tzp::mbar_arrive_expect_tx(&full[stage], CG * (C::A_BYTES + C::B_BYTES + 3 * sfb));
+                        armed |= 1u << stage;
+                        armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
+                    }
+                    const uint32_t bar = CG == 2 ? tzp::mapa(&full[stage], 0) : tzp::smem_u32(&full[stage]);
+                    const uint32_t sa = tzp::smem_u32(smem + stage * C::STAGE);
+                    const uint32_t sb = sa + C::A_BYTES, sf = sb + C::B_BYTES;
+                    tzp::pair_load_2d<CG>(sa, &tmA, kb * 128, mb * 128, bar);
+                    tzp::pair_load_2d<CG>(sb, &tmB, kb * 128, n * BN + static_cast<int>(rank) * C::BNC, bar);
+                    bulk_load_bar(sf, sa_g + kb * 1024ll, sfb, bar);
+                    bulk_load_bar(sf + 1024, sb_g0 + kb * 1024ll, sfb, bar);
+                    bulk_load_bar(sf + 2048, sb_g1 + kb * 1024ll, sfb, bar);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            for (int s = 0; s < STAGES; ++s)  // every copy has landed before the CTA can exit (bounded)
+                if (armed & (1u << s)) tzp::pair_wait<CG>(&full[s], (armed_par >> s) & 1u, status, nullptr);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            // ---- MMA issuer ----
+            constexpr uint32_t idesc0 = mx_idesc(128 * CG, BN, 0), idesc2 = mx_idesc(128 * CG, BN, 2);
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int t = t0; ok && t < num_tiles; t += tstep) {
+                int m, n;
+                tile_of(t, m, n);
+                if (!tzp::pair_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
+                tzp::tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                const uint32_t boff = static_cast<uint32_t>((n * BN & 127) / 32);  // the tile's first row inside its scale chunk
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!tzp::pair_wait<CG>(&full[stage], phase, status, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tzp::tc_fence_after();
+                    const uint32_t sa = tzp::smem_u32(smem + stage * C::STAGE);
+                    const uint32_t sf = sa + C::A_BYTES + C::B_BYTES;
+                    const uint32_t tsf = tmem_base + static_cast<uint32_t>(C::SF0 + stage * C::SF_COLS);
+                    const int left = p.k - kb * 256;
+                    // TMEM columns of the stage: A chunk 0 (4), A chunk 1 (4), B chunk 0 (8), B chunk 1 (8)
+                    sf_copy<CG>(tsf, sf);
+                    sf_copy<CG>(tsf + 8, sf + 1024);
+                    sf_copy<CG>(tsf + 12, sf + 2048);
+                    if (left > 128) {
+                        sf_copy<CG>(tsf + 4, sf + 512);
+                        sf_copy<CG>(tsf + 16, sf + 1536);
+                        sf_copy<CG>(tsf + 20, sf + 2560);
+                    }
+                    const uint64_t ad = tzp::sdesc_k128(sa), bd = tzp::sdesc_k128(sa + C::A_BYTES);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (k == 0 || left > 64 * k)
+                            mx_mma<CG>(d, ad + 2u * k, bd + 2u * k, (k & 1) ? idesc2 : idesc0, tsf + 4 * (k >> 1), tsf + 8 + 8 * (k >> 1) + boff,
+                                       (kb | k) != 0 ? 1u : 0u);
+                    tzp::pair_commit<CG>(&empty[stage]);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                tzp::pair_commit<CG>(&tfull[acc]);
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+            tzp::pair_commit<CG>(drain);
+            tzp::pair_wait<CG>(drain, 0, status, nullptr);
+        }
+    } else {
+        // ---- epilogue: TMEM lane quarter (warp % 4), half of the columns, in chunks of 32 ----
+        const int e = warp - 2, q4 = warp & 3, hf = e >> 2;
+        const uint32_t box = tzp::smem_u32(staging) + static_cast<uint32_t>(e * 4096);
+        uint8_t* boxp = staging + e * 4096;
+        int acc = 0, nb = 0;
+        uint32_t acc_phase = 0;
+        for (int t = t0; t < num_tiles; t += tstep) {
+            int m, n;
+            tile_of(t, m, n);
+            if (!tzp::pair_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
+            tzp::tc_fence_after();
+            const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN);
+            const int row0 = (m * CG + static_cast<int>(rank)) * 128 + q4 * 32;
+#pragma unroll 1
+            for (int c = 0; c < BN / 64; ++c) {
+                const int cc = (hf * (BN / 64) + c) * 32;
+                const int col0 = n * BN + cc;
+                if (col0 >= p.n) break;
+                uint32_t v[32];
+                tzp::tmem_ld32(td + cc, v);
+                tzp::tmem_ld_wait();
+                if constexpr (GATED) {
+                    uint32_t o[8];
+#define TZ_G(A)                                                                                              \
+    for (int j = 0; j < 8; ++j) {                                                                            \
+        float d_;                                                                                            \
+        const float a_ = gated_act<A, false>(__uint_as_float(v[2 * j]), d_) * __uint_as_float(v[16 + 2 * j]); \
+        const float b_ = gated_act<A, false>(__uint_as_float(v[2 * j + 1]), d_) * __uint_as_float(v[17 + 2 * j]); \
+        o[j] = tzp::pack16x2<OUT == DT_BF16>(a_, b_);                                                        \
+    }
+                    switch (p.act) {
+                        case TZ_OP_SILU: _Pragma("unroll") TZ_G(TZ_OP_SILU) break;
+                        case TZ_OP_GELU: _Pragma("unroll") TZ_G(TZ_OP_GELU) break;
+                        case TZ_OP_GELU_ERF: _Pragma("unroll") TZ_G(TZ_OP_GELU_ERF) break;
+                        case TZ_OP_RELU: _Pragma("unroll") TZ_G(TZ_OP_RELU) break;
+                        default: _Pragma("unroll") TZ_G(TZ_OP_SIGMOID) break;
+                    }
+#undef TZ_G
+                    if (lane == 0) tzp::bulk_wait_read<1>();
+                    __syncwarp();
+                    const uint32_t b = box + nb * 1024 + lane * 32;  // 32-byte rows, 32-byte swizzle
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        tzp::st_shared_v4(b + ((u ^ ((lane >> 2) & 1)) << 4), o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                    tzp::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tzp::tma_store_2d(&tmO, boxp + nb * 1024, col0 / 2, row0);
+                        tzp::bulk_commit();
+                    }
+                    nb ^= 1;
+                } else {
+                    if (p.bias) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            if (col0 + j < p.n) {  // n is a multiple of 8
+                                const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + col0 + j));
+                                v[j] = __float_as_uint(__uint_as_float(v[j]) + b4.x);
+                                v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + b4.y);
+                                v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) + b4.z);
+                                v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) + b4.w);
+                            }
+                        }
+                    }
+                    if constexpr (OUT == DT_F32) {
+                        if (lane == 0) tzp::bulk_wait_read<0>();
+                        __syncwarp();
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            tzp::st_shared_v4(box + lane * 128 + ((u ^ (lane & 7)) << 4), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+                        tzp::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tzp::tma_store_2d(&tmO, boxp, col0, row0);
+                            tzp::bulk_commit();
+                        }
+                    } else {
+                        uint32_t o[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            o[j] = tzp::pack16x2<OUT == DT_BF16>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                        if (lane == 0) tzp::bulk_wait_read<1>();
+                        __syncwarp();
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            tzp::st_shared_v4(box + nb * 2048 + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4), o[4 * u], o[4 * u + 1], o[4 * u + 2],
+                                              o[4 * u + 3]);
+                        tzp::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tzp::tma_store_2d(&tmO, boxp + nb * 2048, col0, row0);
+                            tzp::bulk_commit();
+                        }
+                        nb ^= 1;
+                    }
+                }
+            }
+            tzp::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2)
+                    tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
+                else
+                    tzp::mbar_arrive(&tempty[acc]);
+            }
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        if (lane == 0) tzp::bulk_wait_all();
+    }
+
+    tzp::tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) tzp::cluster_sync();
+    if (warp == 1) {
+        __syncwarp();
+        tzp::tc_fence_after();
+        tzp::pair_tmem_dealloc<CG>(tmem_base, 512);
+    }
+}
+
+constexpr int kCG = 1;
+
+int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+struct Q4 {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    int64_t rows;
+};
+
+template <int OUT, bool GATED>
+int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, void* y, int act, cudaStream_t s) {
+    using C = MxCfg<kCG>;
+    auto kern = mxfp4_mm_kernel<kCG, OUT, GATED>;
+    static std::atomic<unsigned> done{0};
+    int rc = ensure_smem(kern, C::SMEM, done);
+    if (rc) return rc;
+    CUtensorMap ma, mb, mo;
+    const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B;
+    if ((rc = encode_tmap_2d_swz(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.codes, k / 2, a.rows, k / 2, 128, 128, S128))) return rc;
+    if ((rc = encode_tmap_2d_swz(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b.codes, k / 2, b.rows, k / 2, 128, C::BNC, S128))) return rc;
+    const int64_t cols = GATED ? b.rows / 2 : b.rows;
+    if (OUT == DT_F32)
+        rc = encode_tmap_2d_swz(&mo, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, y, cols, a.rows, cols * 4, 32, 32, S128);
+    else
+        rc = encode_tmap_2d_swz(&mo, OUT == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, y, cols, a.rows,
+                                cols * 2, GATED ? 16 : 32, 32, GATED ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc) return rc;
+    MxParams p{};
+    p.m_tiles = ceil_div(a.rows, 128 * kCG);
+    p.n_tiles = ceil_div(b.rows, C::BN);
+    p.rows = static_cast<int>(a.rows);
+    p.n = static_cast<int>(b.rows);
+    p.k = k;
+    p.k_chunks = ceil_div(k, 128);
+    p.a_blocks = ceil_div(a.rows, 128);
+    p.b_blocks = ceil_div(b.rows, 128);
+    p.sfa = a.scales;
+    p.sfb = b.scales;
+    p.bias = bias;
+    p.act = act;
+    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+    const int groups = (ctx->sm_count - ctx->sm_reserve) / kCG;
+    const int grid = static_cast<int>(tiles < groups ? tiles : groups) * kCG;
+    TZ_CHECK(grid > 0, TZ_EINVAL, "mxfp4 kernels need %d free SMs", kCG);
+    return launch_cluster(kern, kCG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma, mb, mo, p, ctx->d_status);
+}
+
+template <int DT, int G>
+int launch_quant(tz_ctx_t ctx, const void* x, int64_t ldx, void* codes, void* scales, int64_t rows, int cols, int off, cudaStream_t s) {
+    const long long warps = rows * ceil_div(cols, 256);
+    const long long want = (warps + 7) / 8, most = static_cast<long long>(ctx->sm_count) * 8 * 4;
+    return launch_kernel(quantize_mxfp4_kernel<DT, G>, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, s, true, x,
+                         static_cast<long long>(ldx), static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), static_cast<long long>(rows),
+                         cols, off);
+}
+template <int G>
+int quant_any(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, void* codes, void* scales, int64_t rows, int cols, int off, cudaStream_t s) {
+    if (dtype == DT_F32) return launch_quant<DT_F32, G>(ctx, x, ldx, codes, scales, rows, cols, off, s);
+    if (dtype == DT_F16) return launch_quant<DT_F16, G>(ctx, x, ldx, codes, scales, rows, cols, off, s);
+    return launch_quant<DT_BF16, G>(ctx, x, ldx, codes, scales, rows, cols, off, s);
+}
+
+size_t a256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+size_t code_bytes(int64_t rows, int cols) { return static_cast<size_t>(rows) * (cols / 2); }
+size_t scale_bytes(int64_t rows, int cols) { return static_cast<size_t>((rows + 127) / 128) * ((cols + 127) / 128) * 512; }
+bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check_dims(const char* fn, int64_t rows, int cols) {
+    TZ_CHECK(rows >= 0 && rows <= (1 << 30) && cols > 0 && cols <= (1 << 24), TZ_EINVAL, "%s: bad sizes (%lld rows, %d values)", fn,
+             static_cast<long long>(rows), cols);
+    TZ_CHECK(cols % 32 == 0, TZ_EINVAL, "%s: the row length must be a multiple of 32 (%d)", fn, cols);
+    return TZ_OK;
+}
+int check_dt(const char* fn, int dtype, bool f32_ok) {
+    TZ_CHECK(dtype == DT_F16 || dtype == DT_BF16 || (f32_ok && dtype == DT_F32), TZ_EINVAL, "%s: unsupported dtype %d", fn, dtype);
+    return TZ_OK;
+}
+int check_rows(const char* fn, const void* x, int64_t ldx, int cols, int dtype) {
+    const int al = dtype == DT_F32 ? 4 : 8;
+    TZ_CHECK(ldx >= cols && ldx % al == 0, TZ_EINVAL, "%s: row stride %lld (at least the row length, 16-byte rows)", fn, static_cast<long long>(ldx));
+    TZ_CHECK(al16(x), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    return TZ_OK;
+}
+
+int product(tz_ctx_t ctx, const char* fn, const Q4& a, const Q4& w, int k, const float* bias, void* y, int y_dtype, cudaStream_t s) {
+    TZ_CHECK(w.rows % 8 == 0, TZ_EINVAL, "%s: n must be a multiple of 8 (%lld)", fn, static_cast<long long>(w.rows));
+    TZ_CHECK(al16(a.codes) && al16(a.scales) && al16(w.codes) && al16(w.scales) && al16(bias) && al16(y), TZ_EINVAL,
+             "%s: pointers must be 16-byte aligned", fn);
+    if (y_dtype == DT_F32) return launch_mx<DT_F32, false>(ctx, a, w, k, bias, y, 0, s);
+    if (y_dtype == DT_F16) return launch_mx<DT_F16, false>(ctx, a, w, k, bias, y, 0, s);
+    return launch_mx<DT_BF16, false>(ctx, a, w, k, bias, y, 0, s);
+}
+
+}  // namespace
+}  // namespace tz
+
+using namespace tz;
+
+extern "C" {
+
+int64_t tz_mxfp4_scale_bytes(int64_t rows, int cols) { return rows < 0 || cols <= 0 ? 0 : static_cast<int64_t>(scale_bytes(rows, cols)); }
+
+int tz_quantize_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, void* codes, void* scales, int64_t rows, int cols, tz_stream_t stream) {
+    const char* fn = "tz_quantize_mxfp4";
+    TZ_CHECK(ctx, TZ_EINVAL, "%s: null context", fn);
+    int rc;
+    if ((rc = check_dims(fn, rows, cols)) || (rc = check_dt(fn, dtype, true))) return rc;
+    if (rows == 0) return TZ_OK;
+    TZ_CHECK(x && codes && scales, TZ_EINVAL, "%s: null pointer", fn);
+    if ((rc = check_rows(fn, x, ldx, cols, dtype))) return rc;
+    TZ_CHECK(al16(codes) && al16(scales), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    return quant_any<0>(ctx, x, ldx, dtype, codes, scales, rows, cols, 0, pick_stream(ctx, stream));
+}
+
+int tz_dequantize_mxfp4(tz_ctx_t ctx, const void* codes, const void* scales, void* out, int dtype, int64_t rows, int cols, tz_stream_t stream) {
+    const char* fn = "tz_dequantize_mxfp4";
+    TZ_CHECK(ctx, TZ_EINVAL, "%s: null context", fn);
+    int rc;
+    if ((rc = check_dims(fn, rows, cols)) || (rc = check_dt(fn, dtype, true))) return rc;
+    if (rows == 0) return TZ_OK;
+    TZ_CHECK(codes && scales && out, TZ_EINVAL, "%s: null pointer", fn);
+    TZ_CHECK(al16(codes) && al16(scales) && al16(out), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    const long long n8 = rows * (cols / 8), want = (n8 + 255) / 256, most = static_cast<long long>(ctx->sm_count) * 32;
+    const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+    auto* kern = dtype == DT_F32 ? dequantize_mxfp4_kernel<DT_F32> : dtype == DT_F16 ? dequantize_mxfp4_kernel<DT_F16> : dequantize_mxfp4_kernel<DT_BF16>;
+    return launch_kernel(kern, grid, dim3(256), 0, pick_stream(ctx, stream), true, static_cast<const uint8_t*>(codes),
+                         static_cast<const uint8_t*>(scales), out, static_cast<long long>(rows), cols);
+}
+
+int tz_pack_gated_mxfp4(tz_ctx_t ctx, const void* w_gate, const void* w_up, int dtype, void* codes, void* scales, int f, int d, tz_stream_t stream) {
+    const char* fn = "tz_pack_gated_mxfp4";
+    TZ_CHECK(ctx && w_gate && w_up && codes && scales, TZ_EINVAL, "%s: null pointer", fn);
+    int rc;
+    if ((rc = check_dims(fn, f, d)) || (rc = check_dt(fn, dtype, true))) return rc;
+    TZ_CHECK(f > 0 && f % GROUP == 0 && f <= (1 << 24), TZ_EINVAL, "%s: f must be a positive multiple of 16 (%d)", fn, f);
+    if ((rc = check_rows(fn, w_gate, d, d, dtype)) || (rc = check_rows(fn, w_up, d, d, dtype))) return rc;
+    TZ_CHECK(al16(codes) && al16(scales), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    cudaStream_t s = pick_stream(ctx, stream);
+    if ((rc = quant_any<GROUP>(ctx, w_gate, d, dtype, codes, scales, f, d, 0, s))) return rc;
+    return quant_any<GROUP>(ctx, w_up, d, dtype, codes, scales, f, d, GROUP, s);
+}
+
+int tz_gemm_mxfp4(tz_ctx_t ctx, const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales, const float* bias, void* y,
+                  int y_dtype, int64_t m, int k, int n, tz_stream_t stream) {
+    const char* fn = "tz_gemm_mxfp4";
+    TZ_CHECK(ctx, TZ_EINVAL, "%s: null context", fn);
+    int rc;
+    if ((rc = check_dims(fn, m, k)) || (rc = check_dims(fn, n, k)) || (rc = check_dt(fn, y_dtype, true))) return rc;
+    TZ_CHECK(n > 0, TZ_EINVAL, "%s: n must be positive", fn);
+    if (m == 0) return TZ_OK;
+    TZ_CHECK(a_codes && a_scales && w_codes && w_scales && y, TZ_EINVAL, "%s: null pointer", fn);
+    return product(ctx, fn, {static_cast<const uint8_t*>(a_codes), static_cast<const uint8_t*>(a_scales), m},
+                   {static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), n}, k, bias, y, y_dtype, pick_stream(ctx, stream));
+}
+
+int tz_linear_mxfp4_workspace(tz_ctx_t ctx, int64_t m, int k, int n, size_t* bytes) {
+    const char* fn = "tz_linear_mxfp4_workspace";
+    TZ_CHECK(ctx && bytes, TZ_EINVAL, "%s: null argument", fn);
+    int rc;
+    if ((rc = check_dims(fn, m, k)) || (rc = check_dims(fn, n, k))) return rc;
+    *bytes = a256(code_bytes(m, k)) + a256(scale_bytes(m, k));
+    return TZ_OK;
+}
+
+static int quantize_input(tz_ctx_t ctx, const char* fn, const void* x, int64_t ldx, int x_dtype, void* ws, size_t ws_bytes, int64_t m, int k, int n,
+                          cudaStream_t s, Q4* out) {
+    size_t need = 0;
+    int rc = tz_linear_mxfp4_workspace(ctx, m, k, n, &need);
+    if (rc) return rc;
+    TZ_CHECK(ws && al16(ws) && ws_bytes >= need, TZ_EINVAL, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", fn, ws_bytes, need);
+    if ((rc = check_rows(fn, x, ldx, k, x_dtype))) return rc;
+    uint8_t* codes = static_cast<uint8_t*>(ws);
+    uint8_t* scales = codes + a256(code_bytes(m, k));
+    *out = {codes, scales, m};
+    return quant_any<0>(ctx, x, ldx, x_dtype, codes, scales, m, k, 0, s);
+}
+
+int tz_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, const void* w_codes, const void* w_scales, const float* bias, void* y,
+                    int y_dtype, void* workspace, size_t workspace_bytes, int64_t m, int k, int n, tz_stream_t stream) {
+    const char* fn = "tz_linear_mxfp4";
+    TZ_CHECK(ctx, TZ_EINVAL, "%s: null context", fn);
+    int rc;
+    if ((rc = check_dims(fn, m, k)) || (rc = check_dims(fn, n, k)) || (rc = check_dt(fn, x_dtype, true)) || (rc = check_dt(fn, y_dtype, true))) return rc;
+    TZ_CHECK(n > 0 && n % 8 == 0, TZ_EINVAL, "%s: n must be a positive multiple of 8 (%d)", fn, n);
+    if (m == 0) return TZ_OK;
+    TZ_CHECK(x && w_codes && w_scales && y, TZ_EINVAL, "%s: null pointer", fn);
+    cudaStream_t s = pick_stream(ctx, stream);
+    Q4 a;
+    if ((rc = quantize_input(ctx, fn, x, ldx, x_dtype, workspace, workspace_bytes, m, k, n, s, &a))) return rc;
+    return product(ctx, fn, a, {static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), n}, k, bias, y, y_dtype, s);
+}
+
+int tz_gated_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, const void* w_codes, const void* w_scales, void* h, int act,
+                          void* workspace, size_t workspace_bytes, int64_t t, int d, int f, tz_stream_t stream) {
+    const char* fn = "tz_gated_linear_mxfp4";
+    TZ_CHECK(ctx, TZ_EINVAL, "%s: null context", fn);
+    int rc;
+    if ((rc = check_dims(fn, t, d)) || (rc = check_dt(fn, dtype, false))) return rc;
+    TZ_CHECK(gated_act_ok(act), TZ_EINVAL, "%s: activation %d is not silu, gelu, gelu_erf, relu or sigmoid", fn, act);
+    TZ_CHECK(f > 0 && f % GROUP == 0 && f <= (1 << 24), TZ_EINVAL, "%s: f must be a positive multiple of 16 (%d)", fn, f);
+    if (t == 0) return TZ_OK;
+    TZ_CHECK(x && w_codes && w_scales && h, TZ_EINVAL, "%s: null pointer", fn);
+    TZ_CHECK(al16(w_codes) && al16(w_scales) && al16(h), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    cudaStream_t s = pick_stream(ctx, stream);
+    Q4 a;
+    if ((rc = quantize_input(ctx, fn, x, ldx, dtype, workspace, workspace_bytes, t, d, 2 * f, s, &a))) return rc;
+    const Q4 w{static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), 2ll * f};
+    return dtype == DT_F16 ? launch_mx<DT_F16, true>(ctx, a, w, d, nullptr, h, act, s) : launch_mx<DT_BF16, true>(ctx, a, w, d, nullptr, h, act, s);
+}
+
+}  // extern "C"

@@ -9,6 +9,8 @@ every computation runs in libtenzor_cuda.so).  Names follow the reference kernel
   ew_unary_chain        codegen.zig:15-74             reduce              codegen.zig:151-205
   gather_rows           gather.zig:15-57
 Gated feed-forward block (no counterpart in the reference): gated_linear, gated_linear_backward.
+Microscaled 4-bit floating point (no counterpart): quantize_mxfp4, dequantize_mxfp4, linear_mxfp4,
+pack_gated_mxfp4, gated_linear_mxfp4.
 N-D forms (executor.zig / onnx/executor.zig): batched_matmul, matmul_f32x3, reduce_axis, softmax_axis,
 permute, cast, concat.
 """
@@ -356,3 +358,128 @@ def gated_linear_backward(ctx: Context, x, w_gate, w_up, dh, act: str = "silu"):
     L.check(L.lib().tz_gated_linear_backward(ctx.handle, _p(x), ldx, _p(w_gate), _p(w_up), _p(dh), lddh, _p(dx), _p(dwg),
                                              _p(dwu), _p(ws), need.value, T, D, F, code, dt, _stream()))
     return dx, dwg, dwu
+
+
+# ---- microscaled 4-bit floating point --------------------------------------------------------------
+_DTF = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # TZ_DT_*
+
+
+class Mxfp4:
+    """A matrix [rows, cols] in MXFP4 on the device: `codes` [rows, cols / 2] and the tiled `scales` (layout in
+    tenzor_cuda.h).  With `gated` the rows are two weight matrices interleaved by pack_gated_mxfp4."""
+
+    __slots__ = ("codes", "scales", "rows", "cols", "gated")
+
+    def __init__(self, rows, cols, device, gated=False):
+        self.rows, self.cols, self.gated = rows, cols, gated
+        self.codes = torch.empty((rows, cols // 2), device=device, dtype=torch.uint8)
+        self.scales = torch.empty(L.lib().tz_mxfp4_scale_bytes(rows, cols), device=device, dtype=torch.uint8)
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+
+def _dtype_f(fn, dtype):
+    d = _DTF.get(dtype)
+    if d is None:
+        raise TypeError(f"{fn}: float32, float16 or bfloat16, got {dtype}")
+    return d
+
+
+def _mx_cols(fn, cols):
+    if cols < 32 or cols % 32:
+        raise ValueError(f"{fn}: the row length must be a positive multiple of 32, got {cols}")
+
+
+def quantize_mxfp4(ctx: Context, x) -> Mxfp4:
+    """x [rows, cols] (float32, float16 or bfloat16; rows may be strided) in MXFP4, cols a multiple of 32."""
+    dt = _dtype_f("quantize_mxfp4", x.dtype)
+    if x.dim() != 2:
+        raise ValueError(f"quantize_mxfp4: a matrix, got {tuple(x.shape)}")
+    rows, cols = x.shape
+    _mx_cols("quantize_mxfp4", cols)
+    ldx = _rows16("quantize_mxfp4", "x", x, (rows, cols), x.dtype)
+    q = Mxfp4(rows, cols, x.device)
+    L.check(L.lib().tz_quantize_mxfp4(ctx.handle, _p(x), ldx, dt, _p(q.codes), _p(q.scales), rows, cols, _stream()))
+    return q
+
+
+def dequantize_mxfp4(ctx: Context, q: Mxfp4, dtype=torch.float32):
+    """The values q stands for, as [rows, cols] of `dtype`."""
+    dt = _dtype_f("dequantize_mxfp4", dtype)
+    if q.gated:
+        raise ValueError("dequantize_mxfp4: a gated pair's rows are interleaved; quantise the matrices one by one")
+    out = torch.empty(q.shape, device=q.codes.device, dtype=dtype)
+    L.check(L.lib().tz_dequantize_mxfp4(ctx.handle, _p(q.codes), _p(q.scales), _p(out), dt, q.rows, q.cols, _stream()))
+    return out
+
+
+def pack_gated_mxfp4(ctx: Context, w_gate, w_up) -> Mxfp4:
+    """w_gate and w_up [F, D] (F a multiple of 16, D of 32) as the weights of gated_linear_mxfp4."""
+    dt = _dtype_f("pack_gated_mxfp4", w_gate.dtype)
+    if w_gate.dim() != 2 or w_gate.shape[0] % 16 or w_gate.shape[0] == 0:
+        raise ValueError(f"pack_gated_mxfp4: [F, D] with F a positive multiple of 16, got {tuple(w_gate.shape)}")
+    F, D = w_gate.shape
+    _mx_cols("pack_gated_mxfp4", D)
+    _full16("pack_gated_mxfp4", "w_gate", w_gate, (F, D), w_gate.dtype)
+    _full16("pack_gated_mxfp4", "w_up", w_up, (F, D), w_gate.dtype)
+    q = Mxfp4(2 * F, D, w_gate.device, gated=True)
+    L.check(L.lib().tz_pack_gated_mxfp4(ctx.handle, _p(w_gate), _p(w_up), dt, _p(q.codes), _p(q.scales), F, D, _stream()))
+    return q
+
+
+def _mx_workspace(ctx, m, k, n, device):
+    need = C.c_size_t()
+    L.check(L.lib().tz_linear_mxfp4_workspace(ctx.handle, m, k, n, C.byref(need)))
+    return torch.empty(max(need.value, 1), device=device, dtype=torch.uint8), need.value
+
+
+def linear_mxfp4(ctx: Context, x, w: Mxfp4, bias=None, out_dtype=None, out=None):
+    """q(x) @ w.T (+ bias f32 [N]): x [M, K] (float32, float16 or bfloat16, quantised in the call) or an Mxfp4;
+    returns [M, N] of `out_dtype` (x's type; float32 for an Mxfp4).  N is a multiple of 8."""
+    given = isinstance(x, Mxfp4)
+    if w.gated or (given and x.gated):
+        raise ValueError("linear_mxfp4: a gated pair of weights goes to gated_linear_mxfp4")
+    if len(x.shape) != 2 or x.shape[1] != w.cols:
+        raise ValueError(f"linear_mxfp4: x [M, {w.cols}], got {tuple(x.shape)}")
+    M, K = x.shape
+    N = w.rows
+    out_dtype = out_dtype or (torch.float32 if given else x.dtype)
+    ydt = _dtype_f("linear_mxfp4", out_dtype)
+    if bias is not None:
+        _full16("linear_mxfp4", "bias", bias, (N,), torch.float32)
+    if out is None:
+        out = torch.empty((M, N), device=w.codes.device, dtype=out_dtype)
+    else:
+        _full16("linear_mxfp4", "out", out, (M, N), out_dtype)
+    if given:
+        L.check(L.lib().tz_gemm_mxfp4(ctx.handle, _p(x.codes), _p(x.scales), _p(w.codes), _p(w.scales), _p(bias), _p(out), ydt,
+                                      M, K, N, _stream()))
+        return out
+    ldx = _rows16("linear_mxfp4", "x", x, (M, K), x.dtype)
+    ws, size = _mx_workspace(ctx, M, K, N, x.device)
+    L.check(L.lib().tz_linear_mxfp4(ctx.handle, _p(x), ldx, _dtype_f("linear_mxfp4", x.dtype), _p(w.codes), _p(w.scales), _p(bias),
+                                    _p(out), ydt, _p(ws), size, M, K, N, _stream()))
+    return out
+
+
+def gated_linear_mxfp4(ctx: Context, x, w: Mxfp4, act: str = "silu", out=None):
+    """act(q(x) @ wg.T) * (q(x) @ wu.T) with the weights of pack_gated_mxfp4: x [T, D] float16 or bfloat16;
+    returns [T, F]."""
+    _dtype16("gated_linear_mxfp4", x)
+    if not w.gated:
+        raise ValueError("gated_linear_mxfp4: weights come from pack_gated_mxfp4")
+    if x.dim() != 2 or x.shape[1] != w.cols:
+        raise ValueError(f"gated_linear_mxfp4: x [T, {w.cols}], got {tuple(x.shape)}")
+    T, D = x.shape
+    F = w.rows // 2
+    ldx = _rows16("gated_linear_mxfp4", "x", x, (T, D), x.dtype)
+    if out is None:
+        out = torch.empty((T, F), device=x.device, dtype=x.dtype)
+    else:
+        _full16("gated_linear_mxfp4", "out", out, (T, F), x.dtype)
+    ws, size = _mx_workspace(ctx, T, D, 2 * F, x.device)
+    L.check(L.lib().tz_gated_linear_mxfp4(ctx.handle, _p(x), ldx, _DTF[x.dtype], _p(w.codes), _p(w.scales), _p(out),
+                                          _act_code("gated_linear_mxfp4", act), _p(ws), size, T, D, F, _stream()))
+    return out

@@ -1,0 +1,269 @@
+"""MXFP4 quantiser and products against the format's definition in 64 bits.
+
+The quantiser is compared exactly.  Products of E2M1 values are exact, so a product differs from the 64-bit
+one by its f32 sum (one rounding or truncation, 2^-23, per 64 products and 8 more for joined partial sums,
+relative to the sum of the absolute products) and by the rounding to the output's type (U, TINY)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f32": 2.0 ** -150, "f16": 2.0 ** -25, "bf16": 2.0 ** -134}
+GRID = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+
+
+def quant64(x):
+    """(values, element codes, scale codes) of a float array [rows, cols], from the definition."""
+    x = x.astype(np.float64)
+    b = x.reshape(x.shape[0], -1, 32)
+    top = np.abs(b).max(axis=2)
+    _, e = np.frexp(np.where(np.isfinite(top) & (top > 0), top, 1.0))
+    code = np.where(top > 0, np.maximum(e - 3, -127), -127) + 127
+    s = np.ldexp(1.0, code - 127)[..., None]
+    y = np.abs(np.where(np.isfinite(b), b, 0.0)) / s
+    d = np.abs(np.minimum(y, 6.0)[..., None] - GRID)  # distance to every grid point
+    low = d.min(axis=-1, keepdims=True)
+    even = np.where(d == low, np.arange(8) % 2, 2).argmin(axis=-1)  # of two equally near codes the even one
+    q = np.where(np.signbit(b), -GRID[even], GRID[even]) * s
+    bad = ~np.isfinite(top)
+    q[bad] = np.nan
+    code = np.where(bad, 255, code)
+    return q.reshape(x.shape), (even + 8 * np.signbit(b)).reshape(x.shape), code
+
+
+def scale_codes(q):
+    """The scale codes [rows, cols / 32] of an Mxfp4, from its documented layout."""
+    kc = -(-q.cols // 128)
+    raw = q.scales.cpu().numpy()
+    r, b = np.meshgrid(np.arange(q.rows), np.arange(q.cols // 32), indexing="ij")
+    return raw[((r // 128) * kc + b // 4) * 512 + (r % 32) * 16 + (r % 128) // 32 * 4 + b % 4]
+
+
+def element_codes(q):
+    raw = q.codes.cpu().numpy()
+    return np.stack([raw & 15, raw >> 4], axis=-1).reshape(q.rows, q.cols)
+
+
+def rand(rows, cols, dt, seed, spread=True):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((rows, cols), generator=gen, device="cuda")
+    if spread:  # scales over several binades
+        x = x * torch.exp2(torch.randint(-6, 5, (rows, cols // 32, 1), generator=gen, device="cuda").float()).expand(-1, -1, 32).reshape(rows, cols)
+    return x.to(DT[dt])
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1, 32), (2, 64), (3, 96), (5, 160), (31, 224), (33, 256), (127, 288), (128, 384), (129, 512), (300, 4096)])
+def test_quantiser_exact(ctx, rows, cols, dt):
+    from tenzor_b200 import ops
+    x = rand(rows, cols, dt, rows + cols)
+    q = ops.quantize_mxfp4(ctx, x)
+    want, codes, scales = quant64(x.float().cpu().numpy())
+    assert np.array_equal(scale_codes(q), scales)
+    assert np.array_equal(element_codes(q), codes)
+    for out in ("f32", "bf16"):
+        assert np.array_equal(ops.dequantize_mxfp4(ctx, q, DT[out]).double().cpu().numpy(), want)
+    f16 = torch.from_numpy(want).to(torch.float16)  # one rounding where f16 is too narrow
+    assert torch.equal(ops.dequantize_mxfp4(ctx, q, torch.float16).cpu(), f16)
+
+
+def test_ties_saturation_and_edges(ctx):
+    from tenzor_b200 import ops
+    x = torch.zeros(12, 32)
+    x[0, :10] = torch.tensor([4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.9, -0.25])
+    x[1, :3] = torch.tensor([7.99, 5.01, -7.5])  # above the largest code: saturates
+    x[2] = -0.0
+    x[3, 0] = 2.0 ** -149  # subnormal maximum: the smallest scale
+    x[4, 1] = 2.0 ** -126
+    x[5, 2] = 3.0e38
+    x[6, 7] = float("inf")
+    x[7, 8] = float("nan")
+    x[8, 9] = -float("inf")
+    x[9] = torch.arange(32) * 2.0 ** -130
+    x[10, 0], x[10, 1] = 1.0, 2.0 ** -140
+    x = x.cuda()
+    q = ops.quantize_mxfp4(ctx, x)
+    want, codes, scales = quant64(x.cpu().numpy())
+    assert np.array_equal(scale_codes(q), scales)
+    ok = scales[:, 0] != 255
+    assert np.array_equal(element_codes(q)[ok], codes[ok])
+    got = ops.dequantize_mxfp4(ctx, q).double().cpu().numpy()
+    assert np.array_equal(got, want, equal_nan=True)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_quantiser_strided_rows(ctx, dt):
+    from tenzor_b200 import ops
+    x = rand(37, 96, dt, 1)
+    wide = torch.full((37, 160), float("nan"), device="cuda", dtype=x.dtype)
+    wide[:, 32:128] = x
+    a, b = ops.quantize_mxfp4(ctx, wide[:, 32:128]), ops.quantize_mxfp4(ctx, x)
+    assert torch.equal(a.codes, b.codes) and np.array_equal(scale_codes(a), scale_codes(b))
+
+
+def product64(x, w, bias=None):
+    a = torch.from_numpy(quant64(x.float().cpu().numpy())[0]).cuda()
+    b = torch.from_numpy(quant64(w.float().cpu().numpy())[0]).cuda()
+    y = a @ b.t()
+    err = (x.shape[1] / 64 + 8) * 2.0 ** -23 * (a.abs() @ b.abs().t())
+    if bias is not None:
+        y = y + bias.double()
+        err = err + 2.0 ** -24 * (y.abs() + err)
+    return y, err
+
+
+def near(got, want, tol, what=""):
+    assert got.shape == want.shape
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((got.double() - want).abs().max()), float(tol.max()))
+
+
+SIZES = [(1, 32, 8), (1, 4096, 1024), (2, 64, 16), (3, 96, 200), (5, 160, 136), (8, 2048, 512), (9, 224, 24), (16, 1024, 1000),
+         (17, 288, 192), (31, 512, 384), (33, 320, 392), (64, 4096, 264), (65, 448, 200), (127, 128, 128), (128, 256, 576),
+         (129, 384, 1536), (257, 1536, 384), (300, 1056, 328), (1000, 384, 1536), (3000, 96, 72)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_linear_sizes(ctx, M, K, N, dt):
+    from tenzor_b200 import ops
+    x, w = rand(M, K, dt, M + K), (rand(N, K, dt, N).float() * K ** -0.5).to(DT[dt])
+    bias = torch.randn(N, device="cuda") if M % 2 else None
+    y = ops.linear_mxfp4(ctx, x, ops.quantize_mxfp4(ctx, w), bias)
+    torch.cuda.synchronize()
+    ctx.check_status()
+    want, err = product64(x, w, bias)
+    near(y, want, err + U[dt] * (want.abs() + err) + TINY[dt])
+
+
+@pytest.mark.parametrize("M", [4, 200])
+def test_linear_of_quantised_input_and_output_types(ctx, M):
+    from tenzor_b200 import ops
+    x, w = rand(M, 192, "bf16", 3), rand(104, 192, "f16", 4)
+    xq, wq = ops.quantize_mxfp4(ctx, x), ops.quantize_mxfp4(ctx, w)
+    want, err = product64(x, w)
+    for dt in ("f32", "f16", "bf16"):
+        tol = err + U[dt] * (want.abs() + err) + TINY[dt]
+        a = ops.linear_mxfp4(ctx, x, wq, out_dtype=DT[dt])
+        near(a, want, tol)
+        near(ops.linear_mxfp4(ctx, xq, wq, out_dtype=DT[dt]), want, tol)
+    assert ops.linear_mxfp4(ctx, xq, wq).dtype == torch.float32
+    out = torch.empty_like(a)
+    assert ops.linear_mxfp4(ctx, x, wq, out=out) is out and torch.equal(out, a)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_erf", "relu", "sigmoid"])
+@pytest.mark.parametrize("T,D,F", [(1, 32, 16), (1, 2048, 512), (6, 160, 112), (16, 1024, 208), (33, 512, 48), (140, 96, 336), (520, 384, 1536)])
+def test_gated(ctx, act, T, D, F):
+    from test_gpu_gated import act64
+    from tenzor_b200 import ops
+    dt = "bf16" if T % 2 else "f16"
+    x, wg, wu = rand(T, D, dt, T), rand(F, D, dt, 1), rand(F, D, dt, 2)
+    wg, wu = (wg.float() * 0.5 * D ** -0.5).to(DT[dt]), (wu.float() * 0.5 * D ** -0.5).to(DT[dt])
+    h = ops.gated_linear_mxfp4(ctx, x, ops.pack_gated_mxfp4(ctx, wg, wu), act)
+    torch.cuda.synchronize()
+    ctx.check_status()
+    (g, eg), (u, eu) = product64(x, wg), product64(x, wu)
+    a = act64(act, g)
+    ea = 1.13 * eg + 2.0 ** -19 * (1 + g.abs())  # |act'| <= 1.13; the fast exponential
+    err = u.abs() * ea + a.abs() * eu + ea * eu
+    near(h, a * u, err + U[dt] * ((a * u).abs() + err) + TINY[dt])
+
+
+@pytest.mark.parametrize("M", [3, 150])
+def test_bad_values_stay_in_their_rows(ctx, M):
+    from tenzor_b200 import ops
+    x, w = rand(M, 256, "bf16", 8), ops.quantize_mxfp4(ctx, rand(72, 256, "bf16", 9))
+    clean = ops.linear_mxfp4(ctx, x, w)
+    x[1, 40], x[2, 200] = float("nan"), float("inf")
+    y = ops.linear_mxfp4(ctx, x, w)
+    keep = [r for r in range(M) if r not in (1, 2)]
+    assert torch.equal(y[keep], clean[keep]) and torch.isnan(y[1:3]).all()
+
+
+@pytest.mark.parametrize("M", [5, 150])
+def test_extreme_scales(ctx, M):
+    """Scales at both ends of f32: products of a tiny and a huge block."""
+    from tenzor_b200 import ops
+    x = rand(M, 64, "f32", 1, spread=False) * 2.0 ** -100
+    w = rand(40, 64, "f32", 2, spread=False) * 2.0 ** 110
+    y = ops.linear_mxfp4(ctx, x, ops.quantize_mxfp4(ctx, w))
+    want, err = product64(x, w)
+    near(y, want, err + U["f32"] * want.abs())
+
+
+@pytest.mark.parametrize("M", [1, 7, 200])
+def test_repeats_streams_and_graphs(ctx, M):
+    from tenzor_b200 import ops
+    x, w = rand(M, 1024, "bf16", 5), ops.quantize_mxfp4(ctx, rand(520, 1024, "bf16", 6))
+    want = ops.linear_mxfp4(ctx, x, w)
+    assert torch.equal(want, ops.linear_mxfp4(ctx, x, w))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.linear_mxfp4(ctx, x, w)
+    s.synchronize()
+    assert torch.equal(got, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.linear_mxfp4(ctx, x, w)
+    got.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_no_rows(ctx):
+    from tenzor_b200 import ops
+    w = ops.quantize_mxfp4(ctx, rand(16, 64, "bf16", 1))
+    x = torch.empty((0, 64), device="cuda", dtype=torch.bfloat16)
+    q = ops.quantize_mxfp4(ctx, x)
+    assert ops.dequantize_mxfp4(ctx, q).shape == (0, 64)
+    assert ops.linear_mxfp4(ctx, x, w).shape == (0, 16) and ops.linear_mxfp4(ctx, q, w).shape == (0, 16)
+    wp = ops.pack_gated_mxfp4(ctx, rand(16, 64, "bf16", 1), rand(16, 64, "bf16", 2))
+    assert ops.gated_linear_mxfp4(ctx, x, wp).shape == (0, 16)
+
+
+def test_refusals(ctx):
+    from tenzor_b200 import TenzorError, _lib, ops
+    x = rand(4, 64, "bf16", 1)
+    w = ops.quantize_mxfp4(ctx, rand(16, 64, "bf16", 2))
+    wp = ops.pack_gated_mxfp4(ctx, rand(16, 64, "bf16", 1), rand(16, 64, "bf16", 2))
+    with pytest.raises(TypeError):
+        ops.quantize_mxfp4(ctx, x.double())
+    with pytest.raises(ValueError):
+        ops.quantize_mxfp4(ctx, x[:, :48].contiguous())
+    with pytest.raises(ValueError):
+        ops.quantize_mxfp4(ctx, x.cpu())
+    with pytest.raises(ValueError):
+        ops.linear_mxfp4(ctx, x[:, :32].contiguous(), w)
+    with pytest.raises(ValueError):
+        ops.linear_mxfp4(ctx, x, wp)
+    with pytest.raises(ValueError):
+        ops.gated_linear_mxfp4(ctx, x, w)
+    with pytest.raises(TypeError):
+        ops.gated_linear_mxfp4(ctx, x.float(), wp)
+    with pytest.raises(ValueError):
+        ops.gated_linear_mxfp4(ctx, x, wp, act="exp")
+    with pytest.raises(ValueError):
+        ops.dequantize_mxfp4(ctx, wp)
+    with pytest.raises(ValueError):
+        ops.linear_mxfp4(ctx, x, w, bias=torch.zeros(16, device="cuda", dtype=torch.float16))
+    with pytest.raises(ValueError):
+        ops.pack_gated_mxfp4(ctx, x, x)
+    with pytest.raises(TenzorError):
+        ops.linear_mxfp4(ctx, x, ops.quantize_mxfp4(ctx, rand(12, 64, "bf16", 2)))
+    with pytest.raises(TenzorError):
+        ops.quantize_mxfp4(ctx, torch.zeros(4 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(4, 64))
+    Lb, p = _lib.lib(), (lambda t: C.c_void_p(t.data_ptr()))
+    y = torch.empty(4, 16, device="cuda", dtype=torch.bfloat16)
+    assert Lb.tz_linear_mxfp4(ctx.handle, p(x), 64, 2, p(w.codes), p(w.scales), None, p(y), 2, p(y), 16, 4, 64, 16, None) == _lib.TZ_EINVAL
+    assert "workspace" in Lb.tz_get_last_error().decode()
+    assert Lb.tz_linear_mxfp4(ctx.handle, p(x), 64, 3, p(w.codes), p(w.scales), None, p(y), 2, p(y), 16, 4, 64, 16, None) == _lib.TZ_EINVAL
+    assert Lb.tz_quantize_mxfp4(None, p(x), 64, 2, p(w.codes), p(w.scales), 4, 64, None) == _lib.TZ_EINVAL
+    assert Lb.tz_mxfp4_scale_bytes(-1, 64) == 0 and Lb.tz_mxfp4_scale_bytes(129, 160) == 2 * 2 * 512
