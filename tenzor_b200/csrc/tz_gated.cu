@@ -406,7 +406,13 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
 
     tzp::tc_fence_before();
     __syncthreads();
-    if constexpr (CG == 2) tzp::cluster_sync();  // no CTA leaves while the other may still signal it
+    if constexpr (CG == 2) {
+        // The leader's last commit has arrived in CTA 1 too and both CTAs are done: nothing is under way to a
+        // CTA that has left.
+        if (rank == 1 && threadIdx.x == 32) tzp::pair_wait<CG>(drain, 0, status, nullptr);
+        __syncwarp();
+        tzp::cluster_sync();
+    }
     if (warp == 1) {
         __syncwarp();
         tzp::tc_fence_after();

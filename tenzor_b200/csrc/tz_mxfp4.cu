@@ -166,9 +166,8 @@ __global__ void __launch_bounds__(256) dequantize_mxfp4_kernel(const uint8_t* co
 // 16 up rows, and so on, so a 32-column chunk of the accumulator holds the gate and the up values of 16 outputs.
 //
 // The structure of the 16-bit gated kernel (persistent, TMA producer, MMA issuer, 8 epilogue warps, two
-// accumulators, CTA pairs).  A K block is 128 bytes = 256 values: four MMAs of 64.  Its scales arrive by bulk
-// copies (2 chunks for the CTA's 128 rows of A, up to 4 for the columns' rows of W: both CTAs of a pair keep
-// all of them) and go to TMEM by tcgen05.cp, each stage to its own 24 columns: a stage's scales are only
+// accumulators, CTA pairs).  A K block is 128 bytes = 256 values: four MMAs of 64.  Its scales are two
+// chunks for the CTA's 128 rows of A and four for the columns' rows of W (both CTAs of a pair keep all of them) and go to TMEM by tcgen05.cp, each stage to its own 24 columns: a stage's scales are only
 // replaced once its MMAs have completed.  BN = 192 leaves TMEM for that: 2 x 192 + 24 x stages <= 512 columns.
 constexpr int GROUP = 16;
 
@@ -177,9 +176,6 @@ struct MxParams {
     int rows, n;        // of the output before the gate
     int k_chunks;       // scale chunks per row block
     int k;              // values
-    int a_blocks, b_blocks;  // 128-row blocks of the scales
-    const uint8_t* sfa;
-    const uint8_t* sfb;
     const float* bias;
     int act;
 };
@@ -238,17 +234,10 @@ __device__ __forceinline__ void sf_copy(uint32_t taddr, uint32_t smem_addr) {
         asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
-// Bulk copy into this CTA's shared memory, counted on the barrier at cluster address `bar`.
-__device__ __forceinline__ void bulk_load_bar(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-                 : "memory");
-}
-
 template <int CG, int OUT, bool GATED>
 __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
     mxfp4_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO,
-                    const MxParams p, int* status) {
+                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const MxParams p, int* status) {
     using C = MxCfg<CG>;
     constexpr int STAGES = C::STAGES, BN = C::BN;
     extern __shared__ uint8_t smem_raw[];
@@ -314,17 +303,13 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                 tile_of(t, m, n);
                 const int mb = m * CG + static_cast<int>(rank);
                 const int nb = n * BN / 128;
-                const uint8_t* sa_g = p.sfa + sf_chunk(min(mb, p.a_blocks - 1), 0, p.k_chunks);
-                const uint8_t* sb_g0 = p.sfb + sf_chunk(nb, 0, p.k_chunks);
-                const uint8_t* sb_g1 = p.sfb + sf_chunk(min(nb + 1, p.b_blocks - 1), 0, p.k_chunks);
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!tzp::pair_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t sfb = 2 * kb + 1 < p.k_chunks ? 1024u : 512u;  // the last K block may hold one chunk
                     if (rank == 0) {
-                        tzp::mbar_arrive_expect_tx(&full[stage], CG * (C::A_BYTES + C::B_BYTES + 3 * sfb));
+                        tzp::mbar_arrive_expect_tx(&full[stage], CG * C::STAGE);
                         armed |= 1u << stage;
                         armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
                     }
@@ -333,9 +318,10 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                     const uint32_t sb = sa + C::A_BYTES, sf = sb + C::B_BYTES;
                     tzp::pair_load_2d<CG>(sa, &tmA, kb * 128, mb * 128, bar);
                     tzp::pair_load_2d<CG>(sb, &tmB, kb * 128, n * BN + static_cast<int>(rank) * C::BNC, bar);
-                    bulk_load_bar(sf, sa_g + kb * 1024ll, sfb, bar);
-                    bulk_load_bar(sf + 1024, sb_g0 + kb * 1024ll, sfb, bar);
-                    bulk_load_bar(sf + 2048, sb_g1 + kb * 1024ll, sfb, bar);
+                    // two chunks each (past a row block's last chunk: of the next one or zeros, which no MMA uses)
+                    tzp::pair_load_2d<CG>(sf, &tmSA, 0, mb * p.k_chunks + 2 * kb, bar);
+                    tzp::pair_load_2d<CG>(sf + 1024, &tmSB, 0, nb * p.k_chunks + 2 * kb, bar);
+                    tzp::pair_load_2d<CG>(sf + 2048, &tmSB, 0, (nb + 1) * p.k_chunks + 2 * kb, bar);
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
@@ -397,6 +383,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                     acc_phase ^= 1u;
                 }
             }
+            // Every MMA issued has completed before TMEM is released.
             tzp::pair_commit<CG>(drain);
             tzp::pair_wait<CG>(drain, 0, status, nullptr);
         }
@@ -516,7 +503,13 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
 
     tzp::tc_fence_before();
     __syncthreads();
-    if constexpr (CG == 2) tzp::cluster_sync();
+    if constexpr (CG == 2) {
+        // The leader's last commit has arrived in CTA 1 too and both CTAs are done: nothing is under way to a
+        // CTA that has left.
+        if (rank == 1 && threadIdx.x == 32) tzp::pair_wait<CG>(drain, 0, status, nullptr);
+        __syncwarp();
+        tzp::cluster_sync();
+    }
     if (warp == 1) {
         __syncwarp();
         tzp::tc_fence_after();
@@ -524,7 +517,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
     }
 }
 
-constexpr int kCG = 1;
+constexpr int kCG = 2;
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -541,8 +534,12 @@ int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, 
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::SMEM, done);
     if (rc) return rc;
-    CUtensorMap ma, mb, mo;
-    const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B;
+    CUtensorMap ma, mb, mo, msa, msb;
+    const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B, S0 = CU_TENSOR_MAP_SWIZZLE_NONE;
+    const int kc = ceil_div(k, 128);  // scale chunks: rows of 128 words
+    if ((rc = encode_tmap_2d_swz(&msa, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.scales, 128, static_cast<uint64_t>(ceil_div(a.rows, 128)) * kc, 512, 128, 2, S0)) ||
+        (rc = encode_tmap_2d_swz(&msb, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, b.scales, 128, static_cast<uint64_t>(ceil_div(b.rows, 128)) * kc, 512, 128, 2, S0)))
+        return rc;
     if ((rc = encode_tmap_2d_swz(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.codes, k / 2, a.rows, k / 2, 128, 128, S128))) return rc;
     if ((rc = encode_tmap_2d_swz(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b.codes, k / 2, b.rows, k / 2, 128, C::BNC, S128))) return rc;
     const int64_t cols = GATED ? b.rows / 2 : b.rows;
@@ -558,18 +555,14 @@ int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, 
     p.rows = static_cast<int>(a.rows);
     p.n = static_cast<int>(b.rows);
     p.k = k;
-    p.k_chunks = ceil_div(k, 128);
-    p.a_blocks = ceil_div(a.rows, 128);
-    p.b_blocks = ceil_div(b.rows, 128);
-    p.sfa = a.scales;
-    p.sfb = b.scales;
+    p.k_chunks = kc;
     p.bias = bias;
     p.act = act;
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
     const int groups = (ctx->sm_count - ctx->sm_reserve) / kCG;
     const int grid = static_cast<int>(tiles < groups ? tiles : groups) * kCG;
     TZ_CHECK(grid > 0, TZ_EINVAL, "mxfp4 kernels need %d free SMs", kCG);
-    return launch_cluster(kern, kCG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma, mb, mo, p, ctx->d_status);
+    return launch_cluster(kern, kCG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma, mb, mo, msa, msb, p, ctx->d_status);
 }
 
 template <int DT, int G>
