@@ -352,8 +352,9 @@ int tz_reduce(tz_ctx_t ctx, int reduce_op, const int* pre_ops, int n_pre, const 
  * rounded once. */
 int tz_gated_linear(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate, const void* w_up, void* h,
                     int64_t t, int d, int f, int act, int dtype, tz_stream_t stream);
-/* Bytes of device workspace one tz_gated_linear_backward call of these sizes needs. */
-int tz_gated_linear_backward_workspace(tz_ctx_t ctx, int64_t t, int d, int f, size_t* bytes);
+/* Bytes of device workspace one tz_gated_linear_backward call of these sizes needs on a context with `sms`
+ * SMs in use (tz_cuda_sm_count minus the reserve: the sums are split to fill them). */
+int tz_gated_linear_backward_workspace(int sms, int64_t t, int d, int f, size_t* bytes);
 /* dx [t, d], dw_gate and dw_up [f, d] from dh [t, f] (row stride lddh).  Nothing of the forward pass is
  * kept: gate and up are computed again in f32.  Their gradients are rounded once to `dtype` as operands of
  * the next products (an f16 value beyond 65504 there becomes an infinity); every sum is f32, and the order
@@ -388,7 +389,7 @@ int tz_pack_gated_mxfp4(tz_ctx_t ctx, const void* w_gate, const void* w_up, int 
 int tz_gemm_mxfp4(tz_ctx_t ctx, const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,
                   const float* bias, void* y, int y_dtype, int64_t m, int k, int n, tz_stream_t stream);
 /* Device workspace of the two calls below (n = 2f for the gated one). */
-int tz_linear_mxfp4_workspace(tz_ctx_t ctx, int64_t m, int k, int n, size_t* bytes);
+int tz_linear_mxfp4_workspace(int64_t m, int k, int n, size_t* bytes);
 /* y = quantised(x) w^T (+ bias): x [m, k] with row stride ldx is quantised in the call. */
 int tz_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, const void* w_codes, const void* w_scales,
                     const float* bias, void* y, int y_dtype, void* workspace, size_t workspace_bytes, int64_t m,

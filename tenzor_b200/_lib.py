@@ -180,12 +180,12 @@ def _declare(L):
         "tz_cast": [P, P, i, P, i, i64, P],
         "tz_concat": [P, P, P, i, i64, i64, i, P, P],
         "tz_gated_linear": [P, P, i64, P, P, P, i64, i, i, i, i, P],
-        "tz_gated_linear_backward_workspace": [P, i64, i, i, C.POINTER(u)],
+        "tz_gated_linear_backward_workspace": [i, i64, i, i, C.POINTER(u)],
         "tz_quantize_mxfp4": [P, P, i64, i, P, P, i64, i, P],
         "tz_dequantize_mxfp4": [P, P, P, P, i, i64, i, P],
         "tz_pack_gated_mxfp4": [P, P, P, i, P, P, i, i, P],
         "tz_gemm_mxfp4": [P, P, P, P, P, P, P, i, i64, i, i, P],
-        "tz_linear_mxfp4_workspace": [P, i64, i, i, C.POINTER(u)],
+        "tz_linear_mxfp4_workspace": [i64, i, i, C.POINTER(u)],
         "tz_linear_mxfp4": [P, P, i64, i, P, P, P, P, i, P, u, i64, i, i, P],
         "tz_gated_linear_mxfp4": [P, P, i64, i, P, P, P, i, P, u, i64, i, i, P],
         "tz_gated_linear_backward": [P, P, i64, P, P, P, i64, P, P, P, P, u, i64, i, i, i, i, P],

@@ -488,8 +488,8 @@ constexpr int kCG = 2, kBN = 256;
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 // Splits of the K blocks so that the tiles fill the GPU, each with at least 8 K blocks.
-int pick_splits(tz_ctx_t ctx, int64_t tiles, int kblocks) {
-    const int groups = (ctx->sm_count - ctx->sm_reserve) / kCG;
+int pick_splits(int sms, int64_t tiles, int kblocks) {
+    const int groups = sms / kCG;
     int s = static_cast<int>(groups / (tiles < 1 ? 1 : tiles));
     if (s > kblocks / 8) s = kblocks / 8;
     if (s > 16) s = 16;
@@ -501,13 +501,13 @@ struct BwdPlan {
     size_t dgdu, part_dx, part_dw;  // bytes
     int s_dx, s_dw;
 };
-BwdPlan plan_bwd(tz_ctx_t ctx, int64_t T, int64_t D, int64_t F) {
+BwdPlan plan_bwd(int sms, int64_t T, int64_t D, int64_t F) {
     BwdPlan b{};
     auto a256 = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
     b.dgdu = a256(static_cast<size_t>(T) * F * 2);
     const int mt = ceil_div(T, 128 * kCG), nt = ceil_div(D, kBN), ft = ceil_div(F, 128 * kCG);
-    b.s_dx = pick_splits(ctx, static_cast<int64_t>(mt) * nt, 2 * ceil_div(F, 64));
-    b.s_dw = pick_splits(ctx, 2ll * ft * nt, ceil_div(T, 64));
+    b.s_dx = pick_splits(sms, static_cast<int64_t>(mt) * nt, 2 * ceil_div(F, 64));
+    b.s_dw = pick_splits(sms, 2ll * ft * nt, ceil_div(T, 64));
     if (b.s_dx > 1) b.part_dx = a256(static_cast<size_t>(b.s_dx) * mt * 128 * kCG * D * 4);
     if (b.s_dw > 1) b.part_dw = a256(static_cast<size_t>(b.s_dw) * 2 * ft * 128 * kCG * D * 4);
     return b;
@@ -537,7 +537,7 @@ template <bool BF>
 int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& dh, const Mat& dx, const Mat& dwg, const Mat& dwu,
              int act, char* ws, cudaStream_t s) {
     const int64_t T = x.rows, D = x.cols, F = dh.cols;
-    const BwdPlan b = plan_bwd(ctx, T, D, F);
+    const BwdPlan b = plan_bwd(ctx->sm_count - ctx->sm_reserve, T, D, F);
     const Mat dg{ws, T, F, F}, du{ws + b.dgdu, T, F, F};
     float* part_dx = reinterpret_cast<float*>(ws + 2 * b.dgdu);
     float* part_dw = reinterpret_cast<float*>(ws + 2 * b.dgdu + b.part_dx);
@@ -623,11 +623,11 @@ int tz_gated_linear(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate
     return dtype == TZ_PREC_BF16 ? forward<true>(ctx, mx, mg, mu, mh, act, s) : forward<false>(ctx, mx, mg, mu, mh, act, s);
 }
 
-int tz_gated_linear_backward_workspace(tz_ctx_t ctx, int64_t t, int d, int f, size_t* bytes) {
-    TZ_CHECK(ctx && bytes, TZ_EINVAL, "tz_gated_linear_backward_workspace: null argument");
+int tz_gated_linear_backward_workspace(int sms, int64_t t, int d, int f, size_t* bytes) {
+    TZ_CHECK(sms > 0 && bytes, TZ_EINVAL, "tz_gated_linear_backward_workspace: bad argument");
     int rc = check_shape("tz_gated_linear_backward_workspace", t, d, f, TZ_PREC_F16, TZ_OP_SILU);
     if (rc) return rc;
-    const BwdPlan b = plan_bwd(ctx, t, d, f);
+    const BwdPlan b = plan_bwd(sms, t, d, f);
     *bytes = 2 * b.dgdu + b.part_dx + b.part_dw;
     return TZ_OK;
 }
@@ -651,7 +651,7 @@ int tz_gated_linear_backward(tz_ctx_t ctx, const void* x, int64_t ldx, const voi
     TZ_CHECK(al16(x) && al16(w_gate) && al16(w_up) && al16(dh) && al16(dx) && al16(dw_gate) && al16(dw_up) && al16(workspace), TZ_EINVAL,
              "tz_gated_linear_backward: pointers must be 16-byte aligned");
     size_t need = 0;
-    if ((rc = tz_gated_linear_backward_workspace(ctx, t, d, f, &need))) return rc;
+    if ((rc = tz_gated_linear_backward_workspace(ctx->sm_count - ctx->sm_reserve, t, d, f, &need))) return rc;
     TZ_CHECK(workspace_bytes >= need, TZ_EINVAL, "tz_gated_linear_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     const Mat mx{x, t, d, ldx}, mg{w_gate, f, d, d}, mu{w_up, f, d, d}, mdh{dh, t, f, lddh}, mdx{dx, t, d, d}, mwg{dw_gate, f, d, d},
         mwu{dw_up, f, d, d};

@@ -673,9 +673,9 @@ int tz_gemm_mxfp4(tz_ctx_t ctx, const void* a_codes, const void* a_scales, const
                    {static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), n}, k, bias, y, y_dtype, pick_stream(ctx, stream));
 }
 
-int tz_linear_mxfp4_workspace(tz_ctx_t ctx, int64_t m, int k, int n, size_t* bytes) {
+int tz_linear_mxfp4_workspace(int64_t m, int k, int n, size_t* bytes) {
     const char* fn = "tz_linear_mxfp4_workspace";
-    TZ_CHECK(ctx && bytes, TZ_EINVAL, "%s: null argument", fn);
+    TZ_CHECK(bytes, TZ_EINVAL, "%s: null argument", fn);
     int rc;
     if ((rc = check_dims(fn, m, k)) || (rc = check_dims(fn, n, k))) return rc;
     *bytes = a256(code_bytes(m, k)) + a256(scale_bytes(m, k));
@@ -685,7 +685,7 @@ int tz_linear_mxfp4_workspace(tz_ctx_t ctx, int64_t m, int k, int n, size_t* byt
 static int quantize_input(tz_ctx_t ctx, const char* fn, const void* x, int64_t ldx, int x_dtype, void* ws, size_t ws_bytes, int64_t m, int k, int n,
                           cudaStream_t s, Q4* out) {
     size_t need = 0;
-    int rc = tz_linear_mxfp4_workspace(ctx, m, k, n, &need);
+    int rc = tz_linear_mxfp4_workspace(m, k, n, &need);
     if (rc) return rc;
     TZ_CHECK(ws && al16(ws) && ws_bytes >= need, TZ_EINVAL, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", fn, ws_bytes, need);
     if ((rc = check_rows(fn, x, ldx, k, x_dtype))) return rc;

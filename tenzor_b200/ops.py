@@ -17,6 +17,7 @@ permute, cast, concat.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -34,8 +35,8 @@ CUDA_STREAM_LEGACY = 0x1  # cudaStreamLegacy: the handle torch's default stream 
 def _stream(s=None):
     """The stream to launch on: torch's current stream.  Its default stream has handle 0, which the C
     ABI reads as 'the context's own stream', so it is passed as cudaStreamLegacy instead."""
-    h = torch.cuda.current_stream().cuda_stream if s is None else s
-    return C.c_void_p(h if h else CUDA_STREAM_LEGACY)
+    h = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) if s is None else s
+    return h if h else CUDA_STREAM_LEGACY
 
 
 def _dev(t, dtype):
@@ -330,12 +331,19 @@ def gated_linear(ctx: Context, x, w_gate, w_up, act: str = "silu", out=None):
     _full16("gated_linear", "w_gate", w_gate, (F, D), x.dtype)
     _full16("gated_linear", "w_up", w_up, (F, D), x.dtype)
     if out is None:
-        out = torch.empty((T, F), device=x.device, dtype=x.dtype)
+        out = x.new_empty((T, F))
     else:
         _full16("gated_linear", "out", out, (T, F), x.dtype)
     L.check(L.lib().tz_gated_linear(ctx.handle, _p(x), ldx, _p(w_gate), _p(w_up), _p(out), T, D, F,
                                     _act_code("gated_linear", act), dt, _stream()))
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _gated_workspace(sms, t, d, f):
+    need = C.c_size_t()
+    L.check(L.lib().tz_gated_linear_backward_workspace(sms, t, d, f, C.byref(need)))
+    return need.value
 
 
 def gated_linear_backward(ctx: Context, x, w_gate, w_up, dh, act: str = "silu"):
@@ -351,12 +359,11 @@ def gated_linear_backward(ctx: Context, x, w_gate, w_up, dh, act: str = "silu"):
     _full16("gated_linear_backward", "w_gate", w_gate, (F, D), x.dtype)
     _full16("gated_linear_backward", "w_up", w_up, (F, D), x.dtype)
     code = _act_code("gated_linear_backward", act)
-    need = C.c_size_t()
-    L.check(L.lib().tz_gated_linear_backward_workspace(ctx.handle, T, D, F, C.byref(need)))
-    ws = torch.empty(max(need.value, 1), device=x.device, dtype=torch.uint8)
-    dx, dwg, dwu = torch.empty((T, D), device=x.device, dtype=x.dtype), torch.empty_like(w_gate), torch.empty_like(w_up)
+    size = _gated_workspace(ctx.sm_count - ctx.sm_reserve, T, D, F)
+    ws = x.new_empty(size, dtype=torch.uint8)
+    dx, dwg, dwu = x.new_empty((T, D)), x.new_empty((F, D)), x.new_empty((F, D))
     L.check(L.lib().tz_gated_linear_backward(ctx.handle, _p(x), ldx, _p(w_gate), _p(w_up), _p(dh), lddh, _p(dx), _p(dwg),
-                                             _p(dwu), _p(ws), need.value, T, D, F, code, dt, _stream()))
+                                             _p(dwu), _p(ws), size, T, D, F, code, dt, _stream()))
     return dx, dwg, dwu
 
 
@@ -366,18 +373,39 @@ _DTF = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # TZ_DT_*
 
 class Mxfp4:
     """A matrix [rows, cols] in MXFP4 on the device: `codes` [rows, cols / 2] and the tiled `scales` (layout in
-    tenzor_cuda.h).  With `gated` the rows are two weight matrices interleaved by pack_gated_mxfp4."""
+    tenzor_cuda.h), one allocation.  With `gated` the rows are two weight matrices interleaved by
+    pack_gated_mxfp4."""
 
-    __slots__ = ("codes", "scales", "rows", "cols", "gated")
+    __slots__ = ("buf", "rows", "cols", "gated", "codes_ptr", "scales_ptr")
 
-    def __init__(self, rows, cols, device, gated=False):
+    def __init__(self, rows, cols, like, gated=False):
         self.rows, self.cols, self.gated = rows, cols, gated
-        self.codes = torch.empty((rows, cols // 2), device=device, dtype=torch.uint8)
-        self.scales = torch.empty(L.lib().tz_mxfp4_scale_bytes(rows, cols), device=device, dtype=torch.uint8)
+        off, size = _mx_layout(rows, cols)
+        self.buf = like.new_empty(size, dtype=torch.uint8)
+        self.codes_ptr = self.buf.data_ptr()
+        self.scales_ptr = self.codes_ptr + off
 
     @property
     def shape(self):
         return (self.rows, self.cols)
+
+    @property
+    def device(self):
+        return self.buf.device
+
+    @property
+    def codes(self):
+        return self.buf[:self.rows * (self.cols // 2)].view(self.rows, self.cols // 2)
+
+    @property
+    def scales(self):
+        return self.buf[_mx_layout(self.rows, self.cols)[0]:]
+
+
+def _mx_layout(rows, cols):
+    """Byte offset of the scales behind the codes, and the bytes of both (what tz_linear_mxfp4_workspace adds up)."""
+    off = (rows * (cols // 2) + 255) // 256 * 256
+    return off, off + (rows + 127) // 128 * ((cols + 127) // 128) * 512
 
 
 def _dtype_f(fn, dtype):
@@ -400,8 +428,8 @@ def quantize_mxfp4(ctx: Context, x) -> Mxfp4:
     rows, cols = x.shape
     _mx_cols("quantize_mxfp4", cols)
     ldx = _rows16("quantize_mxfp4", "x", x, (rows, cols), x.dtype)
-    q = Mxfp4(rows, cols, x.device)
-    L.check(L.lib().tz_quantize_mxfp4(ctx.handle, _p(x), ldx, dt, _p(q.codes), _p(q.scales), rows, cols, _stream()))
+    q = Mxfp4(rows, cols, x)
+    L.check(L.lib().tz_quantize_mxfp4(ctx.handle, _p(x), ldx, dt, q.codes_ptr, q.scales_ptr, rows, cols, _stream()))
     return q
 
 
@@ -410,8 +438,8 @@ def dequantize_mxfp4(ctx: Context, q: Mxfp4, dtype=torch.float32):
     dt = _dtype_f("dequantize_mxfp4", dtype)
     if q.gated:
         raise ValueError("dequantize_mxfp4: a gated pair's rows are interleaved; quantise the matrices one by one")
-    out = torch.empty(q.shape, device=q.codes.device, dtype=dtype)
-    L.check(L.lib().tz_dequantize_mxfp4(ctx.handle, _p(q.codes), _p(q.scales), _p(out), dt, q.rows, q.cols, _stream()))
+    out = q.buf.new_empty(q.shape, dtype=dtype)
+    L.check(L.lib().tz_dequantize_mxfp4(ctx.handle, q.codes_ptr, q.scales_ptr, _p(out), dt, q.rows, q.cols, _stream()))
     return out
 
 
@@ -424,15 +452,16 @@ def pack_gated_mxfp4(ctx: Context, w_gate, w_up) -> Mxfp4:
     _mx_cols("pack_gated_mxfp4", D)
     _full16("pack_gated_mxfp4", "w_gate", w_gate, (F, D), w_gate.dtype)
     _full16("pack_gated_mxfp4", "w_up", w_up, (F, D), w_gate.dtype)
-    q = Mxfp4(2 * F, D, w_gate.device, gated=True)
-    L.check(L.lib().tz_pack_gated_mxfp4(ctx.handle, _p(w_gate), _p(w_up), dt, _p(q.codes), _p(q.scales), F, D, _stream()))
+    q = Mxfp4(2 * F, D, w_gate, gated=True)
+    L.check(L.lib().tz_pack_gated_mxfp4(ctx.handle, _p(w_gate), _p(w_up), dt, q.codes_ptr, q.scales_ptr, F, D, _stream()))
     return q
 
 
-def _mx_workspace(ctx, m, k, n, device):
+@functools.lru_cache(maxsize=4096)
+def _mx_workspace(m, k, n):
     need = C.c_size_t()
-    L.check(L.lib().tz_linear_mxfp4_workspace(ctx.handle, m, k, n, C.byref(need)))
-    return torch.empty(max(need.value, 1), device=device, dtype=torch.uint8), need.value
+    L.check(L.lib().tz_linear_mxfp4_workspace(m, k, n, C.byref(need)))
+    return need.value
 
 
 def linear_mxfp4(ctx: Context, x, w: Mxfp4, bias=None, out_dtype=None, out=None):
@@ -450,16 +479,17 @@ def linear_mxfp4(ctx: Context, x, w: Mxfp4, bias=None, out_dtype=None, out=None)
     if bias is not None:
         _full16("linear_mxfp4", "bias", bias, (N,), torch.float32)
     if out is None:
-        out = torch.empty((M, N), device=w.codes.device, dtype=out_dtype)
+        out = w.buf.new_empty((M, N), dtype=out_dtype)
     else:
         _full16("linear_mxfp4", "out", out, (M, N), out_dtype)
     if given:
-        L.check(L.lib().tz_gemm_mxfp4(ctx.handle, _p(x.codes), _p(x.scales), _p(w.codes), _p(w.scales), _p(bias), _p(out), ydt,
+        L.check(L.lib().tz_gemm_mxfp4(ctx.handle, x.codes_ptr, x.scales_ptr, w.codes_ptr, w.scales_ptr, _p(bias), _p(out), ydt,
                                       M, K, N, _stream()))
         return out
     ldx = _rows16("linear_mxfp4", "x", x, (M, K), x.dtype)
-    ws, size = _mx_workspace(ctx, M, K, N, x.device)
-    L.check(L.lib().tz_linear_mxfp4(ctx.handle, _p(x), ldx, _dtype_f("linear_mxfp4", x.dtype), _p(w.codes), _p(w.scales), _p(bias),
+    size = _mx_workspace(M, K, N)
+    ws = x.new_empty(size, dtype=torch.uint8)
+    L.check(L.lib().tz_linear_mxfp4(ctx.handle, _p(x), ldx, _dtype_f("linear_mxfp4", x.dtype), w.codes_ptr, w.scales_ptr, _p(bias),
                                     _p(out), ydt, _p(ws), size, M, K, N, _stream()))
     return out
 
@@ -476,10 +506,11 @@ def gated_linear_mxfp4(ctx: Context, x, w: Mxfp4, act: str = "silu", out=None):
     F = w.rows // 2
     ldx = _rows16("gated_linear_mxfp4", "x", x, (T, D), x.dtype)
     if out is None:
-        out = torch.empty((T, F), device=x.device, dtype=x.dtype)
+        out = x.new_empty((T, F))
     else:
         _full16("gated_linear_mxfp4", "out", out, (T, F), x.dtype)
-    ws, size = _mx_workspace(ctx, T, D, 2 * F, x.device)
-    L.check(L.lib().tz_gated_linear_mxfp4(ctx.handle, _p(x), ldx, _DTF[x.dtype], _p(w.codes), _p(w.scales), _p(out),
+    size = _mx_workspace(T, D, 2 * F)
+    ws = x.new_empty(size, dtype=torch.uint8)
+    L.check(L.lib().tz_gated_linear_mxfp4(ctx.handle, _p(x), ldx, _DTF[x.dtype], w.codes_ptr, w.scales_ptr, _p(out),
                                           _act_code("gated_linear_mxfp4", act), _p(ws), size, T, D, F, _stream()))
     return out

@@ -16,18 +16,17 @@ class Context:
         L.check(L.lib().tz_cuda_create(device, C.byref(h)))
         self.handle = h
         self.device = device
+        self.sm_count = L.lib().tz_cuda_sm_count(h)
+        self.sm_reserve = 0
         self._owned = weakref.WeakSet()  # models on this context: closed before the context
 
     def _adopt(self, obj):
         self._owned.add(obj)
 
-    @property
-    def sm_count(self) -> int:
-        return L.lib().tz_cuda_sm_count(self.handle)
-
     def set_sm_reserve(self, n: int):
         """Leave n SMs free in the persistent GEMM grids (for a collective running concurrently)."""
         L.check(L.lib().tz_cuda_set_sm_reserve(self.handle, int(n)))
+        self.sm_reserve = int(n)
 
     def synchronize(self):
         L.check(L.lib().tz_cuda_synchronize(self.handle))
