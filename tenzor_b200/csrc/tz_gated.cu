@@ -39,9 +39,7 @@ struct MmParams {
     int half;              // DX: K blocks of one half
     int kper;              // K blocks per split
     int m_pad;             // rows of one partial sum
-    int rows, cols;        // BWD: of dh
-    const void* dh;
-    long long ldh;
+    int cols;              // of the output
     int act;
 };
 
@@ -50,61 +48,56 @@ struct MmCfg {
     static constexpr bool kDual = MODE == MM_FWD || MODE == MM_BWD;
     static constexpr bool kAmn = MODE == MM_DW;
     static constexpr bool kBmn = MODE == MM_DX || MODE == MM_DW;
-    static constexpr int EPI = 8;
+    static constexpr int EPI = kDual ? 16 : 8;
     static constexpr int THREADS = 64 + 32 * EPI;
     static constexpr int BNC = BN / CG;  // B rows (or columns) in one CTA
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int STAGE = A_BYTES + BNC * 128;
-    static constexpr int STAGING = EPI * 4096;
+    static constexpr int BOX = MODE == MM_FWD ? 2048 : 4096;  // staging of one epilogue warp
+    static constexpr int STAGING = EPI * BOX;
     static constexpr int BUDGET = 227 * 1024 - 1024 - 512 - STAGING;
     static constexpr int STAGES = BUDGET / STAGE > 8 ? 8 : BUDGET / STAGE;
     static constexpr int SMEM = STAGES * STAGE + STAGING + 512 + 1024;
+    static_assert(!kDual || BN == 256, "16 epilogue warps of 32 output columns");
     static_assert(!kBmn || BNC % 64 == 0, "MN-major B comes in blocks of 64");
 };
 
-// act over 32 gate / up pairs -> packed 16-bit outputs.
+// 16 gate / up pairs -> 8 words of 16-bit outputs.
 template <int ACT, bool BF>
-__device__ __forceinline__ void fwd_math(const uint32_t (&g)[32], const uint32_t (&u)[32], uint32_t (&o)[16]) {
+__device__ __forceinline__ void fwd_math(const uint32_t (&g)[16], const uint32_t (&u)[16], uint32_t* o) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        float d;
-        const float a = gated_act<ACT, false>(__uint_as_float(g[2 * j]), d) * __uint_as_float(u[2 * j]);
-        const float b = gated_act<ACT, false>(__uint_as_float(g[2 * j + 1]), d) * __uint_as_float(u[2 * j + 1]);
-        o[j] = tzp::pack16x2<BF>(a, b);
-    }
+    for (int j = 0; j < 8; ++j) o[j] = gated_pair<ACT, BF>(g[2 * j], g[2 * j + 1], u[2 * j], u[2 * j + 1]);
 }
 template <int ACT, bool BF>
-__device__ __forceinline__ void bwd_math(const uint32_t (&g)[32], const uint32_t (&u)[32], const uint32_t (&dh)[16],
-                                         uint32_t (&dg)[16], uint32_t (&du)[16]) {
+__device__ __forceinline__ void bwd_math(const uint32_t (&g)[16], const uint32_t (&u)[16], const uint32_t* dh, uint32_t* dg, uint32_t* du) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 8; ++j) {
         float2 h;
         if constexpr (BF)
             h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&dh[j]));
         else
             h = __half22float2(*reinterpret_cast<const __half2*>(&dh[j]));
-        float d0, d1;
-        const float a0 = gated_act<ACT, true>(__uint_as_float(g[2 * j]), d0);
-        const float a1 = gated_act<ACT, true>(__uint_as_float(g[2 * j + 1]), d1);
-        dg[j] = tzp::pack16x2<BF>(h.x * __uint_as_float(u[2 * j]) * d0, h.y * __uint_as_float(u[2 * j + 1]) * d1);
-        du[j] = tzp::pack16x2<BF>(h.x * a0, h.y * a1);
+        uint64_t d;
+        const uint64_t h2 = tzp::f2_pack(h.x, h.y);
+        const uint64_t a = gated_act2<ACT, true>(tzp::f2_pack(__uint_as_float(g[2 * j]), __uint_as_float(g[2 * j + 1])), d);
+        const float2 p = tzp::f2_unpack(tzp::f2_mul(tzp::f2_mul(h2, tzp::f2_pack(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]))), d));
+        const float2 q = tzp::f2_unpack(tzp::f2_mul(h2, a));
+        dg[j] = tzp::pack16x2<BF>(p.x, p.y);
+        du[j] = tzp::pack16x2<BF>(q.x, q.y);
     }
 }
 
-#define TZ_ACT_SWITCH(act, CALL)                          \
-    switch (act) {                                        \
-        case TZ_OP_SILU: CALL(TZ_OP_SILU); break;         \
-        case TZ_OP_GELU: CALL(TZ_OP_GELU); break;         \
-        case TZ_OP_GELU_ERF: CALL(TZ_OP_GELU_ERF); break; \
-        case TZ_OP_RELU: CALL(TZ_OP_RELU); break;         \
-        default: CALL(TZ_OP_SIGMOID); break;              \
-    }
-
-// 32 rows (one per lane) x 64 bytes into a 2 KB box with the 64-byte swizzle.
-__device__ __forceinline__ void stage64(uint32_t buf, int lane, const uint32_t (&o)[16]) {
+// 16-byte units c0 .. c0 + N - 1 of this lane's row of a 32-row box with 64-byte rows and the 64-byte swizzle.
+template <int N>
+__device__ __forceinline__ void stage64(uint32_t buf, int lane, int c0, const uint32_t* o) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-        tzp::st_shared_v4(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+    for (int c = 0; c < N; ++c)
+        tzp::st_shared_v4(buf + lane * 64 + (((c0 + c) ^ ((lane >> 1) & 3)) << 4), o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
 }
 // 32 rows x 128 bytes into a 4 KB box with the 128-byte swizzle.
 __device__ __forceinline__ void stage128(uint32_t buf, int lane, const uint32_t (&v)[32]) {
@@ -117,8 +110,8 @@ template <int CG, int BN, int MODE, bool BF, bool PART>
 __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     gated_mm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
                     const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
-                    const __grid_constant__ CUtensorMap tmO0, const __grid_constant__ CUtensorMap tmO1, const MmParams p,
-                    int* status) {
+                    const __grid_constant__ CUtensorMap tmO0, const __grid_constant__ CUtensorMap tmO1,
+                    const __grid_constant__ CUtensorMap tmDh, const MmParams p, int* status) {
     using C = MmCfg<CG, BN, MODE>;
     constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -130,7 +123,8 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     uint64_t* tfull = empty + STAGES;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* dhbar = drain + 1;  // one per epilogue warp (BWD)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dhbar + C::EPI);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
@@ -147,6 +141,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             tzp::mbar_init(&tempty[a], C::EPI * CG);
         }
         tzp::mbar_init(drain, 1);
+        for (int e = 0; e < C::EPI; ++e) tzp::mbar_init(&dhbar[e], 1);
         *abort_flag = 0;
         tzp::fence_mbar_init();
         tzp::tma_prefetch_desc(&tmA0);
@@ -284,12 +279,24 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             tzp::pair_wait<CG>(drain, 0, status, nullptr);
         }
     } else {
-        // ---- epilogue: warp reads TMEM lane quarter (warp % 4) and half of the columns ----
-        const int e = warp - 2, q4 = warp & 3, hf = e >> 2;
-        const uint32_t box = tzp::smem_u32(staging) + static_cast<uint32_t>(e * 4096);
-        uint8_t* boxp = staging + e * 4096;
+        // ---- epilogue: a warp reads TMEM lane quarter (warp % 4) and a slice of the columns: 32 outputs of a
+        // dual tile (the gate and the up columns of each), half of the columns otherwise ----
+        const int e = warp - 2, q4 = warp & 3, sl = e >> 2;
+        const uint32_t box = tzp::smem_u32(staging) + static_cast<uint32_t>(e * C::BOX);
+        uint8_t* boxp = staging + e * C::BOX;
         int acc = 0, nb = 0;
-        uint32_t acc_phase = 0;
+        uint32_t acc_phase = 0, dh_phase = 0;
+        // BWD: the 32 x 32 box of dh that a tile needs comes by TMA into the box that later takes dg; it is asked
+        // for as soon as the previous tile's stores have read the box.
+        auto fetch_dh = [&](int t) {
+            const Tile q = tile_of(t);
+            tzp::mbar_arrive_expect_tx(&dhbar[e], 2048);
+            tzp::tma_load_2d(boxp, &tmDh, q.n * (BN / 2) + sl * 32, (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32, &dhbar[e]);
+        };
+        if constexpr (MODE == MM_BWD) {
+            if (lane == 0 && t0 < num_tiles) fetch_dh(t0);
+        }
+        bool fetched = MODE == MM_BWD && t0 < num_tiles;
         for (int t = t0; t < num_tiles; t += tstep) {
             const Tile q = tile_of(t);
             if (!tzp::pair_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
@@ -297,65 +304,72 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN);
             const int row0 = (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32;
             if constexpr (C::kDual) {
-                constexpr int CH = BN / 128;  // 32-column chunks of this warp: half of the BN / 2 outputs
-#pragma unroll 1
-                for (int c = 0; c < CH; ++c) {
-                    const int cc = (hf * CH + c) * 32;
-                    const int col0 = q.n * (BN / 2) + cc;
-                    if (col0 >= p.cols) break;
-                    uint32_t dh[16];
-                    if constexpr (MODE == MM_BWD) {
-                        const bool rok = row0 + lane < p.rows;
-                        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.dh) + (row0 + lane) * p.ldh + col0);
+                const int cc = sl * 32;
+                const int col0 = q.n * (BN / 2) + cc;
+                uint32_t dh[16];
+                if constexpr (MODE == MM_BWD) {
+                    if (!tzp::mbar_wait(&dhbar[e], dh_phase, status, abort_flag)) break;
+                    dh_phase ^= 1u;
+                    fetched = false;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint4 v = make_uint4(0, 0, 0, 0);
-                            if (rok && col0 + 8 * j < p.cols) v = __ldg(src + j);
-                            dh[4 * j] = v.x, dh[4 * j + 1] = v.y, dh[4 * j + 2] = v.z, dh[4 * j + 3] = v.w;
+                    for (int c = 0; c < 4; ++c) {
+                        const uint4 v = ld_shared_v4(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
+                        dh[4 * c] = v.x, dh[4 * c + 1] = v.y, dh[4 * c + 2] = v.z, dh[4 * c + 3] = v.w;
+                    }
+                    __syncwarp();  // every lane has its row before any lane writes dg over it
+                } else {
+                    if (lane == 0) tzp::bulk_wait_read<0>();  // the previous tile's store has read the box
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {  // 16 outputs at a time
+                    uint32_t g[16], u[16];
+                    tzp::tmem_ld16(td + cc + 16 * c, g);
+                    tzp::tmem_ld16(td + BN / 2 + cc + 16 * c, u);
+                    tzp::tmem_ld_wait();
+                    if (c == 1) {  // the accumulator is in registers: the MMAs may have it back
+                        tzp::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (CG == 2)
+                                tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
+                            else
+                                tzp::mbar_arrive(&tempty[acc]);
                         }
                     }
-                    uint32_t g[32], u[32];
-                    tzp::tmem_ld32(td + cc, g);
-                    tzp::tmem_ld32(td + BN / 2 + cc, u);
-                    tzp::tmem_ld_wait();
+                    uint32_t o[8], o2[8];
                     if constexpr (MODE == MM_FWD) {
-                        uint32_t o[16];
 #define TZ_FWD(A) fwd_math<A, BF>(g, u, o)
                         TZ_ACT_SWITCH(p.act, TZ_FWD)
 #undef TZ_FWD
-                        if (lane == 0) tzp::bulk_wait_read<1>();  // the store that used this box has read it
-                        __syncwarp();
-                        stage64(box + nb * 2048, lane, o);
-                        tzp::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tzp::tma_store_2d(&tmO0, boxp + nb * 2048, col0, row0);
-                            tzp::bulk_commit();
-                        }
-                        nb ^= 1;
                     } else {
-                        uint32_t dg[16], du[16];
-#define TZ_BWD(A) bwd_math<A, BF>(g, u, dh, dg, du)
+#define TZ_BWD(A) bwd_math<A, BF>(g, u, dh + 8 * c, o, o2)
                         TZ_ACT_SWITCH(p.act, TZ_BWD)
 #undef TZ_BWD
-                        if (lane == 0) tzp::bulk_wait_read<0>();
-                        __syncwarp();
-                        stage64(box, lane, dg);
-                        stage64(box + 2048, lane, du);
-                        tzp::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tzp::tma_store_2d(&tmO0, boxp, col0, row0);
-                            tzp::tma_store_2d(&tmO1, boxp + 2048, col0, row0);
-                            tzp::bulk_commit();
-                        }
+                        stage64<2>(box + 2048, lane, 2 * c, o2);
+                    }
+                    stage64<2>(box, lane, 2 * c, o);
+                }
+                tzp::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    if (col0 < p.cols) {
+                        tzp::tma_store_2d(&tmO0, boxp, col0, row0);
+                        if constexpr (MODE == MM_BWD) tzp::tma_store_2d(&tmO1, boxp + 2048, col0, row0);
+                        tzp::bulk_commit();
+                    }
+                    if constexpr (MODE == MM_BWD) {
+                        tzp::bulk_wait_read<0>();
+                        if (t + tstep < num_tiles) fetch_dh(t + tstep);
                     }
                 }
+                __syncwarp();
+                if constexpr (MODE == MM_BWD) fetched = t + tstep < num_tiles;
             } else {
                 constexpr int CH = BN / 64;
 #pragma unroll 1
                 for (int c = 0; c < CH; ++c) {
-                    const int cc = (hf * CH + c) * 32;
+                    const int cc = (sl * CH + c) * 32;
                     const int col0 = q.n * BN + cc;
                     if (col0 >= p.cols) break;
                     uint32_t v[32];
@@ -377,7 +391,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                         for (int j = 0; j < 16; ++j) o[j] = tzp::pack16x2<BF>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
                         if (lane == 0) tzp::bulk_wait_read<1>();
                         __syncwarp();
-                        stage64(box + nb * 2048, lane, o);
+                        stage64<4>(box + nb * 2048, lane, 0, o);
                         tzp::fence_proxy_async();
                         __syncwarp();
                         if (lane == 0) {
@@ -388,20 +402,25 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                     }
                 }
             }
-            tzp::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (CG == 2)
-                    tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
-                else
-                    tzp::mbar_arrive(&tempty[acc]);
+            if constexpr (!C::kDual) {
+                tzp::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 2)
+                        tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
+                    else
+                        tzp::mbar_arrive(&tempty[acc]);
+                }
             }
             if (++acc == 2) {
                 acc = 0;
                 acc_phase ^= 1u;
             }
         }
-        if (lane == 0) tzp::bulk_wait_all();
+        if (lane == 0) {
+            tzp::bulk_wait_all();
+            if (fetched) tzp::mbar_wait(&dhbar[e], dh_phase, status, nullptr);  // left early: its copy has landed
+        }
     }
 
     tzp::tc_fence_before();
@@ -454,14 +473,14 @@ int map16(CUtensorMap* m, const Mat& a, int box_cols, int box_rows, CUtensorMapS
 }
 
 template <int CG, int BN, int MODE, bool BF, bool PART>
-int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, const Mat& o0, const Mat& o1, MmParams p,
-              float* part, cudaStream_t s) {
+int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, const Mat& o0, const Mat& o1, const Mat* dh,
+              const MmParams& p, float* part, cudaStream_t s) {
     using C = MmCfg<CG, BN, MODE>;
     auto kern = gated_mm_kernel<CG, BN, MODE, BF, PART>;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::SMEM, done);
     if (rc) return rc;
-    CUtensorMap ma0, ma1, mb0, mb1, mo0, mo1;
+    CUtensorMap ma0, ma1, mb0, mb1, mo0, mo1, mdh;
     const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B;
     const int arows = C::kAmn ? 64 : 128, brows = C::kBmn ? 64 : (C::kDual ? BN / 2 : C::BNC);
     if ((rc = map16<BF>(&ma0, a0, 64, arows, S128)) || (rc = map16<BF>(&ma1, a1, 64, arows, S128)) ||
@@ -476,11 +495,13 @@ int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const M
         if (!rc) rc = map16<BF>(&mo1, o1, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
     }
     if (rc) return rc;
+    mdh = mo0;
+    if (dh && (rc = map16<BF>(&mdh, *dh, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * p.which * p.splits;
     const int groups = (ctx->sm_count - ctx->sm_reserve) / CG;
     const int grid = static_cast<int>(tiles < groups ? tiles : groups) * CG;
     TZ_CHECK(grid > 0, TZ_EINVAL, "gated kernels need %d free SMs", CG);
-    return launch_cluster(kern, CG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma0, ma1, mb0, mb1, mo0, mo1, p, ctx->d_status);
+    return launch_cluster(kern, CG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma0, ma1, mb0, mb1, mo0, mo1, mdh, p, ctx->d_status);
 }
 
 constexpr int kCG = 2, kBN = 256;
@@ -527,10 +548,9 @@ int forward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat&
     p.n_tiles = ceil_div(h.cols, kBN / 2);
     p.which = p.splits = 1;
     p.kblocks = p.kper = ceil_div(x.cols, 64);
-    p.rows = static_cast<int>(h.rows);
     p.cols = static_cast<int>(h.cols);
     p.act = act;
-    return launch_mm<kCG, kBN, MM_FWD, BF, false>(ctx, x, x, wg, wu, h, h, p, nullptr, s);
+    return launch_mm<kCG, kBN, MM_FWD, BF, false>(ctx, x, x, wg, wu, h, h, nullptr, p, nullptr, s);
 }
 
 template <bool BF>
@@ -546,12 +566,9 @@ int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat
     p.n_tiles = ceil_div(F, kBN / 2);
     p.which = p.splits = 1;
     p.kblocks = p.kper = ceil_div(D, 64);
-    p.rows = static_cast<int>(T);
     p.cols = static_cast<int>(F);
-    p.dh = dh.p;
-    p.ldh = dh.ld;
     p.act = act;
-    int rc = launch_mm<kCG, kBN, MM_BWD, BF, false>(ctx, x, x, wg, wu, dg, du, p, nullptr, s);
+    int rc = launch_mm<kCG, kBN, MM_BWD, BF, false>(ctx, x, x, wg, wu, dg, du, &dh, p, nullptr, s);
     if (rc) return rc;
 
     MmParams q{};
@@ -563,13 +580,12 @@ int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat
     q.kblocks = 2 * q.half;
     q.kper = ceil_div(q.kblocks, q.splits);
     q.m_pad = q.m_tiles * 128 * kCG;
-    q.rows = static_cast<int>(T);
     q.cols = static_cast<int>(D);
     if (q.splits > 1) {
-        rc = launch_mm<kCG, kBN, MM_DX, BF, true>(ctx, dg, du, wg, wu, dx, dx, q, part_dx, s);
-        if (!rc) rc = sum_parts<BF>(ctx, part_dx, const_cast<void*>(dx.p), nullptr, 1, q.splits, q.m_pad, q.rows, q.cols, s);
+        rc = launch_mm<kCG, kBN, MM_DX, BF, true>(ctx, dg, du, wg, wu, dx, dx, nullptr, q, part_dx, s);
+        if (!rc) rc = sum_parts<BF>(ctx, part_dx, const_cast<void*>(dx.p), nullptr, 1, q.splits, q.m_pad, static_cast<int>(T), q.cols, s);
     } else {
-        rc = launch_mm<kCG, kBN, MM_DX, BF, false>(ctx, dg, du, wg, wu, dx, dx, q, nullptr, s);
+        rc = launch_mm<kCG, kBN, MM_DX, BF, false>(ctx, dg, du, wg, wu, dx, dx, nullptr, q, nullptr, s);
     }
     if (rc) return rc;
 
@@ -581,14 +597,13 @@ int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat
     r.kblocks = ceil_div(T, 64);
     r.kper = ceil_div(r.kblocks, r.splits);
     r.m_pad = r.m_tiles * 128 * kCG;
-    r.rows = static_cast<int>(F);
     r.cols = static_cast<int>(D);
     if (r.splits > 1) {
-        rc = launch_mm<kCG, kBN, MM_DW, BF, true>(ctx, dg, du, x, x, dwg, dwu, r, part_dw, s);
-        if (!rc) rc = sum_parts<BF>(ctx, part_dw, const_cast<void*>(dwg.p), const_cast<void*>(dwu.p), 2, r.splits, r.m_pad, r.rows, r.cols, s);
+        rc = launch_mm<kCG, kBN, MM_DW, BF, true>(ctx, dg, du, x, x, dwg, dwu, nullptr, r, part_dw, s);
+        if (!rc) rc = sum_parts<BF>(ctx, part_dw, const_cast<void*>(dwg.p), const_cast<void*>(dwu.p), 2, r.splits, r.m_pad, static_cast<int>(F), r.cols, s);
         return rc;
     }
-    return launch_mm<kCG, kBN, MM_DW, BF, false>(ctx, dg, du, x, x, dwg, dwu, r, nullptr, s);
+    return launch_mm<kCG, kBN, MM_DW, BF, false>(ctx, dg, du, x, x, dwg, dwu, nullptr, r, nullptr, s);
 }
 
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }

@@ -411,20 +411,9 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                 tzp::tmem_ld_wait();
                 if constexpr (GATED) {
                     uint32_t o[8];
-#define TZ_G(A)                                                                                              \
-    for (int j = 0; j < 8; ++j) {                                                                            \
-        float d_;                                                                                            \
-        const float a_ = gated_act<A, false>(__uint_as_float(v[2 * j]), d_) * __uint_as_float(v[16 + 2 * j]); \
-        const float b_ = gated_act<A, false>(__uint_as_float(v[2 * j + 1]), d_) * __uint_as_float(v[17 + 2 * j]); \
-        o[j] = tzp::pack16x2<OUT == DT_BF16>(a_, b_);                                                        \
-    }
-                    switch (p.act) {
-                        case TZ_OP_SILU: _Pragma("unroll") TZ_G(TZ_OP_SILU) break;
-                        case TZ_OP_GELU: _Pragma("unroll") TZ_G(TZ_OP_GELU) break;
-                        case TZ_OP_GELU_ERF: _Pragma("unroll") TZ_G(TZ_OP_GELU_ERF) break;
-                        case TZ_OP_RELU: _Pragma("unroll") TZ_G(TZ_OP_RELU) break;
-                        default: _Pragma("unroll") TZ_G(TZ_OP_SIGMOID) break;
-                    }
+#define TZ_G(A) \
+    for (int j = 0; j < 8; ++j) o[j] = gated_pair<A, OUT == DT_BF16>(v[2 * j], v[2 * j + 1], v[16 + 2 * j], v[17 + 2 * j])
+                    TZ_ACT_SWITCH(p.act, _Pragma("unroll") TZ_G)
 #undef TZ_G
                     if (lane == 0) tzp::bulk_wait_read<1>();
                     __syncwarp();
