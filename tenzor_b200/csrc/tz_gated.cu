@@ -153,7 +153,6 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     if constexpr (CG == 2) tzp::cluster_sync();  // both CTAs' barriers exist before either signals them
     tzp::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    tzp::pdl_trigger();
     tzp::pdl_wait();
 
     // Tile t of this launch: a group of 8 row blocks walks all column blocks before the next group starts, so
@@ -423,6 +422,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         }
     }
 
+    tzp::pdl_trigger();
     tzp::tc_fence_before();
     __syncthreads();
     if constexpr (CG == 2) {
@@ -442,8 +442,6 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
 // Sums the partial products [splits][which][m_pad][cols] in order and rounds to 16 bits.
 template <bool BF>
 __global__ void sum_parts_kernel(const float* part, void* out0, void* out1, int which, int splits, int m_pad, int rows, int cols) {
-    tzp::pdl_trigger();
-    tzp::pdl_wait();
     const long long n8 = static_cast<long long>(rows) * cols / 8;
     const long long plane = static_cast<long long>(m_pad) * cols;
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n8 * which; i += static_cast<long long>(gridDim.x) * blockDim.x) {
@@ -538,7 +536,7 @@ template <bool BF>
 int sum_parts(tz_ctx_t ctx, const float* part, void* o0, void* o1, int which, int splits, int m_pad, int rows, int cols, cudaStream_t s) {
     const long long n8 = static_cast<long long>(rows) * cols / 8 * which;
     const int blocks = static_cast<int>(n8 / 256 + 1 < ctx->sm_count * 8 ? n8 / 256 + 1 : ctx->sm_count * 8);
-    return launch_kernel(sum_parts_kernel<BF>, dim3(blocks), dim3(256), 0, s, true, part, o0, o1, which, splits, m_pad, rows, cols);
+    return launch_kernel(sum_parts_kernel<BF>, dim3(blocks), dim3(256), 0, s, false, part, o0, o1, which, splits, m_pad, rows, cols);
 }
 
 template <bool BF>

@@ -94,8 +94,6 @@ __device__ __forceinline__ uint32_t quant_block(const float (&v)[8], uint32_t& s
 template <int DT, int GROUP>
 __global__ void __launch_bounds__(256) quantize_mxfp4_kernel(const void* x, long long ldx, uint8_t* codes, uint8_t* scales, long long rows,
                                                              int cols, int off) {
-    tzp::pdl_trigger();
-    tzp::pdl_wait();
     const int lane = threadIdx.x & 31;
     const int k_chunks = (cols + 127) / 128;
     const int steps = (cols + 255) / 256;
@@ -118,6 +116,7 @@ __global__ void __launch_bounds__(256) quantize_mxfp4_kernel(const void* x, long
         if (in && (lane & 15) == 0)
             *reinterpret_cast<uint32_t*>(scales + sf_chunk(ro >> 7, c >> 7, k_chunks) + (ro & 31) * 16 + ((ro & 127) >> 5) * 4) = w;
     }
+    tzp::pdl_trigger();  // the product that follows may set up
 }
 
 // 2^(code - 127) in f32 (code 0 is the subnormal 2^-127, 255 a NaN).
@@ -134,8 +133,6 @@ __device__ __forceinline__ float2 e2m1x2(uint32_t byte) {
 
 template <int DT>
 __global__ void __launch_bounds__(256) dequantize_mxfp4_kernel(const uint8_t* codes, const uint8_t* scales, void* out, long long rows, int cols) {
-    tzp::pdl_trigger();
-    tzp::pdl_wait();
     const int k_chunks = (cols + 127) / 128;
     const long long n8 = rows * (cols / 8);
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n8; i += static_cast<long long>(gridDim.x) * blockDim.x) {
@@ -165,7 +162,7 @@ __global__ void __launch_bounds__(256) dequantize_mxfp4_kernel(const uint8_t* co
 // y = q(x) q(W)^T (+ bias), or with GATED the gated form of interleaved weights: W rows come as 16 gate rows,
 // 16 up rows, and so on, so a 32-column chunk of the accumulator holds the gate and the up values of 16 outputs.
 //
-// The structure of the 16-bit gated kernel (persistent, TMA producer, MMA issuer, 8 epilogue warps, two
+// The structure of the 16-bit gated kernel (persistent, TMA producer, MMA issuer, 12 epilogue warps, two
 // accumulators, CTA pairs).  A K block is 128 bytes = 256 values: four MMAs of 64.  Its scales are two
 // chunks for the CTA's 128 rows of A and four for the columns' rows of W (both CTAs of a pair keep all of them) and go to TMEM by tcgen05.cp, each stage to its own 24 columns: a stage's scales are only
 // replaced once its MMAs have completed.  BN = 192 leaves TMEM for that: 2 x 192 + 24 x stages <= 512 columns.
@@ -183,7 +180,7 @@ struct MxParams {
 template <int CG>
 struct MxCfg {
     static constexpr int BN = 192;
-    static constexpr int EPI = 8;
+    static constexpr int EPI = 12;  // 4 TMEM lane quarters x 3 slices of 64 columns
     static constexpr int THREADS = 64 + 32 * EPI;
     static constexpr int BNC = BN / CG;
     static constexpr int A_BYTES = 128 * 128;
@@ -277,7 +274,6 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
     if constexpr (CG == 2) tzp::cluster_sync();
     tzp::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    tzp::pdl_trigger();
     tzp::pdl_wait();
 
     const int num_tiles = p.m_tiles * p.n_tiles;
@@ -388,99 +384,96 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
             tzp::pair_wait<CG>(drain, 0, status, nullptr);
         }
     } else {
-        // ---- epilogue: TMEM lane quarter (warp % 4), half of the columns, in chunks of 32 ----
-        const int e = warp - 2, q4 = warp & 3, hf = e >> 2;
+        // ---- epilogue: TMEM lane quarter (warp % 4), 64 of the columns ----
+        const int e = warp - 2, q4 = warp & 3, sl = e >> 2;
         const uint32_t box = tzp::smem_u32(staging) + static_cast<uint32_t>(e * 4096);
         uint8_t* boxp = staging + e * 4096;
-        int acc = 0, nb = 0;
+        int acc = 0;
         uint32_t acc_phase = 0;
         for (int t = t0; t < num_tiles; t += tstep) {
             int m, n;
             tile_of(t, m, n);
             if (!tzp::pair_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
             tzp::tc_fence_after();
-            const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN);
+            const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN + sl * 64);
             const int row0 = (m * CG + static_cast<int>(rank)) * 128 + q4 * 32;
-#pragma unroll 1
-            for (int c = 0; c < BN / 64; ++c) {
-                const int cc = (hf * (BN / 64) + c) * 32;
-                const int col0 = n * BN + cc;
-                if (col0 >= p.n) break;
+            const int colt = n * BN + sl * 64;
+            if (lane == 0) tzp::bulk_wait_read<0>();  // the previous tile's stores have read the boxes
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int col0 = colt + 32 * c;
                 uint32_t v[32];
-                tzp::tmem_ld32(td + cc, v);
+                tzp::tmem_ld32(td + 32 * c, v);
                 tzp::tmem_ld_wait();
+                if (c == 1) {  // the accumulator is in registers: the MMAs may have it back
+                    tzp::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (CG == 2)
+                            tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
+                        else
+                            tzp::mbar_arrive(&tempty[acc]);
+                    }
+                }
                 if constexpr (GATED) {
                     uint32_t o[8];
 #define TZ_G(A) \
     for (int j = 0; j < 8; ++j) o[j] = gated_pair<A, OUT == DT_BF16>(v[2 * j], v[2 * j + 1], v[16 + 2 * j], v[17 + 2 * j])
                     TZ_ACT_SWITCH(p.act, _Pragma("unroll") TZ_G)
 #undef TZ_G
-                    if (lane == 0) tzp::bulk_wait_read<1>();
-                    __syncwarp();
-                    const uint32_t b = box + nb * 1024 + lane * 32;  // 32-byte rows, 32-byte swizzle
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
-                        tzp::st_shared_v4(b + ((u ^ ((lane >> 2) & 1)) << 4), o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
-                    tzp::fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tzp::tma_store_2d(&tmO, boxp + nb * 1024, col0 / 2, row0);
-                        tzp::bulk_commit();
-                    }
-                    nb ^= 1;
-                } else {
-                    if (p.bias) {
+                        tzp::st_shared_v4(box + lane * 64 + (((2 * c + u) ^ ((lane >> 1) & 3)) << 4), o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                    continue;
+                }
+                if (p.bias) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            if (col0 + j < p.n) {  // n is a multiple of 8
-                                const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + col0 + j));
-                                v[j] = __float_as_uint(__uint_as_float(v[j]) + b4.x);
-                                v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + b4.y);
-                                v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) + b4.z);
-                                v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) + b4.w);
-                            }
+                    for (int j = 0; j < 32; j += 4) {
+                        if (col0 + j < p.n) {  // n is a multiple of 8
+                            const float4 b4 = __ldg(reinterpret_cast<const float4*>(p.bias + col0 + j));
+                            v[j] = __float_as_uint(__uint_as_float(v[j]) + b4.x);
+                            v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + b4.y);
+                            v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) + b4.z);
+                            v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) + b4.w);
                         }
-                    }
-                    if constexpr (OUT == DT_F32) {
-                        if (lane == 0) tzp::bulk_wait_read<0>();
-                        __syncwarp();
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            tzp::st_shared_v4(box + lane * 128 + ((u ^ (lane & 7)) << 4), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-                        tzp::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tzp::tma_store_2d(&tmO, boxp, col0, row0);
-                            tzp::bulk_commit();
-                        }
-                    } else {
-                        uint32_t o[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            o[j] = tzp::pack16x2<OUT == DT_BF16>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-                        if (lane == 0) tzp::bulk_wait_read<1>();
-                        __syncwarp();
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            tzp::st_shared_v4(box + nb * 2048 + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4), o[4 * u], o[4 * u + 1], o[4 * u + 2],
-                                              o[4 * u + 3]);
-                        tzp::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tzp::tma_store_2d(&tmO, boxp + nb * 2048, col0, row0);
-                            tzp::bulk_commit();
-                        }
-                        nb ^= 1;
                     }
                 }
+                if constexpr (OUT == DT_F32) {  // one box of 32 columns, stored at once
+                    if (c == 1) {
+                        if (lane == 0) tzp::bulk_wait_read<0>();
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        tzp::st_shared_v4(box + lane * 128 + ((u ^ (lane & 7)) << 4), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+                    tzp::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0 && col0 < p.n) {
+                        tzp::tma_store_2d(&tmO, boxp, col0, row0);
+                        tzp::bulk_commit();
+                    }
+                } else if constexpr (!GATED) {
+                    uint32_t o[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j] = tzp::pack16x2<OUT == DT_BF16>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        tzp::st_shared_v4(box + c * 2048 + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4), o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                }
             }
-            tzp::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (CG == 2)
-                    tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
-                else
-                    tzp::mbar_arrive(&tempty[acc]);
+            if constexpr (OUT != DT_F32) {
+                tzp::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0 && colt < p.n) {
+                    if constexpr (GATED) {
+                        tzp::tma_store_2d(&tmO, boxp, colt / 2, row0);
+                    } else {
+                        tzp::tma_store_2d(&tmO, boxp, colt, row0);
+                        if (colt + 32 < p.n) tzp::tma_store_2d(&tmO, boxp + 2048, colt + 32, row0);
+                    }
+                    tzp::bulk_commit();
+                }
             }
             if (++acc == 2) {
                 acc = 0;
@@ -490,6 +483,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
         if (lane == 0) tzp::bulk_wait_all();
     }
 
+    tzp::pdl_trigger();
     tzp::tc_fence_before();
     __syncthreads();
     if constexpr (CG == 2) {
@@ -536,7 +530,7 @@ int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, 
         rc = encode_tmap_2d_swz(&mo, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, y, cols, a.rows, cols * 4, 32, 32, S128);
     else
         rc = encode_tmap_2d_swz(&mo, OUT == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, y, cols, a.rows,
-                                cols * 2, GATED ? 16 : 32, 32, GATED ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
+                                cols * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc) return rc;
     MxParams p{};
     p.m_tiles = ceil_div(a.rows, 128 * kCG);
@@ -558,7 +552,7 @@ template <int DT, int G>
 int launch_quant(tz_ctx_t ctx, const void* x, int64_t ldx, void* codes, void* scales, int64_t rows, int cols, int off, cudaStream_t s) {
     const long long warps = rows * ceil_div(cols, 256);
     const long long want = (warps + 7) / 8, most = static_cast<long long>(ctx->sm_count) * 8 * 4;
-    return launch_kernel(quantize_mxfp4_kernel<DT, G>, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, s, true, x,
+    return launch_kernel(quantize_mxfp4_kernel<DT, G>, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, s, false, x,
                          static_cast<long long>(ldx), static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), static_cast<long long>(rows),
                          cols, off);
 }
@@ -632,7 +626,7 @@ int tz_dequantize_mxfp4(tz_ctx_t ctx, const void* codes, const void* scales, voi
     const long long n8 = rows * (cols / 8), want = (n8 + 255) / 256, most = static_cast<long long>(ctx->sm_count) * 32;
     const dim3 grid(static_cast<unsigned>(want < most ? want : most));
     auto* kern = dtype == DT_F32 ? dequantize_mxfp4_kernel<DT_F32> : dtype == DT_F16 ? dequantize_mxfp4_kernel<DT_F16> : dequantize_mxfp4_kernel<DT_BF16>;
-    return launch_kernel(kern, grid, dim3(256), 0, pick_stream(ctx, stream), true, static_cast<const uint8_t*>(codes),
+    return launch_kernel(kern, grid, dim3(256), 0, pick_stream(ctx, stream), false, static_cast<const uint8_t*>(codes),
                          static_cast<const uint8_t*>(scales), out, static_cast<long long>(rows), cols);
 }
 

@@ -28,8 +28,11 @@ __device__ __forceinline__ uint32_t mapa(const void* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Arrival on the barrier at a cluster address.  Relaxed: it releases TMEM that this thread has read, which
+// tcgen05.wait::ld and tcgen05.fence::before_thread_sync order; a release at cluster scope would hold the warp
+// until its earlier memory operations are done (1500 of the 5000 clocks of a gated tile's epilogue).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar_addr, uint32_t parity) {
     uint32_t ok;
@@ -138,6 +141,12 @@ __device__ __forceinline__ uint64_t sdesc_mn128(uint32_t smem_addr, uint32_t lbo
 namespace tz {
 
 // launch_kernel with a cluster of `cg` CTAs (grid.x a multiple of cg).
+//
+// Programmatic launches and progress: CTAs that wait in griddepcontrol.wait hold their SM's threads and
+// registers.  If small CTAs of a later kernel got there while clusters of the awaited kernel were still to be
+// placed, they could take every slot that such a cluster needs, and both would wait for good.  So the cluster
+// kernels call launch_dependents only when a CTA's work is done, and the small kernels around them
+// (quantisers, partial sums) are launched without the attribute.
 template <typename... KArgs, typename... Args>
 int launch_cluster(void (*kern)(KArgs...), int cg, dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl,
                    Args&&... args) {
