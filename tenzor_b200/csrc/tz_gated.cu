@@ -38,6 +38,8 @@ struct MmParams {
     int kblocks;           // K blocks of 64, both halves for DX
     int half;              // DX: K blocks of one half
     int kper;              // K blocks per split
+    int ring;              // shared-memory stages in use
+    int resident;          // dual forms: the column block's B tiles stay in shared memory (see launch_mm)
     int m_pad;             // rows of one partial sum
     int cols;              // of the output
     int act;
@@ -55,11 +57,14 @@ struct MmCfg {
     static constexpr int STAGE = A_BYTES + BNC * 128;
     static constexpr int BOX = MODE == MM_FWD ? 2048 : 4096;  // staging of one epilogue warp
     static constexpr int STAGING = EPI * BOX;
-    static constexpr int BUDGET = 227 * 1024 - 1024 - 512 - STAGING;
+    static constexpr int BUDGET = (227 * 1024 - 1024 - 512 - STAGING) / 1024 * 1024;
     static constexpr int STAGES = BUDGET / STAGE > 8 ? 8 : BUDGET / STAGE;
-    static constexpr int SMEM = STAGES * STAGE + STAGING + 512 + 1024;
+    static constexpr int SMEM = BUDGET + STAGING + 512 + 1024;
+    static constexpr int ACCS = BN == 384 ? 1 : 2;  // accumulators in TMEM
+    static constexpr int TCOLS = BN == 384 ? 512 : 2 * BN;
     static_assert(!kDual || BN == 256, "16 epilogue warps of 32 output columns");
     static_assert(!kBmn || BNC % 64 == 0, "MN-major B comes in blocks of 64");
+    static_assert(BN == 256 || (BN == 384 && kBmn && CG == 2), "384 columns: two MMAs of 256 and 128");
 };
 
 // 16 gate / up pairs -> 8 words of 16-bit outputs.
@@ -117,7 +122,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = tzp::smem_u32(smem_raw);
     uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
-    uint8_t* staging = smem + STAGES * C::STAGE;
+    uint8_t* staging = smem + C::BUDGET;
     uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::STAGING);
     uint64_t* empty = full + STAGES;
     uint64_t* tfull = empty + STAGES;
@@ -147,7 +152,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         tzp::tma_prefetch_desc(&tmA0);
         tzp::tma_prefetch_desc(&tmB0);
     }
-    if (warp == 1) tzp::pair_tmem_alloc<CG>(tmem_slot, 2 * BN);
+    if (warp == 1) tzp::pair_tmem_alloc<CG>(tmem_slot, C::TCOLS);
     tzp::tc_fence_before();
     __syncthreads();
     if constexpr (CG == 2) tzp::cluster_sync();  // both CTAs' barriers exist before either signals them
@@ -155,15 +160,29 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     const uint32_t tmem_base = *tmem_slot;
     tzp::pdl_wait();
 
-    // Tile t of this launch: a group of 8 row blocks walks all column blocks before the next group starts, so
-    // that the CTAs running at one time share both operands in L2.
+    // Tile i of this CTA (pair).  Round-robin over the tiles: a group of 8 row blocks walks all column blocks
+    // before the next group starts, so that the CTAs running at one time share both operands in L2.  With
+    // resident B tiles: a contiguous range of the tiles in column-block order, so that the column block changes
+    // rarely.
     const int per = p.m_tiles * p.n_tiles;
     const int num_tiles = per * p.which * p.splits;
     struct Tile {
         int m, n, w, s, kb0, kb1;
     };
-    auto tile_of = [&](int t) {
-        Tile r;
+    const int me = static_cast<int>(blockIdx.x) / CG, team = static_cast<int>(gridDim.x) / CG;
+    const int first = p.resident ? static_cast<int>(static_cast<long long>(num_tiles) * me / team) : 0;
+    const int last = p.resident ? static_cast<int>(static_cast<long long>(num_tiles) * (me + 1) / team) : 0;
+    auto tile_at = [&](int i, Tile& r) -> bool {
+        if (C::kDual && p.resident) {
+            const int t = first + i;
+            r.n = t / p.m_tiles;
+            r.m = t - r.n * p.m_tiles;
+            r.w = r.s = r.kb0 = 0;
+            r.kb1 = p.kblocks;
+            return t < last;
+        }
+        int t = me + i * team;
+        if (t >= num_tiles) return false;
         r.s = t / (per * p.which);
         t -= r.s * per * p.which;
         r.w = t / per;
@@ -176,9 +195,23 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         r.n = t / gm;
         r.kb0 = r.s * p.kper;
         r.kb1 = min(p.kblocks, r.kb0 + p.kper);
-        return r;
+        return true;
     };
-    const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
+    const int ring = p.ring;
+    // Shared memory: stage s holds an A tile and a B tile; with resident B tiles a ring of A tiles comes first,
+    // then the B tile of every K block.
+    const uint32_t sbase = tzp::smem_u32(smem);
+    const uint32_t a_step = C::kDual && p.resident ? C::A_BYTES : C::STAGE;
+    auto b_addr = [&](int stage, int kb) {
+        return C::kDual && p.resident ? sbase + ring * C::A_BYTES + kb * (C::BNC * 128) : sbase + stage * C::STAGE + C::A_BYTES;
+    };
+
+    // Column of this CTA's j-th block of 64 of an MN-major B tile.  384 columns are two MMAs: the first takes
+    // blocks 0 and 1 of both CTAs (256 columns), the second block 2 (128).
+    auto b_col = [&](int n, int j) {
+        const int r = static_cast<int>(rank);
+        return n * BN + (BN == 384 ? (j < 2 ? 128 * r + 64 * j : 256 + 64 * r) : r * C::BNC + 64 * j);
+    };
 
     if (warp == 0) {
         if (lane == 0) {
@@ -186,8 +219,14 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             int stage = 0;
             uint32_t phase = 0, armed = 0, armed_par = 0;
             bool ok = true;
-            for (int t = t0; ok && t < num_tiles; t += tstep) {
-                const Tile q = tile_of(t);
+            Tile q;
+            int n_res = -1;  // the column block whose B tiles are resident
+            for (int i = 0; ok && tile_at(i, q); ++i) {
+                // A B tile is overwritten when its column block is done: the K block that used it last is `kblocks`
+                // uses back, and the wait below covers `ring` <= kblocks uses.
+                const bool need_b = !(C::kDual && p.resident) || q.n != n_res;
+                n_res = q.n;
+                const uint32_t bytes = CG * (need_b ? C::STAGE : C::A_BYTES);
                 const int m0 = (q.m * CG + static_cast<int>(rank)) * 128;
                 for (int kb = q.kb0; kb < q.kb1; ++kb) {
                     if (!tzp::pair_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
@@ -195,37 +234,38 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                         break;
                     }
                     if (rank == 0) {
-                        tzp::mbar_arrive_expect_tx(&full[stage], CG * C::STAGE);
+                        tzp::mbar_arrive_expect_tx(&full[stage], bytes);
                         armed |= 1u << stage;
                         armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
                     }
                     const uint32_t bar = CG == 2 ? tzp::mapa(&full[stage], 0) : tzp::smem_u32(&full[stage]);
-                    const uint32_t sa = tzp::smem_u32(smem + stage * C::STAGE);
-                    const uint32_t sb = sa + C::A_BYTES;
+                    const uint32_t sa = sbase + stage * a_step;
+                    const uint32_t sb = b_addr(stage, kb);
                     if constexpr (MODE == MM_DW) {
                         const CUtensorMap* ta = q.w ? &tmA1 : &tmA0;
                         tzp::pair_load_2d<CG>(sa, ta, m0, kb * 64, bar);
                         tzp::pair_load_2d<CG>(sa + 8192, ta, m0 + 64, kb * 64, bar);
 #pragma unroll
                         for (int j = 0; j < C::BNC / 64; ++j)
-                            tzp::pair_load_2d<CG>(sb + j * 8192, &tmB0, q.n * BN + static_cast<int>(rank) * C::BNC + 64 * j, kb * 64, bar);
+                            tzp::pair_load_2d<CG>(sb + j * 8192, &tmB0, b_col(q.n, j), kb * 64, bar);
                     } else if constexpr (MODE == MM_DX) {
                         const bool up = kb >= p.half;
                         const int k = (up ? kb - p.half : kb) * 64;
                         tzp::pair_load_2d<CG>(sa, up ? &tmA1 : &tmA0, k, m0, bar);
 #pragma unroll
                         for (int j = 0; j < C::BNC / 64; ++j)
-                            tzp::pair_load_2d<CG>(sb + j * 8192, up ? &tmB1 : &tmB0, q.n * BN + static_cast<int>(rank) * C::BNC + 64 * j, k, bar);
+                            tzp::pair_load_2d<CG>(sb + j * 8192, up ? &tmB1 : &tmB0, b_col(q.n, j), k, bar);
                     } else {
                         tzp::pair_load_2d<CG>(sa, &tmA0, kb * 64, m0, bar);
-                        if constexpr (CG == 2) {
+                        if (!need_b) {
+                        } else if constexpr (CG == 2) {
                             tzp::pair_load_2d<CG>(sb, rank ? &tmB1 : &tmB0, kb * 64, q.n * (BN / 2), bar);
                         } else {
                             tzp::pair_load_2d<CG>(sb, &tmB0, kb * 64, q.n * (BN / 2), bar);
                             tzp::pair_load_2d<CG>(sb + (BN / 2) * 128, &tmB1, kb * 64, q.n * (BN / 2), bar);
                         }
                     }
-                    if (++stage == STAGES) {
+                    if (++stage == ring) {
                         stage = 0;
                         phase ^= 1u;
                     }
@@ -238,13 +278,15 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             // ---- MMA issuer ----
-            constexpr uint32_t idesc = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, BN) | (C::kAmn ? 1u << 15 : 0u) | (C::kBmn ? 1u << 16 : 0u);
+            constexpr uint32_t major = (C::kAmn ? 1u << 15 : 0u) | (C::kBmn ? 1u << 16 : 0u);
+            constexpr uint32_t idesc = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 256) | major;
+            constexpr uint32_t idesc_b = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 128) | major;  // columns 256 .. 383
             constexpr uint32_t kAstep = C::kAmn ? 2048u >> 4 : 2u, kBstep = C::kBmn ? 2048u >> 4 : 2u;
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
-            for (int t = t0; ok && t < num_tiles; t += tstep) {
-                const Tile q = tile_of(t);
+            Tile q;
+            for (int i = 0; ok && tile_at(i, q); ++i) {
                 if (!tzp::pair_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
@@ -254,21 +296,25 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                         break;
                     }
                     tzp::tc_fence_after();
-                    const uint32_t sa = tzp::smem_u32(smem + stage * C::STAGE);
+                    const uint32_t sa = sbase + stage * a_step;
+                    const uint32_t sb = b_addr(stage, kb);
                     const uint64_t ad = C::kAmn ? tzp::sdesc_mn128(sa, 8192) : tzp::sdesc_k128(sa);
-                    const uint64_t bd = C::kBmn ? tzp::sdesc_mn128(sa + C::A_BYTES, 8192) : tzp::sdesc_k128(sa + C::A_BYTES);
+                    const uint64_t bd = C::kBmn ? tzp::sdesc_mn128(sb, 8192) : tzp::sdesc_k128(sb);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        tzp::pair_mma_f16<CG>(d, ad + kAstep * k, bd + kBstep * k, idesc, (kb > q.kb0 || k > 0) ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t more = (kb > q.kb0 || k > 0) ? 1u : 0u;
+                        tzp::pair_mma_f16<CG>(d, ad + kAstep * k, bd + kBstep * k, idesc, more);
+                        if constexpr (BN == 384) tzp::pair_mma_f16<CG>(d + 256, ad + kAstep * k, bd + (16384u >> 4) + kBstep * k, idesc_b, more);
+                    }
                     tzp::pair_commit<CG>(&empty[stage]);
-                    if (++stage == STAGES) {
+                    if (++stage == ring) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
                 tzp::pair_commit<CG>(&tfull[acc]);
-                if (++acc == 2) {
+                if (++acc == C::ACCS) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
@@ -287,17 +333,19 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         uint32_t acc_phase = 0, dh_phase = 0;
         // BWD: the 32 x 32 box of dh that a tile needs comes by TMA into the box that later takes dg; it is asked
         // for as soon as the previous tile's stores have read the box.
-        auto fetch_dh = [&](int t) {
-            const Tile q = tile_of(t);
+        auto fetch_dh = [&](const Tile& q) {
             tzp::mbar_arrive_expect_tx(&dhbar[e], 2048);
             tzp::tma_load_2d(boxp, &tmDh, q.n * (BN / 2) + sl * 32, (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32, &dhbar[e]);
         };
+        Tile q, next;
+        bool more = tile_at(0, next), fetched = false;
         if constexpr (MODE == MM_BWD) {
-            if (lane == 0 && t0 < num_tiles) fetch_dh(t0);
+            fetched = more;
+            if (lane == 0 && more) fetch_dh(next);
         }
-        bool fetched = MODE == MM_BWD && t0 < num_tiles;
-        for (int t = t0; t < num_tiles; t += tstep) {
-            const Tile q = tile_of(t);
+        for (int i = 1; more; ++i) {
+            q = next;
+            more = tile_at(i, next);
             if (!tzp::pair_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
             tzp::tc_fence_after();
             const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN);
@@ -359,11 +407,11 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                     }
                     if constexpr (MODE == MM_BWD) {
                         tzp::bulk_wait_read<0>();
-                        if (t + tstep < num_tiles) fetch_dh(t + tstep);
+                        if (more) fetch_dh(next);
                     }
                 }
                 __syncwarp();
-                if constexpr (MODE == MM_BWD) fetched = t + tstep < num_tiles;
+                if constexpr (MODE == MM_BWD) fetched = more;
             } else {
                 constexpr int CH = BN / 64;
 #pragma unroll 1
@@ -411,7 +459,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                         tzp::mbar_arrive(&tempty[acc]);
                 }
             }
-            if (++acc == 2) {
+            if (++acc == C::ACCS) {
                 acc = 0;
                 acc_phase ^= 1u;
             }
@@ -435,7 +483,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     if (warp == 1) {
         __syncwarp();
         tzp::tc_fence_after();
-        tzp::pair_tmem_dealloc<CG>(tmem_base, 2 * BN);
+        tzp::pair_tmem_dealloc<CG>(tmem_base, C::TCOLS);
     }
 }
 
@@ -472,7 +520,7 @@ int map16(CUtensorMap* m, const Mat& a, int box_cols, int box_rows, CUtensorMapS
 
 template <int CG, int BN, int MODE, bool BF, bool PART>
 int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, const Mat& o0, const Mat& o1, const Mat* dh,
-              const MmParams& p, float* part, cudaStream_t s) {
+              MmParams p, float* part, cudaStream_t s) {
     using C = MmCfg<CG, BN, MODE>;
     auto kern = gated_mm_kernel<CG, BN, MODE, BF, PART>;
     static std::atomic<unsigned> done{0};
@@ -499,6 +547,19 @@ int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const M
     const int groups = (ctx->sm_count - ctx->sm_reserve) / CG;
     const int grid = static_cast<int>(tiles < groups ? tiles : groups) * CG;
     TZ_CHECK(grid > 0, TZ_EINVAL, "gated kernels need %d free SMs", CG);
+    p.ring = C::STAGES;
+    if (C::kDual && tiles > groups && p.kblocks >= 4) {
+        // Short sums: the B tiles of a whole column block fit beside a ring of A tiles, and keeping them halves what
+        // an SM moves from L2 per tile, which bounds these shapes.  Below 4 K blocks the ring (at most kblocks long)
+        // would be too short; above, it has to keep 3 A tiles.
+        const int left = (C::BUDGET - p.kblocks * C::BNC * 128) / C::A_BYTES;
+        int r = left < p.kblocks ? left : p.kblocks;
+        if (r > C::STAGES) r = C::STAGES;
+        if (r >= 3) {
+            p.resident = 1;
+            p.ring = r;
+        }
+    }
     return launch_cluster(kern, CG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma0, ma1, mb0, mb1, mo0, mo1, mdh, p, ctx->d_status);
 }
 
@@ -506,29 +567,47 @@ constexpr int kCG = 2, kBN = 256;
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
-// Splits of the K blocks so that the tiles fill the GPU, each with at least 8 K blocks.
-int pick_splits(int sms, int64_t tiles, int kblocks) {
-    const int groups = sms / kCG;
-    int s = static_cast<int>(groups / (tiles < 1 ? 1 : tiles));
-    if (s > kblocks / 8) s = kblocks / 8;
-    if (s > 16) s = 16;
-    if (s <= 1) return 1;
-    return ceil_div(kblocks, ceil_div(kblocks, s));  // no split without K blocks
+// Tile width and splits of the sum of a DX or DW product, by an estimate in clocks: rounds of tiles over the
+// pairs, each K block at the rate the operands arrive at (256 columns: 32 KB per SM, 384: 40 KB), a start and an
+// epilogue per round (not hidden with one accumulator), and the partial sums' way out and back.
+struct Split {
+    int bn, splits;
+};
+Split pick_split(int sms, int64_t m_tiles, int which, int64_t rows, int64_t cols, int kblocks) {
+    const int64_t groups = sms / kCG > 0 ? sms / kCG : 1;
+    Split best{256, 1};
+    if (kblocks < 1) return best;  // no tokens
+    double best_cost = 1e300;
+    for (int bn = 256; bn <= 384; bn += 128) {
+        const int64_t tiles = m_tiles * which * ceil_div(cols, bn);
+        for (int sp = 1; sp <= 16; ++sp) {
+            if (sp > 1 && (kblocks / sp < 8 || tiles * sp > groups)) break;
+            const int per = ceil_div(kblocks, sp);
+            if (ceil_div(kblocks, per) != sp) continue;  // every split has work
+            double cost = static_cast<double>(ceil_div(tiles * sp, groups)) * (bn == 256 ? per * 600.0 + 2500.0 : per * 820.0 + 5000.0);
+            if (sp > 1) cost += 6000.0 + static_cast<double>(sp) * which * rows * cols * 8.0 / 2500.0;
+            if (cost < best_cost) {
+                best_cost = cost;
+                best = {bn, sp};
+            }
+        }
+    }
+    return best;
 }
 
 struct BwdPlan {
     size_t dgdu, part_dx, part_dw;  // bytes
-    int s_dx, s_dw;
+    Split dx, dw;
 };
 BwdPlan plan_bwd(int sms, int64_t T, int64_t D, int64_t F) {
     BwdPlan b{};
     auto a256 = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
     b.dgdu = a256(static_cast<size_t>(T) * F * 2);
-    const int mt = ceil_div(T, 128 * kCG), nt = ceil_div(D, kBN), ft = ceil_div(F, 128 * kCG);
-    b.s_dx = pick_splits(sms, static_cast<int64_t>(mt) * nt, 2 * ceil_div(F, 64));
-    b.s_dw = pick_splits(sms, 2ll * ft * nt, ceil_div(T, 64));
-    if (b.s_dx > 1) b.part_dx = a256(static_cast<size_t>(b.s_dx) * mt * 128 * kCG * D * 4);
-    if (b.s_dw > 1) b.part_dw = a256(static_cast<size_t>(b.s_dw) * 2 * ft * 128 * kCG * D * 4);
+    const int mt = ceil_div(T, 128 * kCG), ft = ceil_div(F, 128 * kCG);
+    b.dx = pick_split(sms, mt, 1, T, D, 2 * ceil_div(F, 64));
+    b.dw = pick_split(sms, ft, 2, F, D, ceil_div(T, 64));
+    if (b.dx.splits > 1) b.part_dx = a256(static_cast<size_t>(b.dx.splits) * mt * 128 * kCG * D * 4);
+    if (b.dw.splits > 1) b.part_dw = a256(static_cast<size_t>(b.dw.splits) * 2 * ft * 128 * kCG * D * 4);
     return b;
 }
 
@@ -537,6 +616,16 @@ int sum_parts(tz_ctx_t ctx, const float* part, void* o0, void* o1, int which, in
     const long long n8 = static_cast<long long>(rows) * cols / 8 * which;
     const int blocks = static_cast<int>(n8 / 256 + 1 < ctx->sm_count * 8 ? n8 / 256 + 1 : ctx->sm_count * 8);
     return launch_kernel(sum_parts_kernel<BF>, dim3(blocks), dim3(256), 0, s, false, part, o0, o1, which, splits, m_pad, rows, cols);
+}
+
+template <int MODE, bool BF>
+int launch_any(tz_ctx_t ctx, const Split& w, const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, const Mat& o0, const Mat& o1,
+               const MmParams& p, float* part, cudaStream_t s) {
+    if (w.bn == 384)
+        return p.splits > 1 ? launch_mm<kCG, 384, MODE, BF, true>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, part, s)
+                            : launch_mm<kCG, 384, MODE, BF, false>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, nullptr, s);
+    return p.splits > 1 ? launch_mm<kCG, kBN, MODE, BF, true>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, part, s)
+                        : launch_mm<kCG, kBN, MODE, BF, false>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, nullptr, s);
 }
 
 template <bool BF>
@@ -571,37 +660,32 @@ int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat
 
     MmParams q{};
     q.m_tiles = ceil_div(T, 128 * kCG);
-    q.n_tiles = ceil_div(D, kBN);
+    q.n_tiles = ceil_div(D, b.dx.bn);
     q.which = 1;
-    q.splits = b.s_dx;
+    q.splits = b.dx.splits;
     q.half = ceil_div(F, 64);
     q.kblocks = 2 * q.half;
     q.kper = ceil_div(q.kblocks, q.splits);
     q.m_pad = q.m_tiles * 128 * kCG;
     q.cols = static_cast<int>(D);
-    if (q.splits > 1) {
-        rc = launch_mm<kCG, kBN, MM_DX, BF, true>(ctx, dg, du, wg, wu, dx, dx, nullptr, q, part_dx, s);
-        if (!rc) rc = sum_parts<BF>(ctx, part_dx, const_cast<void*>(dx.p), nullptr, 1, q.splits, q.m_pad, static_cast<int>(T), q.cols, s);
-    } else {
-        rc = launch_mm<kCG, kBN, MM_DX, BF, false>(ctx, dg, du, wg, wu, dx, dx, nullptr, q, nullptr, s);
-    }
+    rc = launch_any<MM_DX, BF>(ctx, b.dx, dg, du, wg, wu, dx, dx, q, part_dx, s);
+    if (!rc && q.splits > 1)
+        rc = sum_parts<BF>(ctx, part_dx, const_cast<void*>(dx.p), nullptr, 1, q.splits, q.m_pad, static_cast<int>(T), q.cols, s);
     if (rc) return rc;
 
     MmParams r{};
     r.m_tiles = ceil_div(F, 128 * kCG);
-    r.n_tiles = ceil_div(D, kBN);
+    r.n_tiles = ceil_div(D, b.dw.bn);
     r.which = 2;
-    r.splits = b.s_dw;
+    r.splits = b.dw.splits;
     r.kblocks = ceil_div(T, 64);
     r.kper = ceil_div(r.kblocks, r.splits);
     r.m_pad = r.m_tiles * 128 * kCG;
     r.cols = static_cast<int>(D);
-    if (r.splits > 1) {
-        rc = launch_mm<kCG, kBN, MM_DW, BF, true>(ctx, dg, du, x, x, dwg, dwu, nullptr, r, part_dw, s);
-        if (!rc) rc = sum_parts<BF>(ctx, part_dw, const_cast<void*>(dwg.p), const_cast<void*>(dwu.p), 2, r.splits, r.m_pad, static_cast<int>(F), r.cols, s);
-        return rc;
-    }
-    return launch_mm<kCG, kBN, MM_DW, BF, false>(ctx, dg, du, x, x, dwg, dwu, nullptr, r, nullptr, s);
+    rc = launch_any<MM_DW, BF>(ctx, b.dw, dg, du, x, x, dwg, dwu, r, part_dw, s);
+    if (!rc && r.splits > 1)
+        rc = sum_parts<BF>(ctx, part_dw, const_cast<void*>(dwg.p), const_cast<void*>(dwu.p), 2, r.splits, r.m_pad, static_cast<int>(F), r.cols, s);
+    return rc;
 }
 
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
