@@ -23,6 +23,7 @@
 #include <cuda_runtime.h>
 
 #include "tz_act.cuh"
+#include "tz_gated_rows.cuh"
 #include "tz_internal.h"
 #include "tz_pair.cuh"
 
@@ -564,6 +565,10 @@ int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const M
 }
 
 constexpr int kCG = 2, kBN = 256;
+// Tokens up to which the forward pass streams weights (gated_rows_kernel).  At 32 tokens it takes 5.2 / 10.2 /
+// 14.5 / 26.8 us at (D, F) = (384, 1536) / (1024, 4096) / (2048, 6144) / (4096, 8192), the tiles of 256 tokens 6.5
+// / 10.4 / 16.1 / 29.2; with room for 64 tokens it takes 6.5 / 14.2 / 16.9 / 29.1.
+constexpr int kRowsMax = 32;
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -628,8 +633,35 @@ int launch_any(tz_ctx_t ctx, const Split& w, const Mat& a0, const Mat& a1, const
                         : launch_mm<kCG, kBN, MODE, BF, false>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, nullptr, s);
 }
 
+template <int N, bool BF>
+int launch_rows(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& h, int act, cudaStream_t s) {
+    using C = RowsCfg<N>;
+    auto kern = gated_rows_kernel<N, BF>;
+    static std::atomic<unsigned> done{0};
+    int rc = ensure_smem(kern, C::SMEM, done);
+    if (rc) return rc;
+    CUtensorMap mx, mg, mu;
+    const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B;
+    if ((rc = map16<BF>(&mx, x, 64, N, S128)) || (rc = map16<BF>(&mg, wg, 64, 128, S128)) || (rc = map16<BF>(&mu, wu, 64, 128, S128))) return rc;
+    RowsParams p{};
+    const int tiles = ceil_div(h.cols, 128);
+    p.kblocks = ceil_div(x.cols, 64);
+    int splits = 1;
+    if ((rc = rows_splits<N>(kern, C::THREADS, C::SMEM, ctx->sm_count - ctx->sm_reserve, tiles, p.kblocks, C::MAX_SPLIT, &splits))) return rc;
+    p.kper = ceil_div(p.kblocks, splits);
+    p.t = static_cast<int>(x.rows);
+    p.f = static_cast<int>(h.cols);
+    p.act = act;
+    p.h = const_cast<void*>(h.p);
+    return launch_cluster(kern, splits, dim3(splits, tiles), dim3(C::THREADS), C::SMEM, s, true, mx, mg, mu, p, ctx->d_status);
+}
+
 template <bool BF>
 int forward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& h, int act, cudaStream_t s) {
+    if (x.rows <= kRowsMax && h.cols <= 128 * 65535) {  // the grid's second extent
+        if (x.rows <= 16) return launch_rows<16, BF>(ctx, x, wg, wu, h, act, s);
+        return launch_rows<32, BF>(ctx, x, wg, wu, h, act, s);
+    }
     MmParams p{};
     p.m_tiles = ceil_div(x.rows, 128 * kCG);
     p.n_tiles = ceil_div(h.cols, kBN / 2);

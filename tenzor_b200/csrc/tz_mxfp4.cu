@@ -17,6 +17,7 @@
 #include <cuda_runtime.h>
 
 #include "tz_act.cuh"
+#include "tz_gated_rows.cuh"
 #include "tz_internal.h"
 #include "tz_pair.cuh"
 
@@ -500,7 +501,228 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
     }
 }
 
+// ---- few rows (serving) ----------------------------------------------------------------------------
+// The product for up to 32 rows of x, bound by reading the 4-bit weights once.  As in gated_rows_kernel the weights
+// are the A operand (128 of their rows: M) and the rows of x the B operand (N = 16 or 32), and the K blocks of a
+// tile are split over a cluster.  x is quantised inside the kernel, straight into the MMA's operand layout: each
+// CTA needs its K slice only, so the work (0.5 us for 16 rows of 4096) hides behind the first weight copies and the
+// separate quantiser launch goes away.  With GATED a warp's 32 TMEM lanes are 16 gate rows and their 16 up rows.
+struct MxRowsParams {
+    const void* x;
+    long long ldx;
+    void* y;
+    const float* bias;
+    int rows, k, n;      // of x, of a row, weight rows
+    int k_chunks, kblocks, kper;
+    int act;
+};
+
+template <int N>
+struct MxRowsCfg {
+    static constexpr int QWARPS = 8;
+    static constexpr int THREADS = 64 + 32 * QWARPS;
+    static constexpr int STAGE = 16384 + 1024;
+    static constexpr int STAGES = 5;
+    static constexpr int SF_COLS = 16;           // per stage: A 2 x 4, B 2 x 4
+    static constexpr int SF0 = 32;
+    static constexpr int TCOLS = 128;            // 32 + 5 * 16 = 112
+    static constexpr int B_KB = N * 128 + 1024;  // one K block of x: codes and two scale chunks
+    static constexpr int PART = 128 * N * 4;
+    static constexpr int MAX_SPLIT = 1 + STAGES * STAGE / PART;
+    static constexpr int MAX_KB = (227 * 1024 - 2048 - STAGES * STAGE) / B_KB < 32 ? (227 * 1024 - 2048 - STAGES * STAGE) / B_KB : 32;
+    static constexpr int smem(int kper) { return STAGES * STAGE + kper * B_KB + 1024 + 1024; }
+};
+
+template <int N, int XDT, int OUT, bool GATED>
+__global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
+    mxfp4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW, const MxRowsParams p, int* status) {
+    using C = MxRowsCfg<N>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (tzp::smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* xq = smem + STAGES * C::STAGE;  // [K block][codes N x 128 swizzled | 2 scale chunks]
+    uint64_t* full = reinterpret_cast<uint64_t*>(xq + p.kper * C::B_KB);
+    uint64_t* empty = full + STAGES;
+    uint64_t* done = empty + STAGES;
+    uint64_t* xready = done + 1;  // one per K block of this CTA (at most 32)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xready + 32);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(tzp::cluster_ctarank());
+    const int n0 = static_cast<int>(blockIdx.y) * 128;
+    const int kb0 = rank * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tzp::mbar_init(&full[s], 1);
+            tzp::mbar_init(&empty[s], 1);
+        }
+        tzp::mbar_init(done, 1);
+        for (int i = 0; i < 32; ++i) tzp::mbar_init(&xready[i], C::QWARPS);
+        *abort_flag = 0;
+        tzp::fence_mbar_init();
+        tzp::tma_prefetch_desc(&tmW);
+        tzp::tma_prefetch_desc(&tmSW);
+    }
+    if (warp == 1) {
+        tzp::tmem_alloc(tmem_slot, C::TCOLS);
+        tzp::tmem_relinquish();
+    }
+    tzp::tc_fence_before();
+    __syncthreads();
+    tzp::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    tzp::pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t armed = 0, armed_par = 0;
+            for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+                const int s = i % STAGES;
+                const uint32_t phase = (i / STAGES) & 1;
+                if (!tzp::mbar_wait(&empty[s], phase ^ 1u, status, abort_flag)) break;
+                uint8_t* a = smem + s * C::STAGE;
+                tzp::mbar_arrive_expect_tx(&full[s], C::STAGE);
+                armed |= 1u << s;
+                armed_par = (armed_par & ~(1u << s)) | (phase << s);
+                tzp::tma_load_2d(a, &tmW, kb * 128, n0, &full[s]);
+                tzp::tma_load_2d(a + 16384, &tmSW, 0, static_cast<int>(blockIdx.y) * p.k_chunks + 2 * kb, &full[s]);
+            }
+            for (int s = 0; s < STAGES; ++s)  // every copy has landed before the stages are used again (bounded)
+                if (armed & (1u << s)) tzp::mbar_wait(&full[s], (armed_par >> s) & 1u, status, nullptr);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc0 = mx_idesc(128, N, 0), idesc2 = mx_idesc(128, N, 2);
+            for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+                const int s = i % STAGES;
+                if (!tzp::mbar_wait(&xready[i], 0, status, abort_flag)) break;
+                if (!tzp::mbar_wait(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
+                tzp::tc_fence_after();
+                const uint32_t a = tzp::smem_u32(smem + s * C::STAGE), b = tzp::smem_u32(xq + i * C::B_KB);
+                const uint32_t tsf = tmem_base + static_cast<uint32_t>(C::SF0 + s * C::SF_COLS);
+                const int left = p.k - kb * 256;
+                sf_copy<1>(tsf, a + 16384);
+                sf_copy<1>(tsf + 8, b + N * 128);
+                if (left > 128) {
+                    sf_copy<1>(tsf + 4, a + 16384 + 512);
+                    sf_copy<1>(tsf + 12, b + N * 128 + 512);
+                }
+                const uint64_t ad = tzp::sdesc_k128(a), bd = tzp::sdesc_k128(b);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k == 0 || left > 64 * k)
+                        mx_mma<1>(tmem_base, ad + 2u * k, bd + 2u * k, (k & 1) ? idesc2 : idesc0, tsf + 4 * (k >> 1), tsf + 8 + 4 * (k >> 1),
+                                  (i | k) != 0 ? 1u : 0u);
+                tzp::umma_commit(&empty[s]);
+            }
+            tzp::umma_commit(done);
+            tzp::mbar_wait(done, 0, status, nullptr);
+        }
+    } else {
+        // ---- quantise this CTA's K slice of x, one K block (256 values of N rows) after the other; a warp takes a
+        // row of the block, a lane 8 values.  Rows past the last one are zeros with the smallest scale. ----
+        for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+            uint8_t* blk = xq + i * C::B_KB;
+            const int c = kb * 256 + lane * 8;
+#pragma unroll
+            for (int j = 0; j < N / C::QWARPS; ++j) {
+                const int r = warp - 2 + j * C::QWARPS;
+                float v[8] = {};
+                if (r < p.rows && c < p.k) load8<XDT>(p.x, r * p.ldx + c, v);
+                uint32_t sc;
+                const uint32_t q = quant_block(v, sc);
+                // 4 bytes at byte 4 * lane of a 128-byte row, 128-byte swizzle (16-byte unit u at u ^ (r % 8))
+                *reinterpret_cast<uint32_t*>(blk + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = q;
+                uint32_t w = sc << (8 * ((lane >> 2) & 3));
+                w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+                w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
+                if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(blk + N * 128 + (lane >> 4) * 512 + r * 16) = w;
+            }
+            tzp::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tzp::mbar_arrive(&xready[i]);
+        }
+    }
+    // All products of this CTA are in its TMEM and its stages are free; then the same of every CTA.
+    tzp::tc_fence_before();
+    __syncthreads();
+    const bool split = p.kper < p.kblocks;
+    if (split) tzp::cluster_sync();
+    tzp::tc_fence_after();
+
+    const int q4 = warp & 3, row = q4 * 32 + lane;  // weight row n0 + row
+    float* part = reinterpret_cast<float*>(smem);   // [rank - 1][N][128]
+    const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16);
+    const bool epi = warp >= 2 && warp < 6;
+    if (rank > 0 && epi) {
+        const uint32_t dst = tzp::mapa(part + (rank - 1) * N * 128 + row, 0);
+#pragma unroll 1
+        for (int c = 0; c < N; c += 16) {
+            uint32_t v[16];
+            tzp::tmem_ld16(td + c, v);
+            tzp::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) st_cluster_f32(dst + (c + j) * 512, __uint_as_float(v[j]));
+        }
+    }
+    if (split) tzp::cluster_sync();
+    if (rank == 0 && epi) {
+        const int ranks = (p.kblocks + p.kper - 1) / p.kper;
+        const float bias = !GATED && p.bias && n0 + row < p.n ? __ldg(p.bias + n0 + row) : 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < N; c += 16) {
+            if (c >= p.rows) break;
+            uint32_t v[16];
+            tzp::tmem_ld16(td + c, v);
+            tzp::tmem_ld_wait();
+            for (int r = 1; r < ranks; ++r) {
+                const float* src = part + (r - 1) * N * 128 + row;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + src[(c + j) * 128]);
+            }
+            if constexpr (GATED) {
+                uint32_t u[16], o[8];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) u[j] = __shfl_down_sync(0xFFFFFFFFu, v[j], 16);
+#define TZ_G(A) \
+    for (int j = 0; j < 8; ++j) o[j] = gated_pair<A, OUT == DT_BF16>(v[2 * j], v[2 * j + 1], u[2 * j], u[2 * j + 1])
+                TZ_ACT_SWITCH(p.act, _Pragma("unroll") TZ_G)
+#undef TZ_G
+                const int f = (n0 + q4 * 32) / 2 + lane;
+                if (lane < 16 && 2 * f < p.n) {
+                    uint16_t* out = reinterpret_cast<uint16_t*>(p.y) + f;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (c + j < p.rows) out[static_cast<long long>(c + j) * (p.n / 2)] = static_cast<uint16_t>(o[j / 2] >> (16 * (j & 1)));
+                }
+            } else if (n0 + row < p.n) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (c + j >= p.rows) break;
+                    const float y = p.bias ? __uint_as_float(v[j]) + bias : __uint_as_float(v[j]);
+                    const long long o = static_cast<long long>(c + j) * p.n + n0 + row;
+                    if constexpr (OUT == DT_F32)
+                        reinterpret_cast<float*>(p.y)[o] = y;
+                    else if constexpr (OUT == DT_F16)
+                        reinterpret_cast<__half*>(p.y)[o] = __float2half_rn(y);
+                    else
+                        reinterpret_cast<__nv_bfloat16*>(p.y)[o] = __float2bfloat16_rn(y);
+                }
+            }
+        }
+    }
+    tzp::pdl_trigger();
+    tzp::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tzp::tc_fence_after();
+        tzp::tmem_dealloc(tmem_base, C::TCOLS);
+    }
+}
+
 constexpr int kCG = 2;
+constexpr int kRowsMax = 32;  // rows up to which the product streams weights (mxfp4_rows_kernel)
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -546,6 +768,59 @@ int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, 
     const int grid = static_cast<int>(tiles < groups ? tiles : groups) * kCG;
     TZ_CHECK(grid > 0, TZ_EINVAL, "mxfp4 kernels need %d free SMs", kCG);
     return launch_cluster(kern, kCG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma, mb, mo, msa, msb, p, ctx->d_status);
+}
+
+// The few-rows kernel, where its K slice of x fits shared memory; *ran says whether it did.
+template <int N, int XDT, int OUT, bool GATED>
+int launch_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int rows, const Q4& w, int k, const float* bias, void* y, int act, cudaStream_t s,
+                   bool* ran) {
+    using C = MxRowsCfg<N>;
+    auto kern = mxfp4_rows_kernel<N, XDT, OUT, GATED>;
+    const int tiles = ceil_div(w.rows, 128), kblocks = ceil_div(k, 256);
+    *ran = false;
+    if (tiles > 65535) return TZ_OK;  // the grid's second extent
+    static std::atomic<unsigned> done{0};
+    int rc = ensure_smem(kern, C::smem(C::MAX_KB), done);
+    if (rc) return rc;
+    int splits = 1;
+    if ((rc = rows_splits<N * 100 + XDT * 20 + OUT * 4 + GATED + 1>(kern, C::THREADS, C::smem(8), ctx->sm_count - ctx->sm_reserve, tiles, kblocks,
+                                                                    C::MAX_SPLIT, &splits)))
+        return rc;
+    MxRowsParams p{};
+    p.kblocks = kblocks;
+    p.kper = ceil_div(kblocks, splits);
+    if (p.kper > C::MAX_KB) return TZ_OK;
+    p.x = x;
+    p.ldx = ldx;
+    p.y = y;
+    p.bias = bias;
+    p.rows = rows;
+    p.k = k;
+    p.n = static_cast<int>(w.rows);
+    p.k_chunks = ceil_div(k, 128);
+    p.act = act;
+    CUtensorMap mw, msw;
+    if ((rc = encode_tmap_2d_swz(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.codes, k / 2, w.rows, k / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)) ||
+        (rc = encode_tmap_2d_swz(&msw, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, w.scales, 128, static_cast<uint64_t>(tiles) * p.k_chunks, 512, 128, 2,
+                                 CU_TENSOR_MAP_SWIZZLE_NONE)))
+        return rc;
+    *ran = true;
+    return launch_cluster(kern, splits, dim3(splits, tiles), dim3(C::THREADS), C::smem(p.kper), s, true, mw, msw, p, ctx->d_status);
+}
+template <int XDT, int OUT, bool GATED>
+int try_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int64_t rows, const Q4& w, int k, const float* bias, void* y, int act, cudaStream_t s,
+                bool* ran) {
+    *ran = false;
+    if (rows > kRowsMax) return TZ_OK;
+    return rows <= 16 ? launch_mx_rows<16, XDT, OUT, GATED>(ctx, x, ldx, static_cast<int>(rows), w, k, bias, y, act, s, ran)
+                      : launch_mx_rows<32, XDT, OUT, GATED>(ctx, x, ldx, static_cast<int>(rows), w, k, bias, y, act, s, ran);
+}
+template <int OUT>
+int try_mx_rows_x(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, int64_t rows, const Q4& w, int k, const float* bias, void* y,
+                  cudaStream_t s, bool* ran) {
+    if (x_dtype == DT_F32) return try_mx_rows<DT_F32, OUT, false>(ctx, x, ldx, rows, w, k, bias, y, 0, s, ran);
+    if (x_dtype == DT_F16) return try_mx_rows<DT_F16, OUT, false>(ctx, x, ldx, rows, w, k, bias, y, 0, s, ran);
+    return try_mx_rows<DT_BF16, OUT, false>(ctx, x, ldx, rows, w, k, bias, y, 0, s, ran);
 }
 
 template <int DT, int G>
@@ -665,13 +940,14 @@ int tz_linear_mxfp4_workspace(int64_t m, int k, int n, size_t* bytes) {
     return TZ_OK;
 }
 
-static int quantize_input(tz_ctx_t ctx, const char* fn, const void* x, int64_t ldx, int x_dtype, void* ws, size_t ws_bytes, int64_t m, int k, int n,
-                          cudaStream_t s, Q4* out) {
+static int check_workspace(const char* fn, const void* ws, size_t ws_bytes, int64_t m, int k, int n) {
     size_t need = 0;
     int rc = tz_linear_mxfp4_workspace(m, k, n, &need);
     if (rc) return rc;
     TZ_CHECK(ws && al16(ws) && ws_bytes >= need, TZ_EINVAL, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", fn, ws_bytes, need);
-    if ((rc = check_rows(fn, x, ldx, k, x_dtype))) return rc;
+    return TZ_OK;
+}
+static int quantize_input(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, void* ws, int64_t m, int k, cudaStream_t s, Q4* out) {
     uint8_t* codes = static_cast<uint8_t*>(ws);
     uint8_t* scales = codes + a256(code_bytes(m, k));
     *out = {codes, scales, m};
@@ -687,10 +963,19 @@ int tz_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, const
     TZ_CHECK(n > 0 && n % 8 == 0, TZ_EINVAL, "%s: n must be a positive multiple of 8 (%d)", fn, n);
     if (m == 0) return TZ_OK;
     TZ_CHECK(x && w_codes && w_scales && y, TZ_EINVAL, "%s: null pointer", fn);
+    if ((rc = check_rows(fn, x, ldx, k, x_dtype))) return rc;
+    TZ_CHECK(al16(w_codes) && al16(w_scales) && al16(bias) && al16(y), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    if ((rc = check_workspace(fn, workspace, workspace_bytes, m, k, n))) return rc;
     cudaStream_t s = pick_stream(ctx, stream);
+    const Q4 w{static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), n};
+    bool ran = false;
+    rc = y_dtype == DT_F32   ? try_mx_rows_x<DT_F32>(ctx, x, ldx, x_dtype, m, w, k, bias, y, s, &ran)
+         : y_dtype == DT_F16 ? try_mx_rows_x<DT_F16>(ctx, x, ldx, x_dtype, m, w, k, bias, y, s, &ran)
+                             : try_mx_rows_x<DT_BF16>(ctx, x, ldx, x_dtype, m, w, k, bias, y, s, &ran);
+    if (rc || ran) return rc;
     Q4 a;
-    if ((rc = quantize_input(ctx, fn, x, ldx, x_dtype, workspace, workspace_bytes, m, k, n, s, &a))) return rc;
-    return product(ctx, fn, a, {static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), n}, k, bias, y, y_dtype, s);
+    if ((rc = quantize_input(ctx, x, ldx, x_dtype, workspace, m, k, s, &a))) return rc;
+    return product(ctx, fn, a, w, k, bias, y, y_dtype, s);
 }
 
 int tz_gated_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, const void* w_codes, const void* w_scales, void* h, int act,
@@ -704,10 +989,16 @@ int tz_gated_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, c
     if (t == 0) return TZ_OK;
     TZ_CHECK(x && w_codes && w_scales && h, TZ_EINVAL, "%s: null pointer", fn);
     TZ_CHECK(al16(w_codes) && al16(w_scales) && al16(h), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    if ((rc = check_rows(fn, x, ldx, d, dtype))) return rc;
+    if ((rc = check_workspace(fn, workspace, workspace_bytes, t, d, 2 * f))) return rc;
     cudaStream_t s = pick_stream(ctx, stream);
-    Q4 a;
-    if ((rc = quantize_input(ctx, fn, x, ldx, dtype, workspace, workspace_bytes, t, d, 2 * f, s, &a))) return rc;
     const Q4 w{static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), 2ll * f};
+    bool ran = false;
+    rc = dtype == DT_F16 ? try_mx_rows<DT_F16, DT_F16, true>(ctx, x, ldx, t, w, d, nullptr, h, act, s, &ran)
+                         : try_mx_rows<DT_BF16, DT_BF16, true>(ctx, x, ldx, t, w, d, nullptr, h, act, s, &ran);
+    if (rc || ran) return rc;
+    Q4 a;
+    if ((rc = quantize_input(ctx, x, ldx, dtype, workspace, t, d, s, &a))) return rc;
     return dtype == DT_F16 ? launch_mx<DT_F16, true>(ctx, a, w, d, nullptr, h, act, s) : launch_mx<DT_BF16, true>(ctx, a, w, d, nullptr, h, act, s);
 }
 
