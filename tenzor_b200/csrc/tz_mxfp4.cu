@@ -329,8 +329,9 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                 if (armed & (1u << s)) tzp::pair_wait<CG>(&full[s], (armed_par >> s) & 1u, status, nullptr);
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            // ---- MMA issuer ----
+        if (rank == 0) {
+            // ---- MMA issuer (the whole warp; one lane issues) ----
+            const bool issue = tzp::elect_one();
             constexpr uint32_t idesc0 = mx_idesc(128 * CG, BN, 0), idesc2 = mx_idesc(128 * CG, BN, 2);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
@@ -352,36 +353,41 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                     const uint32_t sf = sa + C::A_BYTES + C::B_BYTES;
                     const uint32_t tsf = tmem_base + static_cast<uint32_t>(C::SF0 + stage * C::SF_COLS);
                     const int left = p.k - kb * 256;
-                    // TMEM columns of the stage: A chunk 0 (4), A chunk 1 (4), B chunk 0 (8), B chunk 1 (8)
-                    sf_copy<CG>(tsf, sf);
-                    sf_copy<CG>(tsf + 8, sf + 1024);
-                    sf_copy<CG>(tsf + 12, sf + 2048);
-                    if (left > 128) {
-                        sf_copy<CG>(tsf + 4, sf + 512);
-                        sf_copy<CG>(tsf + 16, sf + 1536);
-                        sf_copy<CG>(tsf + 20, sf + 2560);
-                    }
                     const uint64_t ad = tzp::sdesc_k128(sa), bd = tzp::sdesc_k128(sa + C::A_BYTES);
+                    if (issue) {
+                        // TMEM columns of the stage: A chunk 0 (4), A chunk 1 (4), B chunk 0 (8), B chunk 1 (8)
+                        sf_copy<CG>(tsf, sf);
+                        sf_copy<CG>(tsf + 8, sf + 1024);
+                        sf_copy<CG>(tsf + 12, sf + 2048);
+                        if (left > 128) {
+                            sf_copy<CG>(tsf + 4, sf + 512);
+                            sf_copy<CG>(tsf + 16, sf + 1536);
+                            sf_copy<CG>(tsf + 20, sf + 2560);
+                        }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (k == 0 || left > 64 * k)
-                            mx_mma<CG>(d, ad + 2u * k, bd + 2u * k, (k & 1) ? idesc2 : idesc0, tsf + 4 * (k >> 1), tsf + 8 + 8 * (k >> 1) + boff,
-                                       (kb | k) != 0 ? 1u : 0u);
-                    tzp::pair_commit<CG>(&empty[stage]);
+                        for (int k = 0; k < 4; ++k)
+                            if (k == 0 || left > 64 * k)
+                                mx_mma<CG>(d, ad + 2u * k, bd + 2u * k, (k & 1) ? idesc2 : idesc0, tsf + 4 * (k >> 1),
+                                           tsf + 8 + 8 * (k >> 1) + boff, (kb | k) != 0 ? 1u : 0u);
+                        tzp::pair_commit<CG>(&empty[stage]);
+                    }
+                    __syncwarp();
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                tzp::pair_commit<CG>(&tfull[acc]);
+                if (issue) tzp::pair_commit<CG>(&tfull[acc]);
+                __syncwarp();
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
             }
             // Every MMA issued has completed before TMEM is released.
-            tzp::pair_commit<CG>(drain);
+            if (issue) tzp::pair_commit<CG>(drain);
+            __syncwarp();
             tzp::pair_wait<CG>(drain, 0, status, nullptr);
         }
     } else {
@@ -592,7 +598,8 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
                 if (armed & (1u << s)) tzp::mbar_wait(&full[s], (armed_par >> s) & 1u, status, nullptr);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        {  // the whole warp; one lane issues
+            const bool issue = tzp::elect_one();
             constexpr uint32_t idesc0 = mx_idesc(128, N, 0), idesc2 = mx_idesc(128, N, 2);
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
@@ -602,21 +609,25 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
                 const uint32_t a = tzp::smem_u32(smem + s * C::STAGE), b = tzp::smem_u32(xq + i * C::B_KB);
                 const uint32_t tsf = tmem_base + static_cast<uint32_t>(C::SF0 + s * C::SF_COLS);
                 const int left = p.k - kb * 256;
-                sf_copy<1>(tsf, a + 16384);
-                sf_copy<1>(tsf + 8, b + N * 128);
-                if (left > 128) {
-                    sf_copy<1>(tsf + 4, a + 16384 + 512);
-                    sf_copy<1>(tsf + 12, b + N * 128 + 512);
-                }
                 const uint64_t ad = tzp::sdesc_k128(a), bd = tzp::sdesc_k128(b);
+                if (issue) {
+                    sf_copy<1>(tsf, a + 16384);
+                    sf_copy<1>(tsf + 8, b + N * 128);
+                    if (left > 128) {
+                        sf_copy<1>(tsf + 4, a + 16384 + 512);
+                        sf_copy<1>(tsf + 12, b + N * 128 + 512);
+                    }
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (k == 0 || left > 64 * k)
-                        mx_mma<1>(tmem_base, ad + 2u * k, bd + 2u * k, (k & 1) ? idesc2 : idesc0, tsf + 4 * (k >> 1), tsf + 8 + 4 * (k >> 1),
-                                  (i | k) != 0 ? 1u : 0u);
-                tzp::umma_commit(&empty[s]);
+                    for (int k = 0; k < 4; ++k)
+                        if (k == 0 || left > 64 * k)
+                            mx_mma<1>(tmem_base, ad + 2u * k, bd + 2u * k, (k & 1) ? idesc2 : idesc0, tsf + 4 * (k >> 1), tsf + 8 + 4 * (k >> 1),
+                                      (i | k) != 0 ? 1u : 0u);
+                    tzp::umma_commit(&empty[s]);
+                }
+                __syncwarp();
             }
-            tzp::umma_commit(done);
+            if (issue) tzp::umma_commit(done);
+            __syncwarp();
             tzp::mbar_wait(done, 0, status, nullptr);
         }
     } else {

@@ -14,6 +14,14 @@
 
 namespace tzp {
 
+// One lane of a converged warp (always the same one).  The MMA issuers run their loops with the whole warp and
+// issue under this predicate: addresses and descriptors then stay in uniform registers, where a branch on the
+// lane number moves each operand of each instruction there one by one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
