@@ -215,8 +215,9 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     };
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---- TMA producer ----
+        {
+            // ---- TMA producer (the whole warp; one lane issues) ----
+            const bool issue = tzp::elect_one();
             int stage = 0;
             uint32_t phase = 0, armed = 0, armed_par = 0;
             bool ok = true;
@@ -230,42 +231,45 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                 const uint32_t bytes = CG * (need_b ? C::STAGE : C::A_BYTES);
                 const int m0 = (q.m * CG + static_cast<int>(rank)) * 128;
                 for (int kb = q.kb0; kb < q.kb1; ++kb) {
-                    if (!tzp::pair_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
+                    if (!tzp::warp_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
                         ok = false;
                         break;
                     }
                     if (rank == 0) {
-                        tzp::mbar_arrive_expect_tx(&full[stage], bytes);
                         armed |= 1u << stage;
                         armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
                     }
                     const uint32_t bar = CG == 2 ? tzp::mapa(&full[stage], 0) : tzp::smem_u32(&full[stage]);
                     const uint32_t sa = sbase + stage * a_step;
                     const uint32_t sb = b_addr(stage, kb);
-                    if constexpr (MODE == MM_DW) {
-                        const CUtensorMap* ta = q.w ? &tmA1 : &tmA0;
-                        tzp::pair_load_2d<CG>(sa, ta, m0, kb * 64, bar);
-                        tzp::pair_load_2d<CG>(sa + 8192, ta, m0 + 64, kb * 64, bar);
+                    if (issue) {
+                        if (rank == 0) tzp::mbar_arrive_expect_tx(&full[stage], bytes);
+                        if constexpr (MODE == MM_DW) {
+                            const CUtensorMap* ta = q.w ? &tmA1 : &tmA0;
+                            tzp::pair_load_2d<CG>(sa, ta, m0, kb * 64, bar);
+                            tzp::pair_load_2d<CG>(sa + 8192, ta, m0 + 64, kb * 64, bar);
 #pragma unroll
-                        for (int j = 0; j < C::BNC / 64; ++j)
-                            tzp::pair_load_2d<CG>(sb + j * 8192, &tmB0, b_col(q.n, j), kb * 64, bar);
-                    } else if constexpr (MODE == MM_DX) {
-                        const bool up = kb >= p.half;
-                        const int k = (up ? kb - p.half : kb) * 64;
-                        tzp::pair_load_2d<CG>(sa, up ? &tmA1 : &tmA0, k, m0, bar);
+                            for (int j = 0; j < C::BNC / 64; ++j)
+                                tzp::pair_load_2d<CG>(sb + j * 8192, &tmB0, b_col(q.n, j), kb * 64, bar);
+                        } else if constexpr (MODE == MM_DX) {
+                            const bool up = kb >= p.half;
+                            const int k = (up ? kb - p.half : kb) * 64;
+                            tzp::pair_load_2d<CG>(sa, up ? &tmA1 : &tmA0, k, m0, bar);
 #pragma unroll
-                        for (int j = 0; j < C::BNC / 64; ++j)
-                            tzp::pair_load_2d<CG>(sb + j * 8192, up ? &tmB1 : &tmB0, b_col(q.n, j), k, bar);
-                    } else {
-                        tzp::pair_load_2d<CG>(sa, &tmA0, kb * 64, m0, bar);
-                        if (!need_b) {
-                        } else if constexpr (CG == 2) {
-                            tzp::pair_load_2d<CG>(sb, rank ? &tmB1 : &tmB0, kb * 64, q.n * (BN / 2), bar);
+                            for (int j = 0; j < C::BNC / 64; ++j)
+                                tzp::pair_load_2d<CG>(sb + j * 8192, up ? &tmB1 : &tmB0, b_col(q.n, j), k, bar);
                         } else {
-                            tzp::pair_load_2d<CG>(sb, &tmB0, kb * 64, q.n * (BN / 2), bar);
-                            tzp::pair_load_2d<CG>(sb + (BN / 2) * 128, &tmB1, kb * 64, q.n * (BN / 2), bar);
+                            tzp::pair_load_2d<CG>(sa, &tmA0, kb * 64, m0, bar);
+                            if (!need_b) {
+                            } else if constexpr (CG == 2) {
+                                tzp::pair_load_2d<CG>(sb, rank ? &tmB1 : &tmB0, kb * 64, q.n * (BN / 2), bar);
+                            } else {
+                                tzp::pair_load_2d<CG>(sb, &tmB0, kb * 64, q.n * (BN / 2), bar);
+                                tzp::pair_load_2d<CG>(sb + (BN / 2) * 128, &tmB1, kb * 64, q.n * (BN / 2), bar);
+                            }
                         }
                     }
+                    __syncwarp();
                     if (++stage == ring) {
                         stage = 0;
                         phase ^= 1u;
@@ -277,8 +281,9 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                 if (armed & (1u << s)) tzp::pair_wait<CG>(&full[s], (armed_par >> s) & 1u, status, nullptr);
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            // ---- MMA issuer ----
+        if (rank == 0) {
+            // ---- MMA issuer (the whole warp; one lane issues) ----
+            const bool issue = tzp::elect_one();
             constexpr uint32_t major = (C::kAmn ? 1u << 15 : 0u) | (C::kBmn ? 1u << 16 : 0u);
             constexpr uint32_t idesc = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 256) | major;
             constexpr uint32_t idesc_b = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 128) | major;  // columns 256 .. 383
@@ -288,11 +293,11 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             bool ok = true;
             Tile q;
             for (int i = 0; ok && tile_at(i, q); ++i) {
-                if (!tzp::pair_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
+                if (!tzp::warp_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                 for (int kb = q.kb0; kb < q.kb1; ++kb) {
-                    if (!tzp::pair_wait<CG>(&full[stage], phase, status, abort_flag)) {
+                    if (!tzp::warp_wait<CG>(&full[stage], phase, status, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -301,27 +306,33 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                     const uint32_t sb = b_addr(stage, kb);
                     const uint64_t ad = C::kAmn ? tzp::sdesc_mn128(sa, 8192) : tzp::sdesc_k128(sa);
                     const uint64_t bd = C::kBmn ? tzp::sdesc_mn128(sb, 8192) : tzp::sdesc_k128(sb);
+                    if (issue) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t more = (kb > q.kb0 || k > 0) ? 1u : 0u;
-                        tzp::pair_mma_f16<CG>(d, ad + kAstep * k, bd + kBstep * k, idesc, more);
-                        if constexpr (BN == 384) tzp::pair_mma_f16<CG>(d + 256, ad + kAstep * k, bd + (16384u >> 4) + kBstep * k, idesc_b, more);
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t more = (kb > q.kb0 || k > 0) ? 1u : 0u;
+                            tzp::pair_mma_f16<CG>(d, ad + kAstep * k, bd + kBstep * k, idesc, more);
+                            if constexpr (BN == 384)
+                                tzp::pair_mma_f16<CG>(d + 256, ad + kAstep * k, bd + (16384u >> 4) + kBstep * k, idesc_b, more);
+                        }
+                        tzp::pair_commit<CG>(&empty[stage]);
                     }
-                    tzp::pair_commit<CG>(&empty[stage]);
+                    __syncwarp();
                     if (++stage == ring) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                tzp::pair_commit<CG>(&tfull[acc]);
+                if (issue) tzp::pair_commit<CG>(&tfull[acc]);
+                __syncwarp();
                 if (++acc == C::ACCS) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
             }
             // Every MMA issued has completed before TMEM is released.
-            tzp::pair_commit<CG>(drain);
+            if (issue) tzp::pair_commit<CG>(drain);
+            __syncwarp();
             tzp::pair_wait<CG>(drain, 0, status, nullptr);
         }
     } else {
@@ -347,7 +358,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         for (int i = 1; more; ++i) {
             q = next;
             more = tile_at(i, next);
-            if (!tzp::pair_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
+            if (!tzp::warp_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
             tzp::tc_fence_after();
             const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN);
             const int row0 = (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32;
@@ -356,7 +367,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                 const int col0 = q.n * (BN / 2) + cc;
                 uint32_t dh[16];
                 if constexpr (MODE == MM_BWD) {
-                    if (!tzp::mbar_wait(&dhbar[e], dh_phase, status, abort_flag)) break;
+                    if (!tzp::warp_wait<1>(&dhbar[e], dh_phase, status, abort_flag)) break;
                     dh_phase ^= 1u;
                     fetched = false;
 #pragma unroll

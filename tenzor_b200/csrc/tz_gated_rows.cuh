@@ -80,40 +80,49 @@ __global__ void __launch_bounds__(RowsCfg<N>::THREADS, 1)
     tzp::pdl_wait();
 
     if (warp == 0) {
-        if (lane == 0) {
+        {  // the whole warp; one lane issues
+            const bool issue = tzp::elect_one();
             uint32_t armed = 0, armed_par = 0;
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
                 const uint32_t phase = (i / STAGES) & 1;
-                if (!tzp::mbar_wait(&empty[s], phase ^ 1u, status, abort_flag)) break;
+                if (!tzp::warp_wait<1>(&empty[s], phase ^ 1u, status, abort_flag)) break;
                 uint8_t* a = smem + s * C::STAGE;
-                tzp::mbar_arrive_expect_tx(&full[s], C::STAGE);
                 armed |= 1u << s;
                 armed_par = (armed_par & ~(1u << s)) | (phase << s);
-                tzp::tma_load_2d(a, &tmG, kb * 64, f0, &full[s]);
-                tzp::tma_load_2d(a + 16384, &tmU, kb * 64, f0, &full[s]);
-                tzp::tma_load_2d(a + 32768, &tmX, kb * 64, 0, &full[s]);
+                if (issue) {
+                    tzp::mbar_arrive_expect_tx(&full[s], C::STAGE);
+                    tzp::tma_load_2d(a, &tmG, kb * 64, f0, &full[s]);
+                    tzp::tma_load_2d(a + 16384, &tmU, kb * 64, f0, &full[s]);
+                    tzp::tma_load_2d(a + 32768, &tmX, kb * 64, 0, &full[s]);
+                }
+                __syncwarp();
             }
             for (int s = 0; s < STAGES; ++s)  // every copy has landed before the stages are used again (bounded)
                 if (armed & (1u << s)) tzp::mbar_wait(&full[s], (armed_par >> s) & 1u, status, nullptr);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        {  // the whole warp; one lane issues
+            const bool issue = tzp::elect_one();
             constexpr uint32_t idesc = tzp::make_idesc(1, BF ? 1 : 0, 128, N);
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
-                if (!tzp::mbar_wait(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
+                if (!tzp::warp_wait<1>(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t a = tzp::smem_u32(smem + s * C::STAGE);
                 const uint64_t gd = tzp::sdesc_k128(a), ud = tzp::sdesc_k128(a + 16384), xd = tzp::sdesc_k128(a + 32768);
+                if (issue) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    tzp::umma<0>(tmem_base, gd + 2u * k, xd + 2u * k, idesc, (i | k) != 0 ? 1u : 0u);
-                    tzp::umma<0>(tmem_base + N, ud + 2u * k, xd + 2u * k, idesc, (i | k) != 0 ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) {
+                        tzp::umma<0>(tmem_base, gd + 2u * k, xd + 2u * k, idesc, (i | k) != 0 ? 1u : 0u);
+                        tzp::umma<0>(tmem_base + N, ud + 2u * k, xd + 2u * k, idesc, (i | k) != 0 ? 1u : 0u);
+                    }
+                    tzp::umma_commit(&empty[s]);
                 }
-                tzp::umma_commit(&empty[s]);
+                __syncwarp();
             }
-            tzp::umma_commit(done);
+            if (issue) tzp::umma_commit(done);
+            __syncwarp();
             tzp::mbar_wait(done, 0, status, nullptr);
         }
     }

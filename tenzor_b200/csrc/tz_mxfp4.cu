@@ -290,8 +290,9 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
     const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---- TMA producer ----
+        {
+            // ---- TMA producer (the whole warp; one lane issues) ----
+            const bool issue = tzp::elect_one();
             int stage = 0;
             uint32_t phase = 0, armed = 0, armed_par = 0;
             bool ok = true;
@@ -301,24 +302,27 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                 const int mb = m * CG + static_cast<int>(rank);
                 const int nb = n * BN / 128;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!tzp::pair_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
+                    if (!tzp::warp_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
                         ok = false;
                         break;
                     }
                     if (rank == 0) {
-                        tzp::mbar_arrive_expect_tx(&full[stage], CG * C::STAGE);
                         armed |= 1u << stage;
                         armed_par = (armed_par & ~(1u << stage)) | (phase << stage);
                     }
                     const uint32_t bar = CG == 2 ? tzp::mapa(&full[stage], 0) : tzp::smem_u32(&full[stage]);
                     const uint32_t sa = tzp::smem_u32(smem + stage * C::STAGE);
                     const uint32_t sb = sa + C::A_BYTES, sf = sb + C::B_BYTES;
-                    tzp::pair_load_2d<CG>(sa, &tmA, kb * 128, mb * 128, bar);
-                    tzp::pair_load_2d<CG>(sb, &tmB, kb * 128, n * BN + static_cast<int>(rank) * C::BNC, bar);
-                    // two chunks each (past a row block's last chunk: of the next one or zeros, which no MMA uses)
-                    tzp::pair_load_2d<CG>(sf, &tmSA, 0, mb * p.k_chunks + 2 * kb, bar);
-                    tzp::pair_load_2d<CG>(sf + 1024, &tmSB, 0, nb * p.k_chunks + 2 * kb, bar);
-                    tzp::pair_load_2d<CG>(sf + 2048, &tmSB, 0, (nb + 1) * p.k_chunks + 2 * kb, bar);
+                    if (issue) {
+                        if (rank == 0) tzp::mbar_arrive_expect_tx(&full[stage], CG * C::STAGE);
+                        tzp::pair_load_2d<CG>(sa, &tmA, kb * 128, mb * 128, bar);
+                        tzp::pair_load_2d<CG>(sb, &tmB, kb * 128, n * BN + static_cast<int>(rank) * C::BNC, bar);
+                        // two chunks each (past a row block's last chunk: of the next one or zeros, which no MMA uses)
+                        tzp::pair_load_2d<CG>(sf, &tmSA, 0, mb * p.k_chunks + 2 * kb, bar);
+                        tzp::pair_load_2d<CG>(sf + 1024, &tmSB, 0, nb * p.k_chunks + 2 * kb, bar);
+                        tzp::pair_load_2d<CG>(sf + 2048, &tmSB, 0, (nb + 1) * p.k_chunks + 2 * kb, bar);
+                    }
+                    __syncwarp();
                     if (++stage == STAGES) {
                         stage = 0;
                         phase ^= 1u;
@@ -339,12 +343,12 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
             for (int t = t0; ok && t < num_tiles; t += tstep) {
                 int m, n;
                 tile_of(t, m, n);
-                if (!tzp::pair_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
+                if (!tzp::warp_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                 const uint32_t boff = static_cast<uint32_t>((n * BN & 127) / 32);  // the tile's first row inside its scale chunk
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!tzp::pair_wait<CG>(&full[stage], phase, status, abort_flag)) {
+                    if (!tzp::warp_wait<CG>(&full[stage], phase, status, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
         for (int t = t0; t < num_tiles; t += tstep) {
             int m, n;
             tile_of(t, m, n);
-            if (!tzp::pair_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
+            if (!tzp::warp_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
             tzp::tc_fence_after();
             const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN + sl * 64);
             const int row0 = (m * CG + static_cast<int>(rank)) * 128 + q4 * 32;
@@ -581,18 +585,22 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
     tzp::pdl_wait();
 
     if (warp == 0) {
-        if (lane == 0) {
+        {  // the whole warp; one lane issues
+            const bool issue = tzp::elect_one();
             uint32_t armed = 0, armed_par = 0;
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
                 const uint32_t phase = (i / STAGES) & 1;
-                if (!tzp::mbar_wait(&empty[s], phase ^ 1u, status, abort_flag)) break;
+                if (!tzp::warp_wait<1>(&empty[s], phase ^ 1u, status, abort_flag)) break;
                 uint8_t* a = smem + s * C::STAGE;
-                tzp::mbar_arrive_expect_tx(&full[s], C::STAGE);
                 armed |= 1u << s;
                 armed_par = (armed_par & ~(1u << s)) | (phase << s);
-                tzp::tma_load_2d(a, &tmW, kb * 128, n0, &full[s]);
-                tzp::tma_load_2d(a + 16384, &tmSW, 0, static_cast<int>(blockIdx.y) * p.k_chunks + 2 * kb, &full[s]);
+                if (issue) {
+                    tzp::mbar_arrive_expect_tx(&full[s], C::STAGE);
+                    tzp::tma_load_2d(a, &tmW, kb * 128, n0, &full[s]);
+                    tzp::tma_load_2d(a + 16384, &tmSW, 0, static_cast<int>(blockIdx.y) * p.k_chunks + 2 * kb, &full[s]);
+                }
+                __syncwarp();
             }
             for (int s = 0; s < STAGES; ++s)  // every copy has landed before the stages are used again (bounded)
                 if (armed & (1u << s)) tzp::mbar_wait(&full[s], (armed_par >> s) & 1u, status, nullptr);
@@ -603,8 +611,8 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
             constexpr uint32_t idesc0 = mx_idesc(128, N, 0), idesc2 = mx_idesc(128, N, 2);
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
-                if (!tzp::mbar_wait(&xready[i], 0, status, abort_flag)) break;
-                if (!tzp::mbar_wait(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
+                if (!tzp::warp_wait<1>(&xready[i], 0, status, abort_flag)) break;
+                if (!tzp::warp_wait<1>(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t a = tzp::smem_u32(smem + s * C::STAGE), b = tzp::smem_u32(xq + i * C::B_KB);
                 const uint32_t tsf = tmem_base + static_cast<uint32_t>(C::SF0 + s * C::SF_COLS);
@@ -631,23 +639,46 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
             tzp::mbar_wait(done, 0, status, nullptr);
         }
     } else {
-        // ---- quantise this CTA's K slice of x, one K block (256 values of N rows) after the other; a warp takes a
-        // row of the block, a lane 8 values.  Rows past the last one are zeros with the smallest scale. ----
-        for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
-            uint8_t* blk = xq + i * C::B_KB;
+        // ---- quantise this CTA's K slice of x, one K block (256 values of N rows) after the other; a warp takes
+        // N / 8 rows of the block, a lane 8 values of each.  Rows past the last one are zeros with the smallest scale.
+        // The next block's values are on their way while a block is quantised. ----
+        constexpr int R = N / C::QWARPS;
+        float v[R][8];
+        auto fetch = [&](int kb) {
             const int c = kb * 256 + lane * 8;
 #pragma unroll
-            for (int j = 0; j < N / C::QWARPS; ++j) {
+            for (int j = 0; j < R; ++j) {
                 const int r = warp - 2 + j * C::QWARPS;
-                float v[8] = {};
-                if (r < p.rows && c < p.k) load8<XDT>(p.x, r * p.ldx + c, v);
-                uint32_t sc;
-                const uint32_t q = quant_block(v, sc);
+                if (r < p.rows && c < p.k) {
+                    load8<XDT>(p.x, r * p.ldx + c, v[j]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
+                }
+            }
+        };
+        fetch(kb0);
+        for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+            uint8_t* blk = xq + i * C::B_KB;
+            float u[R][8];
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[j][e] = v[j][e];
+            if (kb + 1 < kb1) fetch(kb + 1);
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const int r = warp - 2 + j * C::QWARPS;
+                uint32_t q = 0, w = 0;
+                if (r < p.rows) {  // the same for the whole warp
+                    uint32_t sc;
+                    q = quant_block(u[j], sc);
+                    w = sc << (8 * ((lane >> 2) & 3));
+                    w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+                    w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
+                }
                 // 4 bytes at byte 4 * lane of a 128-byte row, 128-byte swizzle (16-byte unit u at u ^ (r % 8))
                 *reinterpret_cast<uint32_t*>(blk + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = q;
-                uint32_t w = sc << (8 * ((lane >> 2) & 3));
-                w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
-                w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
                 if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(blk + N * 128 + (lane >> 4) * 512 + r * 16) = w;
             }
             tzp::fence_proxy_async();

@@ -72,6 +72,12 @@ __device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, int* s
     }
 }
 
+// The same by a whole warp, with one answer for all lanes (a wait that ran out in one lane must not split the warp).
+template <int CG>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, volatile int* abort) {
+    return __all_sync(0xFFFFFFFFu, pair_wait<CG>(bar, parity, status, abort));
+}
+
 // 2-D tiled load into this CTA's shared memory, its bytes counted on the barrier at cluster address `bar`
 // (the leader's, for a pair).
 template <int CG>
