@@ -88,34 +88,44 @@ __device__ __forceinline__ uint32_t quant_block(const float (&v)[8], uint32_t& s
     return e2m1x8(v, __uint_as_float((254u - (e == 255u ? 0u : sc)) << 23));
 }
 
-// One lane quantises 8 values at a time; 4 lanes make a block and 16 lanes the four scale codes of one word.
-// A warp takes 256 columns of a row per step.  Memory-bound: 2 (or 4) bytes read, 0.53 written per value.
-// Row r of x becomes row `map(r)` of the result: r, or with GROUP > 0 row (r / GROUP) * 2 GROUP + r % GROUP +
-// off, which interleaves two matrices in groups of GROUP rows.
+// One lane quantises 8 values at a time; 4 lanes make a block and 16 lanes the four scale codes of one word.  A warp
+// takes 1024 columns of a row, its four loads of 512 bytes (1024 for f32) in flight together.  Memory-bound: 2 (or 4)
+// bytes read, 0.53 written per value.
+// Row r of x becomes row r of the result, or with GROUP > 0 row (r / GROUP) * 2 GROUP + r % GROUP + off, which
+// interleaves two matrices in groups of GROUP rows.
 template <int DT, int GROUP>
 __global__ void __launch_bounds__(256) quantize_mxfp4_kernel(const void* x, long long ldx, uint8_t* codes, uint8_t* scales, long long rows,
                                                              int cols, int off) {
     const int lane = threadIdx.x & 31;
     const int k_chunks = (cols + 127) / 128;
-    const int steps = (cols + 255) / 256;
-    const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
-    const long long total = rows * steps;
-    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += warps) {
-        const long long r = i / steps;
-        const int c = static_cast<int>(i - r * steps) * 256 + lane * 8;
-        const bool in = c < cols;
-        float v[8] = {};
-        if (in) load8<DT>(x, r * ldx + c, v);
-        uint32_t sc;
-        const uint32_t q = quant_block(v, sc);
+    const int c0 = static_cast<int>(blockIdx.x) * 1024 + lane * 8;
+    for (long long r = blockIdx.y * 8ll + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8ll) {
+        float v[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (c0 + 256 * j < cols) {
+                load8<DT>(x, r * ldx + c0 + 256 * j, v[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
+            }
+        }
         const long long ro = GROUP > 0 ? (r / GROUP) * (2 * GROUP) + r % GROUP + off : r;
-        if (in) *reinterpret_cast<uint32_t*>(codes + (ro * cols + c) / 2) = q;
-        // lanes 0, 4, 8, 12 of each half warp hold the word's four bytes (0 for blocks past the row's end)
-        uint32_t w = in ? sc << (8 * ((lane >> 2) & 3)) : 0u;
-        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
-        w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
-        if (in && (lane & 15) == 0)
-            *reinterpret_cast<uint32_t*>(scales + sf_chunk(ro >> 7, c >> 7, k_chunks) + (ro & 31) * 16 + ((ro & 127) >> 5) * 4) = w;
+        uint8_t* srow = scales + sf_chunk(ro >> 7, 0, k_chunks) + (ro & 31) * 16 + ((ro & 127) >> 5) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + 256 * j;
+            if (blockIdx.x * 1024 + 256 * j >= cols) break;  // the same for the whole warp
+            const bool in = c < cols;
+            uint32_t sc;
+            const uint32_t q = quant_block(v[j], sc);
+            if (in) *reinterpret_cast<uint32_t*>(codes + (ro * cols + c) / 2) = q;
+            // lanes 0, 4, 8, 12 of each half warp hold the word's four bytes (0 for blocks past the row's end)
+            uint32_t w = in ? sc << (8 * ((lane >> 2) & 3)) : 0u;
+            w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+            w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
+            if (in && (lane & 15) == 0) *reinterpret_cast<uint32_t*>(srow + (c >> 7) * 512) = w;
+        }
     }
     tzp::pdl_trigger();  // the product that follows may set up
 }
@@ -132,29 +142,44 @@ __device__ __forceinline__ float2 e2m1x2(uint32_t byte) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// The quantiser's split the other way round.
 template <int DT>
 __global__ void __launch_bounds__(256) dequantize_mxfp4_kernel(const uint8_t* codes, const uint8_t* scales, void* out, long long rows, int cols) {
+    const int lane = threadIdx.x & 31;
     const int k_chunks = (cols + 127) / 128;
-    const long long n8 = rows * (cols / 8);
-    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n8; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const long long r = i / (cols / 8);
-        const int c = static_cast<int>(i - r * (cols / 8)) * 8;
-        const uint32_t q = __ldg(reinterpret_cast<const uint32_t*>(codes) + i);
-        const float s = e8m0(__ldg(scales + sf_chunk(r >> 7, c >> 7, k_chunks) + (r & 31) * 16 + ((r & 127) >> 5) * 4 + ((c >> 5) & 3)));
-        float v[8];
+    const int c0 = static_cast<int>(blockIdx.x) * 1024 + lane * 8;
+    for (long long r = blockIdx.y * 8ll + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8ll) {
+        const uint8_t* srow = scales + sf_chunk(r >> 7, 0, k_chunks) + (r & 31) * 16 + ((r & 127) >> 5) * 4;
+        uint32_t q[4], sc[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float2 f = e2m1x2((q >> (8 * j)) & 255u);
-            v[2 * j] = f.x * s, v[2 * j + 1] = f.y * s;
+            const int c = c0 + 256 * j;
+            if (c < cols) {
+                q[j] = __ldg(reinterpret_cast<const uint32_t*>(codes + (r * cols + c) / 2));
+                sc[j] = __ldg(srow + (c >> 7) * 512 + ((c >> 5) & 3));
+            }
         }
-        if constexpr (DT == DT_F32) {
-            float4* o = reinterpret_cast<float4*>(out) + 2 * i;
-            o[0] = make_float4(v[0], v[1], v[2], v[3]);
-            o[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            constexpr bool BF = DT == DT_BF16;
-            reinterpret_cast<uint4*>(out)[i] = make_uint4(tzp::pack16x2<BF>(v[0], v[1]), tzp::pack16x2<BF>(v[2], v[3]),
-                                                          tzp::pack16x2<BF>(v[4], v[5]), tzp::pack16x2<BF>(v[6], v[7]));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + 256 * j;
+            if (c >= cols) break;
+            const float s = e8m0(sc[j]);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = e2m1x2((q[j] >> (8 * e)) & 255u);
+                v[2 * e] = f.x * s, v[2 * e + 1] = f.y * s;
+            }
+            if constexpr (DT == DT_F32) {
+                float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + r * cols + c);
+                o[0] = make_float4(v[0], v[1], v[2], v[3]);
+                o[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                constexpr bool BF = DT == DT_BF16;
+                *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + r * cols + c) =
+                    make_uint4(tzp::pack16x2<BF>(v[0], v[1]), tzp::pack16x2<BF>(v[2], v[3]), tzp::pack16x2<BF>(v[4], v[5]),
+                               tzp::pack16x2<BF>(v[6], v[7]));
+            }
         }
     }
 }
@@ -821,6 +846,9 @@ int launch_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int rows, const Q4&
     const int tiles = ceil_div(w.rows, 128), kblocks = ceil_div(k, 256);
     *ran = false;
     if (tiles > 65535) return TZ_OK;  // the grid's second extent
+    // With room for 32 rows quantising x costs each CTA more than the tiles of 256 rows cost once there is more than
+    // one CTA per SM: 32 rows, D = 4096, 2 F = 32768 37.9 us here, 28.4 us there; one wave (2 F = 16384) 19.5, 20.2.
+    if (N > 16 && tiles > ctx->sm_count) return TZ_OK;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::smem(C::MAX_KB), done);
     if (rc) return rc;
@@ -865,11 +893,15 @@ int try_mx_rows_x(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, int64_t
     return try_mx_rows<DT_BF16, OUT, false>(ctx, x, ldx, rows, w, k, bias, y, 0, s, ran);
 }
 
+// 8 rows x 1024 columns a block.
+dim3 row_grid(int64_t rows, int cols) {
+    const int64_t y = (rows + 7) / 8;
+    return dim3(static_cast<unsigned>(ceil_div(cols, 1024)), static_cast<unsigned>(y < 65535 ? y : 65535));
+}
+
 template <int DT, int G>
 int launch_quant(tz_ctx_t ctx, const void* x, int64_t ldx, void* codes, void* scales, int64_t rows, int cols, int off, cudaStream_t s) {
-    const long long warps = rows * ceil_div(cols, 256);
-    const long long want = (warps + 7) / 8, most = static_cast<long long>(ctx->sm_count) * 8 * 4;
-    return launch_kernel(quantize_mxfp4_kernel<DT, G>, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, s, false, x,
+    return launch_kernel(quantize_mxfp4_kernel<DT, G>, row_grid(rows, cols), dim3(256), 0, s, false, x,
                          static_cast<long long>(ldx), static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), static_cast<long long>(rows),
                          cols, off);
 }
@@ -940,10 +972,8 @@ int tz_dequantize_mxfp4(tz_ctx_t ctx, const void* codes, const void* scales, voi
     if (rows == 0) return TZ_OK;
     TZ_CHECK(codes && scales && out, TZ_EINVAL, "%s: null pointer", fn);
     TZ_CHECK(al16(codes) && al16(scales) && al16(out), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
-    const long long n8 = rows * (cols / 8), want = (n8 + 255) / 256, most = static_cast<long long>(ctx->sm_count) * 32;
-    const dim3 grid(static_cast<unsigned>(want < most ? want : most));
     auto* kern = dtype == DT_F32 ? dequantize_mxfp4_kernel<DT_F32> : dtype == DT_F16 ? dequantize_mxfp4_kernel<DT_F16> : dequantize_mxfp4_kernel<DT_BF16>;
-    return launch_kernel(kern, grid, dim3(256), 0, pick_stream(ctx, stream), false, static_cast<const uint8_t*>(codes),
+    return launch_kernel(kern, row_grid(rows, cols), dim3(256), 0, pick_stream(ctx, stream), false, static_cast<const uint8_t*>(codes),
                          static_cast<const uint8_t*>(scales), out, static_cast<long long>(rows), cols);
 }
 
