@@ -388,7 +388,8 @@ int tz_pack_gated_mxfp4(tz_ctx_t ctx, const void* w_gate, const void* w_up, int 
  * tensor cores (kind::mxf4), f32 accumulation, one rounding to y_dtype; n a multiple of 8. */
 int tz_gemm_mxfp4(tz_ctx_t ctx, const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,
                   const float* bias, void* y, int y_dtype, int64_t m, int k, int n, tz_stream_t stream);
-/* Device workspace of the two calls below (n = 2f for the gated one). */
+/* Device workspace of the two calls below (n = 2f for the gated one); 0 where x is quantised inside the
+ * product's kernel (m <= 16, k <= 8192): the workspace may then be NULL. */
 int tz_linear_mxfp4_workspace(int64_t m, int k, int n, size_t* bytes);
 /* y = quantised(x) w^T (+ bias): x [m, k] with row stride ldx is quantised in the call. */
 int tz_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, const void* w_codes, const void* w_scales,

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                 const uint32_t bytes = CG * (need_b ? C::STAGE : C::A_BYTES);
                 const int m0 = (q.m * CG + static_cast<int>(rank)) * 128;
                 for (int kb = q.kb0; kb < q.kb1; ++kb) {
-                    if (!tzp::warp_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
+                    if (!tzp::warp_wait(&empty[stage], phase ^ 1u, status, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             }
             // Every copy has landed before the CTA can exit (bounded; the pair's copies all count on the leader).
             for (int s = 0; s < STAGES; ++s)
-                if (armed & (1u << s)) tzp::pair_wait<CG>(&full[s], (armed_par >> s) & 1u, status, nullptr);
+                if (armed & (1u << s)) tzp::mbar_wait(&full[s], (armed_par >> s) & 1u, status, nullptr);
         }
     } else if (warp == 1) {
         if (rank == 0) {
@@ -293,11 +293,11 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             bool ok = true;
             Tile q;
             for (int i = 0; ok && tile_at(i, q); ++i) {
-                if (!tzp::warp_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
+                if (!tzp::warp_wait(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                 for (int kb = q.kb0; kb < q.kb1; ++kb) {
-                    if (!tzp::warp_wait<CG>(&full[stage], phase, status, abort_flag)) {
+                    if (!tzp::warp_wait(&full[stage], phase, status, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             // Every MMA issued has completed before TMEM is released.
             if (issue) tzp::pair_commit<CG>(drain);
             __syncwarp();
-            tzp::pair_wait<CG>(drain, 0, status, nullptr);
+            tzp::mbar_wait(drain, 0, status, nullptr);
         }
     } else {
         // ---- epilogue: a warp reads TMEM lane quarter (warp % 4) and a slice of the columns: 32 outputs of a
@@ -358,7 +358,8 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         for (int i = 1; more; ++i) {
             q = next;
             more = tile_at(i, next);
-            if (!tzp::warp_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
+            if (!more) tzp::pdl_trigger();
+            if (!tzp::warp_wait(&tfull[acc], acc_phase, status, abort_flag)) break;
             tzp::tc_fence_after();
             const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN);
             const int row0 = (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32;
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                 const int col0 = q.n * (BN / 2) + cc;
                 uint32_t dh[16];
                 if constexpr (MODE == MM_BWD) {
-                    if (!tzp::warp_wait<1>(&dhbar[e], dh_phase, status, abort_flag)) break;
+                    if (!tzp::warp_wait(&dhbar[e], dh_phase, status, abort_flag)) break;
                     dh_phase ^= 1u;
                     fetched = false;
 #pragma unroll
@@ -482,13 +483,13 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         }
     }
 
-    tzp::pdl_trigger();
+    if (warp < 2) tzp::pdl_trigger();
     tzp::tc_fence_before();
     __syncthreads();
     if constexpr (CG == 2) {
         // The leader's last commit has arrived in CTA 1 too and both CTAs are done: nothing is under way to a
         // CTA that has left.
-        if (rank == 1 && threadIdx.x == 32) tzp::pair_wait<CG>(drain, 0, status, nullptr);
+        if (rank == 1 && threadIdx.x == 32) tzp::mbar_wait(drain, 0, status, nullptr);
         __syncwarp();
         tzp::cluster_sync();
     }

@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(RowsCfg<N>::THREADS, 1)
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
                 const uint32_t phase = (i / STAGES) & 1;
-                if (!tzp::warp_wait<1>(&empty[s], phase ^ 1u, status, abort_flag)) break;
+                if (!tzp::warp_wait(&empty[s], phase ^ 1u, status, abort_flag)) break;
                 uint8_t* a = smem + s * C::STAGE;
                 armed |= 1u << s;
                 armed_par = (armed_par & ~(1u << s)) | (phase << s);
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(RowsCfg<N>::THREADS, 1)
             constexpr uint32_t idesc = tzp::make_idesc(1, BF ? 1 : 0, 128, N);
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
-                if (!tzp::warp_wait<1>(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
+                if (!tzp::warp_wait(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t a = tzp::smem_u32(smem + s * C::STAGE);
                 const uint64_t gd = tzp::sdesc_k128(a), ud = tzp::sdesc_k128(a + 16384), xd = tzp::sdesc_k128(a + 32768);

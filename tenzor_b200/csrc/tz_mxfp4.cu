@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                 const int mb = m * CG + static_cast<int>(rank);
                 const int nb = n * BN / 128;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!tzp::warp_wait<CG>(&empty[stage], phase ^ 1u, status, abort_flag)) {
+                    if (!tzp::warp_wait(&empty[stage], phase ^ 1u, status, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                 }
             }
             for (int s = 0; s < STAGES; ++s)  // every copy has landed before the CTA can exit (bounded)
-                if (armed & (1u << s)) tzp::pair_wait<CG>(&full[s], (armed_par >> s) & 1u, status, nullptr);
+                if (armed & (1u << s)) tzp::mbar_wait(&full[s], (armed_par >> s) & 1u, status, nullptr);
         }
     } else if (warp == 1) {
         if (rank == 0) {
@@ -368,12 +368,12 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
             for (int t = t0; ok && t < num_tiles; t += tstep) {
                 int m, n;
                 tile_of(t, m, n);
-                if (!tzp::warp_wait<CG>(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
+                if (!tzp::warp_wait(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                 const uint32_t boff = static_cast<uint32_t>((n * BN & 127) / 32);  // the tile's first row inside its scale chunk
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!tzp::warp_wait<CG>(&full[stage], phase, status, abort_flag)) {
+                    if (!tzp::warp_wait(&full[stage], phase, status, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -383,8 +383,22 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                     const uint32_t tsf = tmem_base + static_cast<uint32_t>(C::SF0 + stage * C::SF_COLS);
                     const int left = p.k - kb * 256;
                     const uint64_t ad = tzp::sdesc_k128(sa), bd = tzp::sdesc_k128(sa + C::A_BYTES);
-                    if (issue) {
-                        // TMEM columns of the stage: A chunk 0 (4), A chunk 1 (4), B chunk 0 (8), B chunk 1 (8)
+                    // TMEM columns of the stage: A chunk 0 (4), A chunk 1 (4), B chunk 0 (8), B chunk 1 (8)
+                    if (left >= 256) {
+                        if (issue) {
+                            sf_copy<CG>(tsf, sf);
+                            sf_copy<CG>(tsf + 8, sf + 1024);
+                            sf_copy<CG>(tsf + 12, sf + 2048);
+                            sf_copy<CG>(tsf + 4, sf + 512);
+                            sf_copy<CG>(tsf + 16, sf + 1536);
+                            sf_copy<CG>(tsf + 20, sf + 2560);
+                            mx_mma<CG>(d, ad, bd, idesc0, tsf, tsf + 8 + boff, kb != 0 ? 1u : 0u);
+                            mx_mma<CG>(d, ad + 2u, bd + 2u, idesc2, tsf, tsf + 8 + boff, 1u);
+                            mx_mma<CG>(d, ad + 4u, bd + 4u, idesc0, tsf + 4, tsf + 16 + boff, 1u);
+                            mx_mma<CG>(d, ad + 6u, bd + 6u, idesc2, tsf + 4, tsf + 16 + boff, 1u);
+                            tzp::pair_commit<CG>(&empty[stage]);
+                        }
+                    } else if (issue) {  // the last values of a row
                         sf_copy<CG>(tsf, sf);
                         sf_copy<CG>(tsf + 8, sf + 1024);
                         sf_copy<CG>(tsf + 12, sf + 2048);
@@ -417,7 +431,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
             // Every MMA issued has completed before TMEM is released.
             if (issue) tzp::pair_commit<CG>(drain);
             __syncwarp();
-            tzp::pair_wait<CG>(drain, 0, status, nullptr);
+            tzp::mbar_wait(drain, 0, status, nullptr);
         }
     } else {
         // ---- epilogue: TMEM lane quarter (warp % 4), 64 of the columns ----
@@ -429,7 +443,8 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
         for (int t = t0; t < num_tiles; t += tstep) {
             int m, n;
             tile_of(t, m, n);
-            if (!tzp::warp_wait<CG>(&tfull[acc], acc_phase, status, abort_flag)) break;
+            if (t + tstep >= num_tiles) tzp::pdl_trigger();
+            if (!tzp::warp_wait(&tfull[acc], acc_phase, status, abort_flag)) break;
             tzp::tc_fence_after();
             const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN + sl * 64);
             const int row0 = (m * CG + static_cast<int>(rank)) * 128 + q4 * 32;
@@ -519,13 +534,13 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
         if (lane == 0) tzp::bulk_wait_all();
     }
 
-    tzp::pdl_trigger();
+    if (warp < 2) tzp::pdl_trigger();
     tzp::tc_fence_before();
     __syncthreads();
     if constexpr (CG == 2) {
         // The leader's last commit has arrived in CTA 1 too and both CTAs are done: nothing is under way to a
         // CTA that has left.
-        if (rank == 1 && threadIdx.x == 32) tzp::pair_wait<CG>(drain, 0, status, nullptr);
+        if (rank == 1 && threadIdx.x == 32) tzp::mbar_wait(drain, 0, status, nullptr);
         __syncwarp();
         tzp::cluster_sync();
     }
@@ -616,7 +631,7 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
                 const uint32_t phase = (i / STAGES) & 1;
-                if (!tzp::warp_wait<1>(&empty[s], phase ^ 1u, status, abort_flag)) break;
+                if (!tzp::warp_wait(&empty[s], phase ^ 1u, status, abort_flag)) break;
                 uint8_t* a = smem + s * C::STAGE;
                 armed |= 1u << s;
                 armed_par = (armed_par & ~(1u << s)) | (phase << s);
@@ -636,8 +651,8 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
             constexpr uint32_t idesc0 = mx_idesc(128, N, 0), idesc2 = mx_idesc(128, N, 2);
             for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
                 const int s = i % STAGES;
-                if (!tzp::warp_wait<1>(&xready[i], 0, status, abort_flag)) break;
-                if (!tzp::warp_wait<1>(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
+                if (!tzp::warp_wait(&xready[i], 0, status, abort_flag)) break;
+                if (!tzp::warp_wait(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t a = tzp::smem_u32(smem + s * C::STAGE), b = tzp::smem_u32(xq + i * C::B_KB);
                 const uint32_t tsf = tmem_base + static_cast<uint32_t>(C::SF0 + s * C::SF_COLS);
@@ -1008,7 +1023,8 @@ int tz_linear_mxfp4_workspace(int64_t m, int k, int n, size_t* bytes) {
     TZ_CHECK(bytes, TZ_EINVAL, "%s: null argument", fn);
     int rc;
     if ((rc = check_dims(fn, m, k)) || (rc = check_dims(fn, n, k))) return rc;
-    *bytes = a256(code_bytes(m, k)) + a256(scale_bytes(m, k));
+    const bool in_kernel = m <= 16 && ceil_div(k, 256) <= MxRowsCfg<16>::MAX_KB && n <= 128 * 65535;  // x is quantised there
+    *bytes = in_kernel ? 0 : a256(code_bytes(m, k)) + a256(scale_bytes(m, k));
     return TZ_OK;
 }
 
@@ -1016,7 +1032,7 @@ static int check_workspace(const char* fn, const void* ws, size_t ws_bytes, int6
     size_t need = 0;
     int rc = tz_linear_mxfp4_workspace(m, k, n, &need);
     if (rc) return rc;
-    TZ_CHECK(ws && al16(ws) && ws_bytes >= need, TZ_EINVAL, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", fn, ws_bytes, need);
+    TZ_CHECK(need == 0 || (ws && al16(ws) && ws_bytes >= need), TZ_EINVAL, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", fn, ws_bytes, need);
     return TZ_OK;
 }
 static int quantize_input(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, void* ws, int64_t m, int k, cudaStream_t s, Q4* out) {

@@ -42,40 +42,12 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar_addr, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar_addr), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// mbar_wait (same 1 s bound) with cluster scope: for barriers on which the other CTA of a pair arrives.
-template <int CG>
-__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, int* status, volatile int* abort) {
-    if constexpr (CG == 1) return mbar_wait(bar, parity, status, abort);
-    const uint32_t a = smem_u32(bar);
-    if (mbar_try_wait_cluster(a, parity)) return true;
-    const uint64_t t0 = globaltimer();
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait_cluster(a, parity)) return true;
-        if ((i & 63u) == 0) {
-            if (abort && *abort) return false;
-            if (globaltimer() - t0 > kWaitLimitNs) {
-                if (status) atomicOr(status, TZ_DEV_TIMEOUT);
-                if (abort) *abort = 1;
-                return false;
-            }
-        }
-    }
-}
-
-// The same by a whole warp, with one answer for all lanes (a wait that ran out in one lane must not split the warp).
-template <int CG>
+// A whole warp's bounded wait, with one answer for all lanes (a wait that ran out in one lane must not split the
+// warp).  What the waiting side then reads was written by TMA or by tcgen05, ordered by the barrier's byte count and
+// the tcgen05 fences, so the plain CTA-scope form does for the barriers that the other CTA of a pair signals too.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, volatile int* abort) {
-    return __all_sync(0xFFFFFFFFu, pair_wait<CG>(bar, parity, status, abort));
+    if (__all_sync(0xFFFFFFFFu, mbar_try_wait(smem_u32(bar), parity))) return true;
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, status, abort));
 }
 
 // 2-D tiled load into this CTA's shared memory, its bytes counted on the barrier at cluster address `bar`
@@ -159,8 +131,8 @@ namespace tz {
 // Programmatic launches and progress: CTAs that wait in griddepcontrol.wait hold their SM's threads and
 // registers.  If small CTAs of a later kernel got there while clusters of the awaited kernel were still to be
 // placed, they could take every slot that such a cluster needs, and both would wait for good.  So the cluster
-// kernels call launch_dependents only when a CTA's work is done, and the small kernels around them
-// (quantisers, partial sums) are launched without the attribute.
+// kernels call launch_dependents only at a CTA's last tile, when every cluster of the grid has long been placed,
+// and the small kernels around them (quantisers, partial sums) are launched without the attribute.
 template <typename... KArgs, typename... Args>
 int launch_cluster(void (*kern)(KArgs...), int cg, dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl,
                    Args&&... args) {

@@ -488,7 +488,7 @@ def linear_mxfp4(ctx: Context, x, w: Mxfp4, bias=None, out_dtype=None, out=None)
         return out
     ldx = _rows16("linear_mxfp4", "x", x, (M, K), x.dtype)
     size = _mx_workspace(M, K, N)
-    ws = x.new_empty(size, dtype=torch.uint8)
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
     L.check(L.lib().tz_linear_mxfp4(ctx.handle, _p(x), ldx, _dtype_f("linear_mxfp4", x.dtype), w.codes_ptr, w.scales_ptr, _p(bias),
                                     _p(out), ydt, _p(ws), size, M, K, N, _stream()))
     return out
@@ -510,7 +510,7 @@ def gated_linear_mxfp4(ctx: Context, x, w: Mxfp4, act: str = "silu", out=None):
     else:
         _full16("gated_linear_mxfp4", "out", out, (T, F), x.dtype)
     size = _mx_workspace(T, D, 2 * F)
-    ws = x.new_empty(size, dtype=torch.uint8)
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
     L.check(L.lib().tz_gated_linear_mxfp4(ctx.handle, _p(x), ldx, _DTF[x.dtype], w.codes_ptr, w.scales_ptr, _p(out),
                                           _act_code("gated_linear_mxfp4", act), _p(ws), size, T, D, F, _stream()))
     return out

@@ -261,8 +261,9 @@ def test_refusals(ctx):
     with pytest.raises(TenzorError):
         ops.quantize_mxfp4(ctx, torch.zeros(4 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(4, 64))
     Lb, p = _lib.lib(), (lambda t: C.c_void_p(t.data_ptr()))
-    y = torch.empty(4, 16, device="cuda", dtype=torch.bfloat16)
-    assert Lb.tz_linear_mxfp4(ctx.handle, p(x), 64, 2, p(w.codes), p(w.scales), None, p(y), 2, p(y), 16, 4, 64, 16, None) == _lib.TZ_EINVAL
+    x = rand(40, 64, "bf16", 1)
+    y = torch.empty(40, 16, device="cuda", dtype=torch.bfloat16)
+    assert Lb.tz_linear_mxfp4(ctx.handle, p(x), 64, 2, p(w.codes), p(w.scales), None, p(y), 2, p(y), 16, 40, 64, 16, None) == _lib.TZ_EINVAL
     assert "workspace" in Lb.tz_get_last_error().decode()
     assert Lb.tz_linear_mxfp4(ctx.handle, p(x), 64, 3, p(w.codes), p(w.scales), None, p(y), 2, p(y), 16, 4, 64, 16, None) == _lib.TZ_EINVAL
     assert Lb.tz_quantize_mxfp4(None, p(x), 64, 2, p(w.codes), p(w.scales), 4, 64, None) == _lib.TZ_EINVAL
