@@ -31,34 +31,62 @@ __host__ __device__ __forceinline__ long long sf_chunk(long long row_block, int 
 }
 
 // ---- quantiser -------------------------------------------------------------------------------------
+// Eight consecutive values of a row as loaded: 4 words of 16-bit pairs, or 8 of f32.
 template <int DT>
-struct Elem;
-template <>
-struct Elem<DT_F32> { using T = float; };
-template <>
-struct Elem<DT_F16> { using T = __half; };
-template <>
-struct Elem<DT_BF16> { using T = __nv_bfloat16; };
-
-// 8 consecutive values as f32.
+struct Raw8 {
+    static constexpr int W = DT == DT_F32 ? 8 : 4;
+    uint32_t w[W];
+};
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, long long i, float (&v)[8]) {
+__device__ __forceinline__ Raw8<DT> load8(const void* p, long long i, bool in) {
+    Raw8<DT> r;
+    uint4 a = make_uint4(0, 0, 0, 0);
     if constexpr (DT == DT_F32) {
-        const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
-        const float4 a = __ldg(s), b = __ldg(s + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + i);
+        uint4 b = make_uint4(0, 0, 0, 0);
+        if (in) a = __ldg(s), b = __ldg(s + 1);
+        r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
     } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        if (in) a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i));
+    }
+    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+    if constexpr (DT == DT_BF16)
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    else
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <int DT>
+__device__ __forceinline__ void widen8(const Raw8<DT>& r, float (&v)[8]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float2 f;
-            if constexpr (DT == DT_BF16)
-                f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]));
-            else
-                f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (DT == DT_F32) {
+            v[2 * j] = __uint_as_float(r.w[2 * j]), v[2 * j + 1] = __uint_as_float(r.w[2 * j + 1]);
+        } else {
+            const float2 f = unpack16<DT>(r.w[j]);
             v[2 * j] = f.x, v[2 * j + 1] = f.y;
         }
+    }
+}
+// The largest f32 bit pattern of |x|: orders like the value, and an infinity or NaN stays on top.  16-bit values
+// are compared as packed 15-bit patterns first (the same order), and only the largest is widened.
+template <int DT>
+__device__ __forceinline__ uint32_t top8(const Raw8<DT>& r) {
+    if constexpr (DT == DT_F32) {
+        uint32_t t = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t = max(t, r.w[j] & 0x7FFFFFFFu);
+        return t;
+    } else {
+        uint32_t t = r.w[0] & 0x7FFF7FFFu;
+#pragma unroll
+        for (int j = 1; j < 4; ++j) t = __vmaxu2(t, r.w[j] & 0x7FFF7FFFu);
+        const uint32_t m = max(t & 0xFFFFu, t >> 16);
+        if constexpr (DT == DT_BF16) return m << 16;
+        return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
     }
 }
 
@@ -76,15 +104,15 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8], float inv) {
 }
 
 // Quantises a block spread over 4 neighbouring lanes (8 values each); returns the codes, `sc` the scale code.
-__device__ __forceinline__ uint32_t quant_block(const float (&v)[8], uint32_t& sc) {
-    // The largest bit pattern of |x|: orders like the value, and an infinity or NaN stays on top.
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+template <int DT>
+__device__ __forceinline__ uint32_t quant_block(const Raw8<DT>& r, uint32_t& sc) {
+    uint32_t top = top8<DT>(r);
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
     const uint32_t e = top >> 23;  // floor(log2) + 127; 0 for subnormals, whose scale is the smallest anyway
     sc = e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+    float v[8];
+    widen8<DT>(r, v);
     return e2m1x8(v, __uint_as_float((254u - (e == 255u ? 0u : sc)) << 23));
 }
 
@@ -100,16 +128,9 @@ __global__ void __launch_bounds__(256) quantize_mxfp4_kernel(const void* x, long
     const int k_chunks = (cols + 127) / 128;
     const int c0 = static_cast<int>(blockIdx.x) * 1024 + lane * 8;
     for (long long r = blockIdx.y * 8ll + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8ll) {
-        float v[4][8];
+        Raw8<DT> v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (c0 + 256 * j < cols) {
-                load8<DT>(x, r * ldx + c0 + 256 * j, v[j]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
-            }
-        }
+        for (int j = 0; j < 4; ++j) v[j] = load8<DT>(x, r * ldx + c0 + 256 * j, c0 + 256 * j < cols);
         const long long ro = GROUP > 0 ? (r / GROUP) * (2 * GROUP) + r % GROUP + off : r;
         uint8_t* srow = scales + sf_chunk(ro >> 7, 0, k_chunks) + (ro & 31) * 16 + ((ro & 127) >> 5) * 4;
 #pragma unroll
@@ -118,7 +139,7 @@ __global__ void __launch_bounds__(256) quantize_mxfp4_kernel(const void* x, long
             if (blockIdx.x * 1024 + 256 * j >= cols) break;  // the same for the whole warp
             const bool in = c < cols;
             uint32_t sc;
-            const uint32_t q = quant_block(v[j], sc);
+            const uint32_t q = quant_block<DT>(v[j], sc);
             if (in) *reinterpret_cast<uint32_t*>(codes + (ro * cols + c) / 2) = q;
             // lanes 0, 4, 8, 12 of each half warp hold the word's four bytes (0 for blocks past the row's end)
             uint32_t w = in ? sc << (8 * ((lane >> 2) & 3)) : 0u;
@@ -683,28 +704,21 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
         // N / 8 rows of the block, a lane 8 values of each.  Rows past the last one are zeros with the smallest scale.
         // The next block's values are on their way while a block is quantised. ----
         constexpr int R = N / C::QWARPS;
-        float v[R][8];
+        Raw8<XDT> v[R];
         auto fetch = [&](int kb) {
             const int c = kb * 256 + lane * 8;
 #pragma unroll
             for (int j = 0; j < R; ++j) {
                 const int r = warp - 2 + j * C::QWARPS;
-                if (r < p.rows && c < p.k) {
-                    load8<XDT>(p.x, r * p.ldx + c, v[j]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
-                }
+                v[j] = load8<XDT>(p.x, r * p.ldx + c, r < p.rows && c < p.k);
             }
         };
         fetch(kb0);
         for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
             uint8_t* blk = xq + i * C::B_KB;
-            float u[R][8];
+            Raw8<XDT> u[R];
 #pragma unroll
-            for (int j = 0; j < R; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) u[j][e] = v[j][e];
+            for (int j = 0; j < R; ++j) u[j] = v[j];
             if (kb + 1 < kb1) fetch(kb + 1);
 #pragma unroll
             for (int j = 0; j < R; ++j) {
@@ -712,7 +726,7 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
                 uint32_t q = 0, w = 0;
                 if (r < p.rows) {  // the same for the whole warp
                     uint32_t sc;
-                    q = quant_block(u[j], sc);
+                    q = quant_block<XDT>(u[j], sc);
                     w = sc << (8 * ((lane >> 2) & 3));
                     w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
                     w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
