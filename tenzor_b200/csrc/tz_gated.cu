@@ -198,6 +198,15 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         r.kb1 = min(p.kblocks, r.kb0 + p.kper);
         return true;
     };
+    auto range_at = [&](int i, int& kb0, int& kb1) -> bool {  // tile_at's K blocks alone, without its divisions
+        const int t = C::kDual && p.resident ? first + i : me + i * team;
+        kb0 = 0, kb1 = p.kblocks;
+        if (p.splits > 1 && t < num_tiles) {
+            kb0 = t / (per * p.which) * p.kper;
+            kb1 = min(p.kblocks, kb0 + p.kper);
+        }
+        return t < (C::kDual && p.resident ? last : num_tiles);
+    };
     const int ring = p.ring;
     // Shared memory: stage s holds an A tile and a B tile; with resident B tiles a ring of A tiles comes first,
     // then the B tile of every K block.
@@ -291,12 +300,12 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
-            Tile q;
-            for (int i = 0; ok && tile_at(i, q); ++i) {
+            int kb0, kb1;
+            for (int i = 0; ok && range_at(i, kb0, kb1); ++i) {
                 if (!tzp::warp_wait(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
-                for (int kb = q.kb0; kb < q.kb1; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!tzp::warp_wait(&full[stage], phase, status, abort_flag)) {
                         ok = false;
                         break;
@@ -309,7 +318,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                     if (issue) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const uint32_t more = (kb > q.kb0 || k > 0) ? 1u : 0u;
+                            const uint32_t more = (kb > kb0 || k > 0) ? 1u : 0u;
                             tzp::pair_mma_f16<CG>(d, ad + kAstep * k, bd + kBstep * k, idesc, more);
                             if constexpr (BN == 384)
                                 tzp::pair_mma_f16<CG>(d + 256, ad + kAstep * k, bd + (16384u >> 4) + kBstep * k, idesc_b, more);
@@ -343,8 +352,8 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         uint8_t* boxp = staging + e * C::BOX;
         int acc = 0, nb = 0;
         uint32_t acc_phase = 0, dh_phase = 0;
-        // BWD: the 32 x 32 box of dh that a tile needs comes by TMA into the box that later takes dg; it is asked
-        // for as soon as the previous tile's stores have read the box.
+        // BWD: the 32 x 32 box of dh that a tile needs comes by TMA into the first half of the warp's staging; once it
+        // is in registers the next tile's is asked for.  dg and du take turns in the second half.
         auto fetch_dh = [&](const Tile& q) {
             tzp::mbar_arrive_expect_tx(&dhbar[e], 2048);
             tzp::tma_load_2d(boxp, &tmDh, q.n * (BN / 2) + sl * 32, (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32, &dhbar[e]);
@@ -370,17 +379,18 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                 if constexpr (MODE == MM_BWD) {
                     if (!tzp::warp_wait(&dhbar[e], dh_phase, status, abort_flag)) break;
                     dh_phase ^= 1u;
-                    fetched = false;
+                    fetched = more;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const uint4 v = ld_shared_v4(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
                         dh[4 * c] = v.x, dh[4 * c + 1] = v.y, dh[4 * c + 2] = v.z, dh[4 * c + 3] = v.w;
                     }
-                    __syncwarp();  // every lane has its row before any lane writes dg over it
-                } else {
-                    if (lane == 0) tzp::bulk_wait_read<0>();  // the previous tile's store has read the box
-                    __syncwarp();
+                    __syncwarp();  // every lane has its row
+                    if (lane == 0 && more) fetch_dh(next);
                 }
+                if (lane == 0) tzp::bulk_wait_read<0>();  // the previous tile's last store has read the box
+                __syncwarp();
+                uint32_t o[16];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {  // 16 outputs at a time
                     uint32_t g[16], u[16];
@@ -397,34 +407,42 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                                 tzp::mbar_arrive(&tempty[acc]);
                         }
                     }
-                    uint32_t o[8], o2[8];
                     if constexpr (MODE == MM_FWD) {
-#define TZ_FWD(A) fwd_math<A, BF>(g, u, o)
+#define TZ_FWD(A) fwd_math<A, BF>(g, u, o + 8 * c)
                         TZ_ACT_SWITCH(p.act, TZ_FWD)
 #undef TZ_FWD
+                        stage64<2>(box, lane, 2 * c, o + 8 * c);
                     } else {
-#define TZ_BWD(A) bwd_math<A, BF>(g, u, dh + 8 * c, o, o2)
+                        uint32_t o2[8];
+#define TZ_BWD(A) bwd_math<A, BF>(g, u, dh + 8 * c, o + 8 * c, o2)
                         TZ_ACT_SWITCH(p.act, TZ_BWD)
 #undef TZ_BWD
                         stage64<2>(box + 2048, lane, 2 * c, o2);
                     }
-                    stage64<2>(box, lane, 2 * c, o);
                 }
                 tzp::fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) {
-                    if (col0 < p.cols) {
+                const bool store = lane == 0 && col0 < p.cols;
+                if constexpr (MODE == MM_FWD) {
+                    if (store) {
                         tzp::tma_store_2d(&tmO0, boxp, col0, row0);
-                        if constexpr (MODE == MM_BWD) tzp::tma_store_2d(&tmO1, boxp + 2048, col0, row0);
                         tzp::bulk_commit();
                     }
-                    if constexpr (MODE == MM_BWD) {
+                } else {
+                    if (store) {
+                        tzp::tma_store_2d(&tmO1, boxp + 2048, col0, row0);
+                        tzp::bulk_commit();
                         tzp::bulk_wait_read<0>();
-                        if (more) fetch_dh(next);
+                    }
+                    __syncwarp();
+                    stage64<4>(box + 2048, lane, 0, o);
+                    tzp::fence_proxy_async();
+                    __syncwarp();
+                    if (store) {
+                        tzp::tma_store_2d(&tmO0, boxp + 2048, col0, row0);
+                        tzp::bulk_commit();
                     }
                 }
-                __syncwarp();
-                if constexpr (MODE == MM_BWD) fetched = more;
             } else {
                 constexpr int CH = BN / 64;
 #pragma unroll 1
