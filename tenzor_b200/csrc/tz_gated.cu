@@ -560,16 +560,18 @@ int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const M
     CUtensorMap ma0, ma1, mb0, mb1, mo0, mo1, mdh;
     const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B;
     const int arows = C::kAmn ? 64 : 128, brows = C::kBmn ? 64 : (C::kDual ? BN / 2 : C::BNC);
-    if ((rc = map16<BF>(&ma0, a0, 64, arows, S128)) || (rc = map16<BF>(&ma1, a1, 64, arows, S128)) ||
-        (rc = map16<BF>(&mb0, b0, 64, brows, S128)) || (rc = map16<BF>(&mb1, b1, 64, brows, S128)))
-        return rc;
+    if ((rc = map16<BF>(&ma0, a0, 64, arows, S128)) || (rc = map16<BF>(&mb0, b0, 64, brows, S128))) return rc;
+    ma1 = ma0, mb1 = mb0;  // an encoding costs about as much as the rest of the launch's arguments
+    if (a1.p != a0.p && (rc = map16<BF>(&ma1, a1, 64, arows, S128))) return rc;
+    if (b1.p != b0.p && (rc = map16<BF>(&mb1, b1, 64, brows, S128))) return rc;
     if (PART) {
         rc = encode_tmap_2d_swz(&mo0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, o0.cols,
                                 static_cast<uint64_t>(p.splits) * p.which * p.m_pad, o0.cols * 4, 32, 32, S128);
         mo1 = mo0;
     } else {
         rc = map16<BF>(&mo0, o0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
-        if (!rc) rc = map16<BF>(&mo1, o1, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+        mo1 = mo0;
+        if (!rc && o1.p != o0.p) rc = map16<BF>(&mo1, o1, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
     }
     if (rc) return rc;
     mdh = mo0;

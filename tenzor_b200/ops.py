@@ -288,54 +288,71 @@ def concat(ctx: Context, xs, axis: int):
 
 # ---- gated feed-forward block ----------------------------------------------------------------------
 GATED_ACTS = ("silu", "gelu", "gelu_erf", "relu", "sigmoid")
+_ACT_CODE = {a: L.OP[a] for a in GATED_ACTS}
 _DT16 = {torch.float16: 0, torch.bfloat16: 1}  # tz_gemm_prec
 
 
-def _dtype16(fn, t):
-    d = _DT16.get(t.dtype)
+def _dtype16(fn, dtype):
+    d = _DT16.get(dtype)
     if d is None:
-        raise TypeError(f"{fn}: float16 or bfloat16 tensors, got {t.dtype}")
+        raise TypeError(f"{fn}: float16 or bfloat16 tensors, got {dtype}")
     return d
 
 
 def _act_code(fn, act):
-    if act not in GATED_ACTS:
+    c = _ACT_CODE.get(act)
+    if c is None:
         raise ValueError(f"{fn}: activation {act!r} is not one of {GATED_ACTS}")
-    return L.OP[act]
+    return c
 
 
-def _rows16(fn, name, t, shape, dtype):
-    """Row stride of a 2-D device tensor of `shape` whose rows are contiguous."""
-    if not t.is_cuda or t.dtype != dtype or t.shape != shape or (t.stride(1) != 1 and shape[1] > 1):
-        raise ValueError(f"{fn}: {name} must be a CUDA {dtype} tensor of shape {tuple(shape)} with contiguous rows, "
+def _on(fn, ctx):
+    """The stream to launch on: the current one of the context's device, which has to be the current device."""
+    d = torch.cuda.current_device()
+    if d != ctx.device:
+        raise ValueError(f"{fn}: the context is on device {ctx.device}, the current device is {d}")
+    return torch._C._cuda_getCurrentRawStream(d) or CUDA_STREAM_LEGACY
+
+
+def _rows(fn, name, ctx, t, rows, cols, dtype):
+    """Row stride of a matrix [rows, cols] on the context's device whose rows are contiguous."""
+    if t.dtype is not dtype or t.shape != (rows, cols) or t.get_device() != ctx.device or (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"{fn}: {name} must be a {dtype} tensor of shape {(rows, cols)} on device {ctx.device} with "
+                         f"contiguous rows, got {t.dtype} {tuple(t.shape)} stride {t.stride()} on {t.device}")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _full(fn, name, ctx, t, shape, dtype):
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != ctx.device or not t.is_contiguous():
+        raise ValueError(f"{fn}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on device {ctx.device}, "
                          f"got {t.dtype} {tuple(t.shape)} stride {t.stride()} on {t.device}")
-    return t.stride(0) if shape[0] > 1 else shape[1]
 
 
-def _full16(fn, name, t, shape, dtype):
-    if not t.is_cuda or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{fn}: {name} must be a contiguous CUDA {dtype} tensor of shape {tuple(shape)}, "
-                         f"got {t.dtype} {tuple(t.shape)} stride {t.stride()} on {t.device}")
-    return t
+def _two(fn, x, w):
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"{fn}: x [T, D] and weights [F, D], got {tuple(x.shape)} and {tuple(w.shape)}")
 
 
 def gated_linear(ctx: Context, x, w_gate, w_up, act: str = "silu", out=None):
     """act(x @ w_gate.T) * (x @ w_up.T) in one kernel: x [T, D] (rows may be strided), w_gate and w_up [F, D],
     all float16 or all bfloat16, D and F multiples of 8; returns [T, F].  act: one of GATED_ACTS."""
-    dt = _dtype16("gated_linear", x)
-    if x.dim() != 2 or w_gate.dim() != 2:
-        raise ValueError(f"gated_linear: x [T, D] and weights [F, D], got {tuple(x.shape)} and {tuple(w_gate.shape)}")
+    dtype = x.dtype
+    dt = _dtype16("gated_linear", dtype)
+    code = _act_code("gated_linear", act)
+    _two("gated_linear", x, w_gate)
     T, D = x.shape
     F = w_gate.shape[0]
-    ldx = _rows16("gated_linear", "x", x, (T, D), x.dtype)
-    _full16("gated_linear", "w_gate", w_gate, (F, D), x.dtype)
-    _full16("gated_linear", "w_up", w_up, (F, D), x.dtype)
+    ldx = _rows("gated_linear", "x", ctx, x, T, D, dtype)
+    _full("gated_linear", "w_gate", ctx, w_gate, (F, D), dtype)
+    _full("gated_linear", "w_up", ctx, w_up, (F, D), dtype)
     if out is None:
         out = x.new_empty((T, F))
     else:
-        _full16("gated_linear", "out", out, (T, F), x.dtype)
-    L.check(L.lib().tz_gated_linear(ctx.handle, _p(x), ldx, _p(w_gate), _p(w_up), _p(out), T, D, F,
-                                    _act_code("gated_linear", act), dt, _stream()))
+        _full("gated_linear", "out", ctx, out, (T, F), dtype)
+    rc = L.lib().tz_gated_linear(ctx.handle, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), out.data_ptr(), T, D, F,
+                                 code, dt, _on("gated_linear", ctx))
+    if rc:
+        L.check(rc)
     return out
 
 
@@ -347,23 +364,27 @@ def _gated_workspace(sms, t, d, f):
 
 
 def gated_linear_backward(ctx: Context, x, w_gate, w_up, dh, act: str = "silu"):
-    """(dx, dw_gate, dw_up) of gated_linear for the output's gradient dh [T, F]."""
-    dt = _dtype16("gated_linear_backward", x)
-    if x.dim() != 2 or w_gate.dim() != 2:
-        raise ValueError(f"gated_linear_backward: x [T, D] and weights [F, D], got {tuple(x.shape)} and "
-                         f"{tuple(w_gate.shape)}")
+    """(dx, dw_gate, dw_up) of gated_linear for the output's gradient dh [T, F] (rows may be strided)."""
+    fn = "gated_linear_backward"
+    dtype = x.dtype
+    dt = _dtype16(fn, dtype)
+    code = _act_code(fn, act)
+    _two(fn, x, w_gate)
     T, D = x.shape
     F = w_gate.shape[0]
-    ldx = _rows16("gated_linear_backward", "x", x, (T, D), x.dtype)
-    lddh = _rows16("gated_linear_backward", "dh", dh, (T, F), x.dtype)
-    _full16("gated_linear_backward", "w_gate", w_gate, (F, D), x.dtype)
-    _full16("gated_linear_backward", "w_up", w_up, (F, D), x.dtype)
-    code = _act_code("gated_linear_backward", act)
+    ldx = _rows(fn, "x", ctx, x, T, D, dtype)
+    lddh = _rows(fn, "dh", ctx, dh, T, F, dtype)
+    _full(fn, "w_gate", ctx, w_gate, (F, D), dtype)
+    _full(fn, "w_up", ctx, w_up, (F, D), dtype)
+    stream = _on(fn, ctx)
     size = _gated_workspace(ctx.sm_count - ctx.sm_reserve, T, D, F)
     ws = x.new_empty(size, dtype=torch.uint8)
     dx, dwg, dwu = x.new_empty((T, D)), x.new_empty((F, D)), x.new_empty((F, D))
-    L.check(L.lib().tz_gated_linear_backward(ctx.handle, _p(x), ldx, _p(w_gate), _p(w_up), _p(dh), lddh, _p(dx), _p(dwg),
-                                             _p(dwu), _p(ws), size, T, D, F, code, dt, _stream()))
+    rc = L.lib().tz_gated_linear_backward(ctx.handle, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), dh.data_ptr(), lddh,
+                                          dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), ws.data_ptr(), size, T, D, F, code, dt,
+                                          stream)
+    if rc:
+        L.check(rc)
     return dx, dwg, dwu
 
 
@@ -376,12 +397,13 @@ class Mxfp4:
     tenzor_cuda.h), one allocation.  With `gated` the rows are two weight matrices interleaved by
     pack_gated_mxfp4."""
 
-    __slots__ = ("buf", "rows", "cols", "gated", "codes_ptr", "scales_ptr")
+    __slots__ = ("buf", "rows", "cols", "gated", "index", "codes_ptr", "scales_ptr")
 
     def __init__(self, rows, cols, like, gated=False):
         self.rows, self.cols, self.gated = rows, cols, gated
         off, size = _mx_layout(rows, cols)
         self.buf = like.new_empty(size, dtype=torch.uint8)
+        self.index = like.get_device()
         self.codes_ptr = self.buf.data_ptr()
         self.scales_ptr = self.codes_ptr + off
 
@@ -403,7 +425,7 @@ class Mxfp4:
 
 
 def _mx_layout(rows, cols):
-    """Byte offset of the scales behind the codes, and the bytes of both (what tz_linear_mxfp4_workspace adds up)."""
+    """Byte offset of the scales behind the codes (256-byte aligned), and the bytes of both."""
     off = (rows * (cols // 2) + 255) // 256 * 256
     return off, off + (rows + 127) // 128 * ((cols + 127) // 128) * 512
 
@@ -420,6 +442,11 @@ def _mx_cols(fn, cols):
         raise ValueError(f"{fn}: the row length must be a positive multiple of 32, got {cols}")
 
 
+def _mx(fn, name, ctx, q):
+    if not isinstance(q, Mxfp4) or q.index != ctx.device:
+        raise ValueError(f"{fn}: {name} must be an Mxfp4 on device {ctx.device}")
+
+
 def quantize_mxfp4(ctx: Context, x) -> Mxfp4:
     """x [rows, cols] (float32, float16 or bfloat16; rows may be strided) in MXFP4, cols a multiple of 32."""
     dt = _dtype_f("quantize_mxfp4", x.dtype)
@@ -427,33 +454,42 @@ def quantize_mxfp4(ctx: Context, x) -> Mxfp4:
         raise ValueError(f"quantize_mxfp4: a matrix, got {tuple(x.shape)}")
     rows, cols = x.shape
     _mx_cols("quantize_mxfp4", cols)
-    ldx = _rows16("quantize_mxfp4", "x", x, (rows, cols), x.dtype)
+    ldx = _rows("quantize_mxfp4", "x", ctx, x, rows, cols, x.dtype)
+    stream = _on("quantize_mxfp4", ctx)
     q = Mxfp4(rows, cols, x)
-    L.check(L.lib().tz_quantize_mxfp4(ctx.handle, _p(x), ldx, dt, q.codes_ptr, q.scales_ptr, rows, cols, _stream()))
+    rc = L.lib().tz_quantize_mxfp4(ctx.handle, x.data_ptr(), ldx, dt, q.codes_ptr, q.scales_ptr, rows, cols, stream)
+    if rc:
+        L.check(rc)
     return q
 
 
 def dequantize_mxfp4(ctx: Context, q: Mxfp4, dtype=torch.float32):
     """The values q stands for, as [rows, cols] of `dtype`."""
     dt = _dtype_f("dequantize_mxfp4", dtype)
+    _mx("dequantize_mxfp4", "q", ctx, q)
     if q.gated:
         raise ValueError("dequantize_mxfp4: a gated pair's rows are interleaved; quantise the matrices one by one")
-    out = q.buf.new_empty(q.shape, dtype=dtype)
-    L.check(L.lib().tz_dequantize_mxfp4(ctx.handle, q.codes_ptr, q.scales_ptr, _p(out), dt, q.rows, q.cols, _stream()))
+    stream = _on("dequantize_mxfp4", ctx)
+    out = q.buf.new_empty((q.rows, q.cols), dtype=dtype)
+    rc = L.lib().tz_dequantize_mxfp4(ctx.handle, q.codes_ptr, q.scales_ptr, out.data_ptr(), dt, q.rows, q.cols, stream)
+    if rc:
+        L.check(rc)
     return out
 
 
 def pack_gated_mxfp4(ctx: Context, w_gate, w_up) -> Mxfp4:
     """w_gate and w_up [F, D] (F a multiple of 16, D of 32) as the weights of gated_linear_mxfp4."""
-    dt = _dtype_f("pack_gated_mxfp4", w_gate.dtype)
+    fn = "pack_gated_mxfp4"
+    dt = _dtype_f(fn, w_gate.dtype)
     if w_gate.dim() != 2 or w_gate.shape[0] % 16 or w_gate.shape[0] == 0:
-        raise ValueError(f"pack_gated_mxfp4: [F, D] with F a positive multiple of 16, got {tuple(w_gate.shape)}")
+        raise ValueError(f"{fn}: [F, D] with F a positive multiple of 16, got {tuple(w_gate.shape)}")
     F, D = w_gate.shape
-    _mx_cols("pack_gated_mxfp4", D)
-    _full16("pack_gated_mxfp4", "w_gate", w_gate, (F, D), w_gate.dtype)
-    _full16("pack_gated_mxfp4", "w_up", w_up, (F, D), w_gate.dtype)
+    _mx_cols(fn, D)
+    _full(fn, "w_gate", ctx, w_gate, (F, D), w_gate.dtype)
+    _full(fn, "w_up", ctx, w_up, (F, D), w_gate.dtype)
+    stream = _on(fn, ctx)
     q = Mxfp4(2 * F, D, w_gate, gated=True)
-    L.check(L.lib().tz_pack_gated_mxfp4(ctx.handle, _p(w_gate), _p(w_up), dt, q.codes_ptr, q.scales_ptr, F, D, _stream()))
+    L.check(L.lib().tz_pack_gated_mxfp4(ctx.handle, w_gate.data_ptr(), w_up.data_ptr(), dt, q.codes_ptr, q.scales_ptr, F, D, stream))
     return q
 
 
@@ -467,50 +503,65 @@ def _mx_workspace(m, k, n):
 def linear_mxfp4(ctx: Context, x, w: Mxfp4, bias=None, out_dtype=None, out=None):
     """q(x) @ w.T (+ bias f32 [N]): x [M, K] (float32, float16 or bfloat16, quantised in the call) or an Mxfp4;
     returns [M, N] of `out_dtype` (x's type; float32 for an Mxfp4).  N is a multiple of 8."""
+    fn = "linear_mxfp4"
+    _mx(fn, "w", ctx, w)
     given = isinstance(x, Mxfp4)
     if w.gated or (given and x.gated):
-        raise ValueError("linear_mxfp4: a gated pair of weights goes to gated_linear_mxfp4")
+        raise ValueError(f"{fn}: a gated pair of weights goes to gated_linear_mxfp4")
     if len(x.shape) != 2 or x.shape[1] != w.cols:
-        raise ValueError(f"linear_mxfp4: x [M, {w.cols}], got {tuple(x.shape)}")
+        raise ValueError(f"{fn}: x [M, {w.cols}], got {tuple(x.shape)}")
     M, K = x.shape
     N = w.rows
-    out_dtype = out_dtype or (torch.float32 if given else x.dtype)
-    ydt = _dtype_f("linear_mxfp4", out_dtype)
+    if out_dtype is None:
+        out_dtype = torch.float32 if given else x.dtype
+    ydt = _dtype_f(fn, out_dtype)
     if bias is not None:
-        _full16("linear_mxfp4", "bias", bias, (N,), torch.float32)
+        _full(fn, "bias", ctx, bias, (N,), torch.float32)
+        bias = bias.data_ptr()
+    stream = _on(fn, ctx)
     if out is None:
         out = w.buf.new_empty((M, N), dtype=out_dtype)
     else:
-        _full16("linear_mxfp4", "out", out, (M, N), out_dtype)
+        _full(fn, "out", ctx, out, (M, N), out_dtype)
     if given:
-        L.check(L.lib().tz_gemm_mxfp4(ctx.handle, x.codes_ptr, x.scales_ptr, w.codes_ptr, w.scales_ptr, _p(bias), _p(out), ydt,
-                                      M, K, N, _stream()))
-        return out
-    ldx = _rows16("linear_mxfp4", "x", x, (M, K), x.dtype)
-    size = _mx_workspace(M, K, N)
-    ws = x.new_empty(size, dtype=torch.uint8) if size else None
-    L.check(L.lib().tz_linear_mxfp4(ctx.handle, _p(x), ldx, _dtype_f("linear_mxfp4", x.dtype), w.codes_ptr, w.scales_ptr, _p(bias),
-                                    _p(out), ydt, _p(ws), size, M, K, N, _stream()))
+        _mx(fn, "x", ctx, x)
+        rc = L.lib().tz_gemm_mxfp4(ctx.handle, x.codes_ptr, x.scales_ptr, w.codes_ptr, w.scales_ptr, bias, out.data_ptr(), ydt,
+                                   M, K, N, stream)
+    else:
+        ldx = _rows(fn, "x", ctx, x, M, K, x.dtype)
+        size = _mx_workspace(M, K, N)
+        ws = x.new_empty(size, dtype=torch.uint8) if size else None
+        rc = L.lib().tz_linear_mxfp4(ctx.handle, x.data_ptr(), ldx, _dtype_f(fn, x.dtype), w.codes_ptr, w.scales_ptr, bias,
+                                     out.data_ptr(), ydt, ws.data_ptr() if size else None, size, M, K, N, stream)
+    if rc:
+        L.check(rc)
     return out
 
 
 def gated_linear_mxfp4(ctx: Context, x, w: Mxfp4, act: str = "silu", out=None):
     """act(q(x) @ wg.T) * (q(x) @ wu.T) with the weights of pack_gated_mxfp4: x [T, D] float16 or bfloat16;
     returns [T, F]."""
-    _dtype16("gated_linear_mxfp4", x)
+    fn = "gated_linear_mxfp4"
+    dtype = x.dtype
+    _dtype16(fn, dtype)
+    code = _act_code(fn, act)
+    _mx(fn, "w", ctx, w)
     if not w.gated:
-        raise ValueError("gated_linear_mxfp4: weights come from pack_gated_mxfp4")
+        raise ValueError(f"{fn}: weights come from pack_gated_mxfp4")
     if x.dim() != 2 or x.shape[1] != w.cols:
-        raise ValueError(f"gated_linear_mxfp4: x [T, {w.cols}], got {tuple(x.shape)}")
+        raise ValueError(f"{fn}: x [T, {w.cols}], got {tuple(x.shape)}")
     T, D = x.shape
     F = w.rows // 2
-    ldx = _rows16("gated_linear_mxfp4", "x", x, (T, D), x.dtype)
+    ldx = _rows(fn, "x", ctx, x, T, D, dtype)
+    stream = _on(fn, ctx)
     if out is None:
         out = x.new_empty((T, F))
     else:
-        _full16("gated_linear_mxfp4", "out", out, (T, F), x.dtype)
+        _full(fn, "out", ctx, out, (T, F), dtype)
     size = _mx_workspace(T, D, 2 * F)
     ws = x.new_empty(size, dtype=torch.uint8) if size else None
-    L.check(L.lib().tz_gated_linear_mxfp4(ctx.handle, _p(x), ldx, _DTF[x.dtype], w.codes_ptr, w.scales_ptr, _p(out),
-                                          _act_code("gated_linear_mxfp4", act), _p(ws), size, T, D, F, _stream()))
+    rc = L.lib().tz_gated_linear_mxfp4(ctx.handle, x.data_ptr(), ldx, _DTF[dtype], w.codes_ptr, w.scales_ptr, out.data_ptr(), code,
+                                       ws.data_ptr() if size else None, size, T, D, F, stream)
+    if rc:
+        L.check(rc)
     return out
