@@ -679,7 +679,7 @@ int launch_rows(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const 
     const int tiles = ceil_div(h.cols, 128);
     p.kblocks = ceil_div(x.cols, 64);
     int splits = 1;
-    if ((rc = rows_splits<N>(kern, C::THREADS, C::SMEM, ctx->sm_count - ctx->sm_reserve, tiles, p.kblocks, C::MAX_SPLIT, &splits))) return rc;
+    if ((rc = rows_splits<N>(kern, C::THREADS, [](int) { return C::SMEM; }, ctx->sm_count - ctx->sm_reserve, tiles, p.kblocks, C::MAX_SPLIT, &splits))) return rc;
     p.kper = ceil_div(p.kblocks, splits);
     p.t = static_cast<int>(x.rows);
     p.f = static_cast<int>(h.cols);

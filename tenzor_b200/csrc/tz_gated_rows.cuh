@@ -188,25 +188,27 @@ __global__ void __launch_bounds__(RowsCfg<N>::THREADS, 1)
 }
 
 // K splits of a feature tile: the most (up to 8, each with at least 4 K blocks) with which the clusters of all
-// tiles still run at one time.  How many clusters of a size fit is asked of the runtime once: their CTAs have to
-// lie in one GPC, so 148 SMs hold fewer than 148 / size of them (48 tiles as clusters of 3 took two waves,
-// 18.5 us, where clusters of 2 take one, 12.4 us).  TAG: one per kernel.
-template <int TAG, typename K>
-int rows_splits(K kern, int threads, int smem, int sms, int tiles, int kblocks, int most, int* out) {
-    static std::atomic<int> fit[16][9];  // by device; 0 = not asked
+// tiles still run at one time.  How many clusters of a size and shared memory (`smem` of the K blocks of one rank)
+// fit is asked of the runtime once: their CTAs have to lie in one GPC, so 148 SMs hold fewer than 148 / size of
+// them (48 tiles as clusters of 3 took two waves, 18.5 us, where clusters of 2 take one, 12.4 us).  TAG: one per
+// kernel.
+template <int TAG, typename K, typename Smem>
+int rows_splits(K kern, int threads, Smem smem, int max_ctas, int tiles, int kblocks, int most, int* out) {
+    static std::atomic<int> fit[16][9][33];  // by device, size and K blocks of a rank (32: or more); 0 = not asked
     int dev = 0;
     TZ_CUDA(cudaGetDevice(&dev));
     *out = 1;
     for (int s = most < 8 ? most : 8; s > 1; --s) {
-        if (kblocks < 4 * s || static_cast<int64_t>(tiles) * s > sms) continue;
+        if (kblocks < 4 * s || static_cast<int64_t>(tiles) * s > max_ctas) continue;
         const int per = (kblocks + s - 1) / s;
         if ((kblocks + per - 1) / per != s) continue;  // every rank has work
-        int n = fit[dev & 15][s].load(std::memory_order_relaxed);
+        std::atomic<int>& slot = fit[dev & 15][s][per < 32 ? per : 32];
+        int n = slot.load(std::memory_order_relaxed);
         if (n == 0) {
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3(s);
             cfg.blockDim = dim3(threads);
-            cfg.dynamicSmemBytes = smem;
+            cfg.dynamicSmemBytes = smem(per < 32 ? per : 32);
             cudaLaunchAttribute attr;
             attr.id = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = s;
@@ -215,7 +217,7 @@ int rows_splits(K kern, int threads, int smem, int sms, int tiles, int kblocks, 
             cfg.numAttrs = 1;
             TZ_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
             n = n > 0 ? n : -1;
-            fit[dev & 15][s].store(n, std::memory_order_relaxed);
+            slot.store(n, std::memory_order_relaxed);
         }
         if (tiles <= n) {
             *out = s;

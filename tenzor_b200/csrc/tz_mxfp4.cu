@@ -614,10 +614,10 @@ struct MxRowsCfg {
     static constexpr int QWARPS = 8;
     static constexpr int THREADS = 64 + 32 * QWARPS;
     static constexpr int STAGE = 16384 + 1024;
-    static constexpr int STAGES = 5;
+    static constexpr int STAGES = 4;             // two CTAs fit an SM: the MMA issue of one K block (about 700 clocks) is serial
     static constexpr int SF_COLS = 16;           // per stage: A 2 x 4, B 2 x 4
     static constexpr int SF0 = 32;
-    static constexpr int TCOLS = 128;            // 32 + 5 * 16 = 112
+    static constexpr int TCOLS = 128;            // 32 + 4 * 16
     static constexpr int B_KB = N * 128 + 1024;  // one K block of x: codes and two scale chunks
     static constexpr int PART = 128 * N * 4;
     static constexpr int MAX_SPLIT = 1 + STAGES * STAGE / PART;
@@ -626,7 +626,7 @@ struct MxRowsCfg {
 };
 
 template <int N, int XDT, int OUT, bool GATED>
-__global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
+__global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 2)
     mxfp4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW, const MxRowsParams p, int* status) {
     using C = MxRowsCfg<N>;
     constexpr int STAGES = C::STAGES;
@@ -903,8 +903,8 @@ int launch_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int rows, const Q4&
     int rc = ensure_smem(kern, C::smem(C::MAX_KB), done);
     if (rc) return rc;
     int splits = 1;
-    if ((rc = rows_splits<N * 100 + XDT * 20 + OUT * 4 + GATED + 1>(kern, C::THREADS, C::smem(8), ctx->sm_count - ctx->sm_reserve, tiles, kblocks,
-                                                                    C::MAX_SPLIT, &splits)))
+    const int ctas = 2 * (ctx->sm_count - ctx->sm_reserve);
+    if ((rc = rows_splits<N * 100 + XDT * 20 + OUT * 4 + GATED + 1>(kern, C::THREADS, C::smem, ctas, tiles, kblocks, C::MAX_SPLIT, &splits)))
         return rc;
     MxRowsParams p{};
     p.kblocks = kblocks;
