@@ -701,6 +701,8 @@ int forward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat&
     p.kblocks = p.kper = ceil_div(x.cols, 64);
     p.cols = static_cast<int>(h.cols);
     p.act = act;
+    if (x.rows <= 128 && p.n_tiles > (ctx->sm_count - ctx->sm_reserve) / 2)  // half of a pair's rows would be empty
+        return launch_mm<1, kBN, MM_FWD, BF, false>(ctx, x, x, wg, wu, h, h, nullptr, p, nullptr, s);
     return launch_mm<kCG, kBN, MM_FWD, BF, false>(ctx, x, x, wg, wu, h, h, nullptr, p, nullptr, s);
 }
 

@@ -849,10 +849,10 @@ struct Q4 {
     int64_t rows;
 };
 
-template <int OUT, bool GATED>
-int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, void* y, int act, cudaStream_t s) {
-    using C = MxCfg<kCG>;
-    auto kern = mxfp4_mm_kernel<kCG, OUT, GATED>;
+template <int CG, int OUT, bool GATED>
+int launch_mx_cg(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, void* y, int act, cudaStream_t s) {
+    using C = MxCfg<CG>;
+    auto kern = mxfp4_mm_kernel<CG, OUT, GATED>;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::SMEM, done);
     if (rc) return rc;
@@ -872,7 +872,7 @@ int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, 
                                 cols * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc) return rc;
     MxParams p{};
-    p.m_tiles = ceil_div(a.rows, 128 * kCG);
+    p.m_tiles = ceil_div(a.rows, 128 * CG);
     p.n_tiles = ceil_div(b.rows, C::BN);
     p.rows = static_cast<int>(a.rows);
     p.n = static_cast<int>(b.rows);
@@ -881,10 +881,17 @@ int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, 
     p.bias = bias;
     p.act = act;
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-    const int groups = (ctx->sm_count - ctx->sm_reserve) / kCG;
-    const int grid = static_cast<int>(tiles < groups ? tiles : groups) * kCG;
-    TZ_CHECK(grid > 0, TZ_EINVAL, "mxfp4 kernels need %d free SMs", kCG);
-    return launch_cluster(kern, kCG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma, mb, mo, msa, msb, p, ctx->d_status);
+    const int groups = (ctx->sm_count - ctx->sm_reserve) / CG;
+    const int grid = static_cast<int>(tiles < groups ? tiles : groups) * CG;
+    TZ_CHECK(grid > 0, TZ_EINVAL, "mxfp4 kernels need %d free SMs", CG);
+    return launch_cluster(kern, CG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma, mb, mo, msa, msb, p, ctx->d_status);
+}
+// Pairs of CTAs work on 256 rows; up to 128 rows leave half of such a tile empty, so where the tiles take more than
+// one round of pairs single CTAs take them (64 rows, D = 4096, 2 F = 16384: 14.8 us instead of 18.6).
+template <int OUT, bool GATED>
+int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, void* y, int act, cudaStream_t s) {
+    if (a.rows <= 128 && ceil_div(b.rows, MxCfg<1>::BN) > (ctx->sm_count - ctx->sm_reserve) / 2) return launch_mx_cg<1, OUT, GATED>(ctx, a, b, k, bias, y, act, s);
+    return launch_mx_cg<kCG, OUT, GATED>(ctx, a, b, k, bias, y, act, s);
 }
 
 // The few-rows kernel, where its K slice of x fits shared memory; *ran says whether it did.
@@ -896,8 +903,8 @@ int launch_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int rows, const Q4&
     const int tiles = ceil_div(w.rows, 128), kblocks = ceil_div(k, 256);
     *ran = false;
     if (tiles > 65535) return TZ_OK;  // the grid's second extent
-    // With room for 32 rows quantising x costs each CTA more than the tiles of 256 rows cost once there is more than
-    // one CTA per SM: 32 rows, D = 4096, 2 F = 32768 37.9 us here, 28.4 us there; one wave (2 F = 16384) 19.5, 20.2.
+    // With room for 32 rows quantising x costs each CTA more than the large kernel's tiles cost once there is more
+    // than one CTA per SM: 32 rows, D = 4096, 2 F = 32768 take 30.6 us here, 27.0 there; 2 F = 16384 16.0 and 19.5.
     if (N > 16 && tiles > ctx->sm_count) return TZ_OK;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::smem(C::MAX_KB), done);

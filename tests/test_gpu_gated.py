@@ -97,7 +97,7 @@ def check(ctx, x, wg, wu, dh, act):
 SIZES = [(1, 8, 8), (1, 384, 1536), (2, 64, 72), (3, 2048, 264), (7, 72, 2000), (8, 384, 1536), (9, 40, 8), (16, 1024, 520),
          (17, 136, 136), (31, 200, 96), (64, 384, 1000), (77, 384, 1000), (127, 128, 128), (128, 8, 264), (129, 64, 384),
          (256, 256, 512), (300, 1000, 328), (513, 520, 776), (1000, 384, 1536), (4099, 128, 264),
-         (5003, 384, 1544), (9000, 448, 520), (20000, 256, 264), (700, 768, 2048), (2100, 1160, 336)]
+         (5003, 384, 1544), (9000, 448, 520), (20000, 256, 264), (700, 768, 2048), (2100, 1160, 336), (100, 64, 9736)]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16"])

@@ -125,7 +125,7 @@ def near(got, want, tol, what=""):
 
 SIZES = [(1, 32, 8), (1, 4096, 1024), (2, 64, 16), (3, 96, 200), (5, 160, 136), (8, 2048, 512), (9, 224, 24), (16, 1024, 1000),
          (17, 288, 192), (31, 512, 384), (33, 320, 392), (64, 4096, 264), (65, 448, 200), (127, 128, 128), (128, 256, 576),
-         (129, 384, 1536), (257, 1536, 384), (300, 1056, 328), (1000, 384, 1536), (3000, 96, 72)]
+         (129, 384, 1536), (257, 1536, 384), (300, 1056, 328), (1000, 384, 1536), (3000, 96, 72), (70, 256, 15000)]
 
 
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
@@ -158,7 +158,7 @@ def test_linear_of_quantised_input_and_output_types(ctx, M):
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_erf", "relu", "sigmoid"])
-@pytest.mark.parametrize("T,D,F", [(1, 32, 16), (1, 2048, 512), (6, 160, 112), (16, 1024, 208), (33, 512, 48), (140, 96, 336), (520, 384, 1536)])
+@pytest.mark.parametrize("T,D,F", [(1, 32, 16), (1, 2048, 512), (6, 160, 112), (16, 1024, 208), (33, 512, 48), (140, 96, 336), (520, 384, 1536), (100, 160, 7520)])
 def test_gated(ctx, act, T, D, F):
     from test_gpu_gated import act64
     from tenzor_b200 import ops
@@ -268,3 +268,19 @@ def test_refusals(ctx):
     assert Lb.tz_linear_mxfp4(ctx.handle, p(x), 64, 3, p(w.codes), p(w.scales), None, p(y), 2, p(y), 16, 4, 64, 16, None) == _lib.TZ_EINVAL
     assert Lb.tz_quantize_mxfp4(None, p(x), 64, 2, p(w.codes), p(w.scales), 4, 64, None) == _lib.TZ_EINVAL
     assert Lb.tz_mxfp4_scale_bytes(-1, 64) == 0 and Lb.tz_mxfp4_scale_bytes(129, 160) == 2 * 2 * 512
+
+
+def test_example_trains_and_serves(ctx):
+    """The example's whole path: training with the 16-bit kernels, serving with the 4-bit ones."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "gated_block.py")
+    spec = importlib.util.spec_from_file_location("gated_block", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    losses, cos, same = ex.main(["--dim", "128", "--ffn", "256", "--tokens", "1024", "--steps", "40"])
+    assert losses[-1] < 0.5 * losses[0]
+    # Each 4-bit operand is off by up to a quarter of its value (E2M1 keeps one fraction bit), 0.1 rms; four of them
+    # (x, the two weights, h and Wd in turn) leave an angle of about 0.2 to 0.25.
+    assert float(cos.mean()) > 0.95
+    assert same <= 2.0 ** -6  # the kernels of one token and of a batch round h to 16 bits, then to 4, from other sums
