@@ -4,14 +4,16 @@
 //   backward   dg = dh * u * act'(g),  du = dh * act(g)                   g and u are computed again
 //              dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
 //
-// One persistent kernel template with four forms (what differs is the operands' layout and the epilogue):
+// One persistent kernel template with three forms (what differs is the operands' layout and the epilogue):
 //   FWD  both projections of a tile in one accumulator: its B tile is BN/2 rows of Wg over BN/2 rows of Wu, so
 //        one MMA makes the gate and the up columns of the same outputs; the epilogue multiplies them
 //   BWD  the same products; the epilogue makes dg and du (16 bits) from them and dh, all in f32 before the
 //        one rounding that the tensor core needs for the next products' operands
-//   DX   [dg | du] [Wg ; Wu]: one accumulation over both halves; the weights are read MN-major in place
-//   DW   dg^T x and du^T x: both operands MN-major in place (the sum runs over tokens); where the tiles do not
-//        fill the GPU the tokens are split and the f32 partial sums added in a fixed order by a second kernel
+//   GRAD dx and both weights' gradients in one launch (the two kinds of tiles fill each other's last round):
+//        dx = [dg | du] [Wg ; Wu] is one accumulation over both halves, the weights read MN-major in place;
+//        dWg = dg^T x and dWu = du^T x read both operands MN-major in place (the sum runs over tokens).
+//        Where the tiles do not fill the GPU their sums are split and the f32 partial sums added in a fixed
+//        order by a second kernel
 //
 // Per CTA (64 + 32 * EPI warps): warp 0 TMA producer, warp 1 allocates TMEM and issues the MMAs, the others
 // read the accumulators (two buffers: the epilogue of a tile runs under the next tile's MMAs) and store boxes
@@ -30,27 +32,37 @@
 namespace tz {
 namespace {
 
-enum { MM_FWD = 0, MM_BWD = 1, MM_DX = 2, MM_DW = 3 };
+enum { MM_FWD = 0, MM_BWD = 1, MM_GRAD = 2 };
+
+// One product's tiles: m_tiles row blocks of 128 * CG x n_tiles column blocks (FWD / BWD: of BN / 2 outputs).
+struct Grid {
+    int m_tiles, n_tiles;
+    int which;    // products of this shape: 2 for dWg and dWu, else 1
+    int splits;   // of the K blocks; > 1: f32 partial sums
+    int kblocks;  // K blocks of 64
+    int kper;     // K blocks per split
+    int m_pad;    // rows of one partial sum
+};
 
 struct MmParams {
-    int m_tiles, n_tiles;  // tiles of 128 * CG rows x BN columns (FWD / BWD: BN / 2 output columns)
-    int which;             // DW: 2 (dWg and dWu), else 1
-    int splits;            // of the K blocks; > 1: f32 partial sums
-    int kblocks;           // K blocks of 64, both halves for DX
-    int half;              // DX: K blocks of one half
-    int kper;              // K blocks per split
-    int ring;              // shared-memory stages in use
-    int resident;          // dual forms: the column block's B tiles stay in shared memory (see launch_mm)
-    int m_pad;             // rows of one partial sum
-    int cols;              // of the output
+    Grid g[2];    // GRAD: dx, then the weights' gradients; else g[0] alone
+    int ring;     // shared-memory stages in use
+    int resident; // dual forms: the column block's B tiles stay in shared memory (see launch_mm)
+    int half;     // GRAD: K blocks of one half of dx's sum
+    int cols;     // of the output
     int act;
+};
+
+// Tensor maps: A (FWD / BWD: x; GRAD: dg and du as dx's operand, then as the weights' gradients'), B (Wg and Wu; GRAD:
+// x too), the outputs (h; dg and du; dx, dWg and dWu or their partial sums), and dh.
+struct MmMaps {
+    CUtensorMap a[4], b[3], o[3], dh;
 };
 
 template <int CG, int BN, int MODE>
 struct MmCfg {
     static constexpr bool kDual = MODE == MM_FWD || MODE == MM_BWD;
-    static constexpr bool kAmn = MODE == MM_DW;
-    static constexpr bool kBmn = MODE == MM_DX || MODE == MM_DW;
+    static constexpr bool kBmn = MODE == MM_GRAD;
     static constexpr int EPI = kDual ? 16 : 8;
     static constexpr int THREADS = 64 + 32 * EPI;
     static constexpr int BNC = BN / CG;  // B rows (or columns) in one CTA
@@ -112,12 +124,9 @@ __device__ __forceinline__ void stage128(uint32_t buf, int lane, const uint32_t 
         tzp::st_shared_v4(buf + lane * 128 + ((c ^ (lane & 7)) << 4), v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
 }
 
-template <int CG, int BN, int MODE, bool BF, bool PART>
+template <int CG, int BN, int MODE, bool BF>
 __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
-    gated_mm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
-                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
-                    const __grid_constant__ CUtensorMap tmO0, const __grid_constant__ CUtensorMap tmO1,
-                    const __grid_constant__ CUtensorMap tmDh, const MmParams p, int* status) {
+    gated_mm_kernel(const __grid_constant__ MmMaps tm, const __grid_constant__ MmParams p, int* status) {
     using C = MmCfg<CG, BN, MODE>;
     constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -150,8 +159,8 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         for (int e = 0; e < C::EPI; ++e) tzp::mbar_init(&dhbar[e], 1);
         *abort_flag = 0;
         tzp::fence_mbar_init();
-        tzp::tma_prefetch_desc(&tmA0);
-        tzp::tma_prefetch_desc(&tmB0);
+        tzp::tma_prefetch_desc(&tm.a[0]);
+        tzp::tma_prefetch_desc(&tm.b[0]);
     }
     if (warp == 1) tzp::pair_tmem_alloc<CG>(tmem_slot, C::TCOLS);
     tzp::tc_fence_before();
@@ -165,47 +174,57 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     // before the next group starts, so that the CTAs running at one time share both operands in L2.  With
     // resident B tiles: a contiguous range of the tiles in column-block order, so that the column block changes
     // rarely.
-    const int per = p.m_tiles * p.n_tiles;
-    const int num_tiles = per * p.which * p.splits;
+    const int tiles0 = p.g[0].m_tiles * p.g[0].n_tiles * p.g[0].which * p.g[0].splits;
+    const int num_tiles = tiles0 + (MODE == MM_GRAD ? p.g[1].m_tiles * p.g[1].n_tiles * p.g[1].which * p.g[1].splits : 0);
     struct Tile {
-        int m, n, w, s, kb0, kb1;
+        int dw, m, n, w, s, kb0, kb1;  // dw: a weights' gradient tile
     };
     const int me = static_cast<int>(blockIdx.x) / CG, team = static_cast<int>(gridDim.x) / CG;
     const int first = p.resident ? static_cast<int>(static_cast<long long>(num_tiles) * me / team) : 0;
     const int last = p.resident ? static_cast<int>(static_cast<long long>(num_tiles) * (me + 1) / team) : 0;
     auto tile_at = [&](int i, Tile& r) -> bool {
+        r.dw = 0;
         if (C::kDual && p.resident) {
             const int t = first + i;
-            r.n = t / p.m_tiles;
-            r.m = t - r.n * p.m_tiles;
+            r.n = t / p.g[0].m_tiles;
+            r.m = t - r.n * p.g[0].m_tiles;
             r.w = r.s = r.kb0 = 0;
-            r.kb1 = p.kblocks;
+            r.kb1 = p.g[0].kblocks;
             return t < last;
         }
         int t = me + i * team;
         if (t >= num_tiles) return false;
-        r.s = t / (per * p.which);
-        t -= r.s * per * p.which;
+        if (MODE == MM_GRAD && t >= tiles0) {
+            r.dw = 1;
+            t -= tiles0;
+        }
+        const Grid& g = p.g[MODE == MM_GRAD ? r.dw : 0];
+        const int per = g.m_tiles * g.n_tiles;
+        r.s = t / (per * g.which);
+        t -= r.s * per * g.which;
         r.w = t / per;
         t -= r.w * per;
         constexpr int GM = 8;
-        const int grp = t / (GM * p.n_tiles);
-        const int gm = min(GM, p.m_tiles - grp * GM);
-        t -= grp * GM * p.n_tiles;
+        const int grp = t / (GM * g.n_tiles);
+        const int gm = min(GM, g.m_tiles - grp * GM);
+        t -= grp * GM * g.n_tiles;
         r.m = grp * GM + t % gm;
         r.n = t / gm;
-        r.kb0 = r.s * p.kper;
-        r.kb1 = min(p.kblocks, r.kb0 + p.kper);
+        r.kb0 = r.s * g.kper;
+        r.kb1 = min(g.kblocks, r.kb0 + g.kper);
         return true;
     };
-    auto range_at = [&](int i, int& kb0, int& kb1) -> bool {  // tile_at's K blocks alone, without its divisions
-        const int t = C::kDual && p.resident ? first + i : me + i * team;
-        kb0 = 0, kb1 = p.kblocks;
-        if (p.splits > 1 && t < num_tiles) {
-            kb0 = t / (per * p.which) * p.kper;
-            kb1 = min(p.kblocks, kb0 + p.kper);
+    auto range_at = [&](int i, int& kb0, int& kb1, int& dw) -> bool {  // of tile_at, what the MMA issuer needs
+        int t = C::kDual && p.resident ? first + i : me + i * team;
+        if (t >= (C::kDual && p.resident ? last : num_tiles)) return false;
+        dw = MODE == MM_GRAD && t >= tiles0;
+        const Grid& g = p.g[MODE == MM_GRAD ? dw : 0];
+        kb0 = 0, kb1 = g.kblocks;
+        if (g.splits > 1) {
+            kb0 = (dw ? t - tiles0 : t) / (g.m_tiles * g.n_tiles * g.which) * g.kper;
+            kb1 = min(g.kblocks, kb0 + g.kper);
         }
-        return t < (C::kDual && p.resident ? last : num_tiles);
+        return true;
     };
     const int ring = p.ring;
     // Shared memory: stage s holds an A tile and a B tile; with resident B tiles a ring of A tiles comes first,
@@ -253,28 +272,30 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                     const uint32_t sb = b_addr(stage, kb);
                     if (issue) {
                         if (rank == 0) tzp::mbar_arrive_expect_tx(&full[stage], bytes);
-                        if constexpr (MODE == MM_DW) {
-                            const CUtensorMap* ta = q.w ? &tmA1 : &tmA0;
-                            tzp::pair_load_2d<CG>(sa, ta, m0, kb * 64, bar);
-                            tzp::pair_load_2d<CG>(sa + 8192, ta, m0 + 64, kb * 64, bar);
+                        if constexpr (MODE == MM_GRAD) {
+                            const CUtensorMap* tb;
+                            int k = kb * 64;
+                            if (q.dw) {
+                                const CUtensorMap* ta = &tm.a[2 + q.w];
+                                tzp::pair_load_2d<CG>(sa, ta, m0, k, bar);
+                                tzp::pair_load_2d<CG>(sa + 8192, ta, m0 + 64, k, bar);
+                                tb = &tm.b[2];
+                            } else {
+                                const bool up = kb >= p.half;
+                                if (up) k -= p.half * 64;
+                                tzp::pair_load_2d<CG>(sa, &tm.a[up], k, m0, bar);
+                                tb = &tm.b[up];
+                            }
 #pragma unroll
-                            for (int j = 0; j < C::BNC / 64; ++j)
-                                tzp::pair_load_2d<CG>(sb + j * 8192, &tmB0, b_col(q.n, j), kb * 64, bar);
-                        } else if constexpr (MODE == MM_DX) {
-                            const bool up = kb >= p.half;
-                            const int k = (up ? kb - p.half : kb) * 64;
-                            tzp::pair_load_2d<CG>(sa, up ? &tmA1 : &tmA0, k, m0, bar);
-#pragma unroll
-                            for (int j = 0; j < C::BNC / 64; ++j)
-                                tzp::pair_load_2d<CG>(sb + j * 8192, up ? &tmB1 : &tmB0, b_col(q.n, j), k, bar);
+                            for (int j = 0; j < C::BNC / 64; ++j) tzp::pair_load_2d<CG>(sb + j * 8192, tb, b_col(q.n, j), k, bar);
                         } else {
-                            tzp::pair_load_2d<CG>(sa, &tmA0, kb * 64, m0, bar);
+                            tzp::pair_load_2d<CG>(sa, &tm.a[0], kb * 64, m0, bar);
                             if (!need_b) {
                             } else if constexpr (CG == 2) {
-                                tzp::pair_load_2d<CG>(sb, rank ? &tmB1 : &tmB0, kb * 64, q.n * (BN / 2), bar);
+                                tzp::pair_load_2d<CG>(sb, &tm.b[rank], kb * 64, q.n * (BN / 2), bar);
                             } else {
-                                tzp::pair_load_2d<CG>(sb, &tmB0, kb * 64, q.n * (BN / 2), bar);
-                                tzp::pair_load_2d<CG>(sb + (BN / 2) * 128, &tmB1, kb * 64, q.n * (BN / 2), bar);
+                                tzp::pair_load_2d<CG>(sb, &tm.b[0], kb * 64, q.n * (BN / 2), bar);
+                                tzp::pair_load_2d<CG>(sb + (BN / 2) * 128, &tm.b[1], kb * 64, q.n * (BN / 2), bar);
                             }
                         }
                     }
@@ -293,15 +314,17 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         if (rank == 0) {
             // ---- MMA issuer (the whole warp; one lane issues) ----
             const bool issue = tzp::elect_one();
-            constexpr uint32_t major = (C::kAmn ? 1u << 15 : 0u) | (C::kBmn ? 1u << 16 : 0u);
-            constexpr uint32_t idesc = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 256) | major;
-            constexpr uint32_t idesc_b = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 128) | major;  // columns 256 .. 383
-            constexpr uint32_t kAstep = C::kAmn ? 2048u >> 4 : 2u, kBstep = C::kBmn ? 2048u >> 4 : 2u;
+            constexpr uint32_t idesc0 = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 256) | (C::kBmn ? 1u << 16 : 0u);
+            constexpr uint32_t idesc0_b = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 128) | (C::kBmn ? 1u << 16 : 0u);  // columns 256 .. 383
+            constexpr uint32_t kBstep = C::kBmn ? 2048u >> 4 : 2u;
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
-            int kb0, kb1;
-            for (int i = 0; ok && range_at(i, kb0, kb1); ++i) {
+            int kb0, kb1, dw;
+            for (int i = 0; ok && range_at(i, kb0, kb1, dw); ++i) {
+                const bool amn = MODE == MM_GRAD && dw;  // A is MN-major
+                const uint32_t idesc = idesc0 | (amn ? 1u << 15 : 0u), idesc_b = idesc0_b | (amn ? 1u << 15 : 0u);
+                const uint32_t a_k = amn ? 2048u >> 4 : 2u;
                 if (!tzp::warp_wait(&tempty[acc], acc_phase ^ 1u, status, abort_flag)) break;
                 tzp::tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
@@ -313,15 +336,15 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                     tzp::tc_fence_after();
                     const uint32_t sa = sbase + stage * a_step;
                     const uint32_t sb = b_addr(stage, kb);
-                    const uint64_t ad = C::kAmn ? tzp::sdesc_mn128(sa, 8192) : tzp::sdesc_k128(sa);
+                    const uint64_t ad = amn ? tzp::sdesc_mn128(sa, 8192) : tzp::sdesc_k128(sa);
                     const uint64_t bd = C::kBmn ? tzp::sdesc_mn128(sb, 8192) : tzp::sdesc_k128(sb);
                     if (issue) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uint32_t more = (kb > kb0 || k > 0) ? 1u : 0u;
-                            tzp::pair_mma_f16<CG>(d, ad + kAstep * k, bd + kBstep * k, idesc, more);
+                            tzp::pair_mma_f16<CG>(d, ad + a_k * k, bd + kBstep * k, idesc, more);
                             if constexpr (BN == 384)
-                                tzp::pair_mma_f16<CG>(d + 256, ad + kAstep * k, bd + (16384u >> 4) + kBstep * k, idesc_b, more);
+                                tzp::pair_mma_f16<CG>(d + 256, ad + a_k * k, bd + (16384u >> 4) + kBstep * k, idesc_b, more);
                         }
                         tzp::pair_commit<CG>(&empty[stage]);
                     }
@@ -356,7 +379,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         // is in registers the next tile's is asked for.  dg and du take turns in the second half.
         auto fetch_dh = [&](const Tile& q) {
             tzp::mbar_arrive_expect_tx(&dhbar[e], 2048);
-            tzp::tma_load_2d(boxp, &tmDh, q.n * (BN / 2) + sl * 32, (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32, &dhbar[e]);
+            tzp::tma_load_2d(boxp, &tm.dh, q.n * (BN / 2) + sl * 32, (q.m * CG + static_cast<int>(rank)) * 128 + q4 * 32, &dhbar[e]);
         };
         Tile q, next;
         bool more = tile_at(0, next), fetched = false;
@@ -425,12 +448,12 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                 const bool store = lane == 0 && col0 < p.cols;
                 if constexpr (MODE == MM_FWD) {
                     if (store) {
-                        tzp::tma_store_2d(&tmO0, boxp, col0, row0);
+                        tzp::tma_store_2d(&tm.o[0], boxp, col0, row0);
                         tzp::bulk_commit();
                     }
                 } else {
                     if (store) {
-                        tzp::tma_store_2d(&tmO1, boxp + 2048, col0, row0);
+                        tzp::tma_store_2d(&tm.o[1], boxp + 2048, col0, row0);
                         tzp::bulk_commit();
                         tzp::bulk_wait_read<0>();
                     }
@@ -439,12 +462,15 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                     tzp::fence_proxy_async();
                     __syncwarp();
                     if (store) {
-                        tzp::tma_store_2d(&tmO0, boxp + 2048, col0, row0);
+                        tzp::tma_store_2d(&tm.o[0], boxp + 2048, col0, row0);
                         tzp::bulk_commit();
                     }
                 }
             } else {
                 constexpr int CH = BN / 64;
+                const Grid& g = p.g[q.dw];
+                const CUtensorMap* to = &tm.o[g.splits > 1 ? q.dw : q.dw ? 1 + q.w : 0];
+                if (lane == 0) tzp::bulk_wait_read<0>();  // the two kinds of tiles use the staging differently
 #pragma unroll 1
                 for (int c = 0; c < CH; ++c) {
                     const int cc = (sl * CH + c) * 32;
@@ -453,14 +479,14 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                     uint32_t v[32];
                     tzp::tmem_ld32(td + cc, v);
                     tzp::tmem_ld_wait();
-                    if constexpr (PART) {
+                    if (g.splits > 1) {
                         if (lane == 0) tzp::bulk_wait_read<0>();
                         __syncwarp();
                         stage128(box, lane, v);
                         tzp::fence_proxy_async();
                         __syncwarp();
                         if (lane == 0) {
-                            tzp::tma_store_2d(&tmO0, boxp, col0, (q.s * p.which + q.w) * p.m_pad + row0);
+                            tzp::tma_store_2d(to, boxp, col0, (q.s * g.which + q.w) * g.m_pad + row0);
                             tzp::bulk_commit();
                         }
                     } else {
@@ -473,7 +499,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
                         tzp::fence_proxy_async();
                         __syncwarp();
                         if (lane == 0) {
-                            tzp::tma_store_2d(q.w ? &tmO1 : &tmO0, boxp + nb * 2048, col0, row0);
+                            tzp::tma_store_2d(to, boxp + nb * 2048, col0, row0);
                             tzp::bulk_commit();
                         }
                         nb ^= 1;
@@ -518,22 +544,29 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
     }
 }
 
-// Sums the partial products [splits][which][m_pad][cols] in order and rounds to 16 bits.
+// Sums partial products [splits][which][m_pad][cols] in order and rounds to 16 bits: up to two jobs of one width.
+struct SumJob {
+    const float* part;
+    void* out[2];
+    int which, splits, m_pad, rows;
+};
 template <bool BF>
-__global__ void sum_parts_kernel(const float* part, void* out0, void* out1, int which, int splits, int m_pad, int rows, int cols) {
-    const long long n8 = static_cast<long long>(rows) * cols / 8;
-    const long long plane = static_cast<long long>(m_pad) * cols;
-    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n8 * which; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const int w = i >= n8;
-        const long long o = (i - (w ? n8 : 0)) * 8;
+__global__ void __launch_bounds__(256) sum_parts_kernel(const __grid_constant__ SumJob j0, const __grid_constant__ SumJob j1, int cols) {
+    const long long n0 = static_cast<long long>(j0.rows) * cols / 8, n1 = static_cast<long long>(j1.rows) * cols / 8;
+    const long long t0 = n0 * j0.which, total = t0 + n1 * j1.which;
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const SumJob& j = i < t0 ? j0 : j1;
+        const long long n8 = i < t0 ? n0 : n1, at = i < t0 ? i : i - t0;
+        const int w = at >= n8;
+        const long long o = (at - (w ? n8 : 0)) * 8, plane = static_cast<long long>(j.m_pad) * cols;
         float s[8] = {};
-        for (int k = 0; k < splits; ++k) {
-            const float4* src = reinterpret_cast<const float4*>(part + (static_cast<long long>(k) * which + w) * plane + o);
+        for (int k = 0; k < j.splits; ++k) {
+            const float4* src = reinterpret_cast<const float4*>(j.part + (static_cast<long long>(k) * j.which + w) * plane + o);
             const float4 a = __ldcs(src), b = __ldcs(src + 1);
             s[0] += a.x, s[1] += a.y, s[2] += a.z, s[3] += a.w, s[4] += b.x, s[5] += b.y, s[6] += b.z, s[7] += b.w;
         }
-        uint4 r = make_uint4(tzp::pack16x2<BF>(s[0], s[1]), tzp::pack16x2<BF>(s[2], s[3]), tzp::pack16x2<BF>(s[4], s[5]), tzp::pack16x2<BF>(s[6], s[7]));
-        reinterpret_cast<uint4*>(w ? out1 : out0)[o / 8] = r;
+        reinterpret_cast<uint4*>(j.out[w])[o / 8] = make_uint4(tzp::pack16x2<BF>(s[0], s[1]), tzp::pack16x2<BF>(s[2], s[3]),
+                                                             tzp::pack16x2<BF>(s[4], s[5]), tzp::pack16x2<BF>(s[6], s[7]));
     }
 }
 
@@ -549,120 +582,118 @@ int map16(CUtensorMap* m, const Mat& a, int box_cols, int box_rows, CUtensorMapS
                               a.ld * 2, box_cols, box_rows, swz);
 }
 
-template <int CG, int BN, int MODE, bool BF, bool PART>
-int launch_mm(tz_ctx_t ctx, const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, const Mat& o0, const Mat& o1, const Mat* dh,
-              MmParams p, float* part, cudaStream_t s) {
+template <int CG, int BN, int MODE, bool BF>
+int launch_mm(tz_ctx_t ctx, const MmMaps& tm, MmParams p, cudaStream_t s) {
     using C = MmCfg<CG, BN, MODE>;
-    auto kern = gated_mm_kernel<CG, BN, MODE, BF, PART>;
+    auto kern = gated_mm_kernel<CG, BN, MODE, BF>;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::SMEM, done);
     if (rc) return rc;
-    CUtensorMap ma0, ma1, mb0, mb1, mo0, mo1, mdh;
-    const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B;
-    const int arows = C::kAmn ? 64 : 128, brows = C::kBmn ? 64 : (C::kDual ? BN / 2 : C::BNC);
-    if ((rc = map16<BF>(&ma0, a0, 64, arows, S128)) || (rc = map16<BF>(&mb0, b0, 64, brows, S128))) return rc;
-    ma1 = ma0, mb1 = mb0;  // an encoding costs about as much as the rest of the launch's arguments
-    if (a1.p != a0.p && (rc = map16<BF>(&ma1, a1, 64, arows, S128))) return rc;
-    if (b1.p != b0.p && (rc = map16<BF>(&mb1, b1, 64, brows, S128))) return rc;
-    if (PART) {
-        rc = encode_tmap_2d_swz(&mo0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, o0.cols,
-                                static_cast<uint64_t>(p.splits) * p.which * p.m_pad, o0.cols * 4, 32, 32, S128);
-        mo1 = mo0;
-    } else {
-        rc = map16<BF>(&mo0, o0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
-        mo1 = mo0;
-        if (!rc && o1.p != o0.p) rc = map16<BF>(&mo1, o1, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
-    }
-    if (rc) return rc;
-    mdh = mo0;
-    if (dh && (rc = map16<BF>(&mdh, *dh, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
-    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * p.which * p.splits;
+    auto count = [](const Grid& g) { return static_cast<long long>(g.m_tiles) * g.n_tiles * g.which * g.splits; };
+    const long long tiles = count(p.g[0]) + (MODE == MM_GRAD ? count(p.g[1]) : 0);
     const int groups = (ctx->sm_count - ctx->sm_reserve) / CG;
     const int grid = static_cast<int>(tiles < groups ? tiles : groups) * CG;
     TZ_CHECK(grid > 0, TZ_EINVAL, "gated kernels need %d free SMs", CG);
     p.ring = C::STAGES;
-    if (C::kDual && tiles > groups && p.kblocks >= 4) {
+    const int kb = p.g[0].kblocks;
+    if (C::kDual && tiles > groups && kb >= 4) {
         // Short sums: the B tiles of a whole column block fit beside a ring of A tiles, and keeping them halves what
         // an SM moves from L2 per tile, which bounds these shapes.  Below 4 K blocks the ring (at most kblocks long)
         // would be too short; above, it has to keep 3 A tiles.
-        const int left = (C::BUDGET - p.kblocks * C::BNC * 128) / C::A_BYTES;
-        int r = left < p.kblocks ? left : p.kblocks;
+        const int left = (C::BUDGET - kb * C::BNC * 128) / C::A_BYTES;
+        int r = left < kb ? left : kb;
         if (r > C::STAGES) r = C::STAGES;
         if (r >= 3) {
             p.resident = 1;
             p.ring = r;
         }
     }
-    return launch_cluster(kern, CG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, ma0, ma1, mb0, mb1, mo0, mo1, mdh, p, ctx->d_status);
+    return launch_cluster(kern, CG, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, tm, p, ctx->d_status);
 }
 
 constexpr int kCG = 2, kBN = 256;
-// Tokens up to which the forward pass streams weights (gated_rows_kernel).  At 32 tokens it takes 5.2 / 10.2 /
-// 14.5 / 26.8 us at (D, F) = (384, 1536) / (1024, 4096) / (2048, 6144) / (4096, 8192), the tiles of 256 tokens 6.5
-// / 10.4 / 16.1 / 29.2; with room for 64 tokens it takes 6.5 / 14.2 / 16.9 / 29.1.
+// Tokens up to which the forward pass streams weights (gated_rows_kernel).  At 32 tokens it takes 4.7 / 10.0 /
+// 14.2 / 26.5 us at (D, F) = (384, 1536) / (1024, 4096) / (2048, 6144) / (4096, 8192), the tiles of 256 tokens 6.3
+// / 10.3 / 16.3 / 28.5; with room for 64 tokens it took 6.5 / 14.2 / 16.9 / 29.1.
 constexpr int kRowsMax = 32;
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+size_t a256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
-// Tile width and splits of the sum of a DX or DW product, by an estimate in clocks: rounds of tiles over the
-// pairs, each K block at the rate the operands arrive at (256 columns: 32 KB per SM, 384: 40 KB), a start and an
-// epilogue per round (not hidden with one accumulator), and the partial sums' way out and back.
-struct Split {
-    int bn, splits;
+// How the gradients' launch is cut: tile width, splits of dx's and the weights' sums, and the workspace's parts.
+struct BwdPlan {
+    int bn, s_dx, s_dw;
+    size_t dgdu, part_dx, part_dw;  // bytes
 };
-Split pick_split(int sms, int64_t m_tiles, int which, int64_t rows, int64_t cols, int kblocks) {
+
+// By an estimate in clocks: every tile's K blocks at the rate its operands arrive at (256 columns: 32 KB per SM and
+// K block, 384: 40 KB), an epilogue per tile (with one accumulator, 384 columns, not hidden), the tiles dealt round
+// the pairs, and the partial sums' way out and back.  384 columns cover D = 384 in one tile: 18106 tokens, F = 1536
+// took 166 us with 256 columns and 148 us with 384.
+BwdPlan make_plan(int sms, int64_t T, int64_t D, int64_t F) {
     const int64_t groups = sms / kCG > 0 ? sms / kCG : 1;
-    Split best{256, 1};
-    if (kblocks < 1) return best;  // no tokens
+    const int64_t mt = ceil_div(T, 128 * kCG), ft = ceil_div(F, 128 * kCG);
+    const int kx = 2 * ceil_div(F, 64), kw = ceil_div(T, 64);
+    auto splits_ok = [](int kb, int s) { return s == 1 || (kb / s >= 8 && ceil_div(kb, ceil_div(kb, s)) == s); };
+    BwdPlan best{};
     double best_cost = 1e300;
     for (int bn = 256; bn <= 384; bn += 128) {
-        const int64_t tiles = m_tiles * which * ceil_div(cols, bn);
-        for (int sp = 1; sp <= 16; ++sp) {
-            if (sp > 1 && (kblocks / sp < 8 || tiles * sp > groups)) break;
-            const int per = ceil_div(kblocks, sp);
-            if (ceil_div(kblocks, per) != sp) continue;  // every split has work
-            double cost = static_cast<double>(ceil_div(tiles * sp, groups)) * (bn == 256 ? per * 600.0 + 2500.0 : per * 820.0 + 5000.0);
-            if (sp > 1) cost += 6000.0 + static_cast<double>(sp) * which * rows * cols * 8.0 / 2500.0;
-            if (cost < best_cost) {
-                best_cost = cost;
-                best = {bn, sp};
+        const int64_t nt = ceil_div(D, bn);
+        const double rate = bn == 256 ? 600.0 : 820.0, epi = bn == 256 ? 800.0 : 5000.0;
+        for (int sx = 1; sx <= 16; ++sx) {
+            const int64_t nx = mt * nt * sx;
+            if (!splits_ok(kx, sx) || (sx > 1 && nx > groups)) continue;
+            for (int sw = 1; sw <= 16; ++sw) {
+                const int64_t nw = 2 * ft * nt * sw;
+                if (!splits_ok(kw, sw) || (sw > 1 && nw > groups)) continue;
+                const double cx = ceil_div(kx, sx) * rate + epi, cw = ceil_div(kw, sw) * rate + epi;
+                double cost = 0;  // of the slowest pair: pair g has the tiles g, g + groups, ..., dx's first
+                const int64_t first[3] = {0, nx % groups, (nx + nw) % groups};  // where the counts step down
+                for (int64_t g : first) {
+                    const int64_t a = nx > g ? (nx - g - 1) / groups + 1 : 0;
+                    const int64_t both = nx + nw > g ? (nx + nw - g - 1) / groups + 1 : 0;
+                    const double c = a * cx + (both - a) * cw;
+                    if (c > cost) cost = c;
+                }
+                cost += 3000.0;
+                if (sx > 1 || sw > 1)
+                    cost += 6000.0 + 8.0 * D * ((sx > 1 ? static_cast<double>(sx) * T : 0.0) + (sw > 1 ? 2.0 * sw * F : 0.0)) / 2500.0;
+                if (cost < best_cost) {
+                    best_cost = cost;
+                    best.bn = bn, best.s_dx = sx, best.s_dw = sw;
+                }
             }
         }
     }
+    best.dgdu = a256(static_cast<size_t>(T) * F * 2);
+    if (best.s_dx > 1) best.part_dx = a256(static_cast<size_t>(best.s_dx) * mt * 128 * kCG * D * 4);
+    if (best.s_dw > 1) best.part_dw = a256(static_cast<size_t>(best.s_dw) * 2 * ft * 128 * kCG * D * 4);
     return best;
 }
-
-struct BwdPlan {
-    size_t dgdu, part_dx, part_dw;  // bytes
-    Split dx, dw;
-};
+// The last sizes' plan of this thread: a training step asks for the same one again and again.
 BwdPlan plan_bwd(int sms, int64_t T, int64_t D, int64_t F) {
-    BwdPlan b{};
-    auto a256 = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
-    b.dgdu = a256(static_cast<size_t>(T) * F * 2);
-    const int mt = ceil_div(T, 128 * kCG), ft = ceil_div(F, 128 * kCG);
-    b.dx = pick_split(sms, mt, 1, T, D, 2 * ceil_div(F, 64));
-    b.dw = pick_split(sms, ft, 2, F, D, ceil_div(T, 64));
-    if (b.dx.splits > 1) b.part_dx = a256(static_cast<size_t>(b.dx.splits) * mt * 128 * kCG * D * 4);
-    if (b.dw.splits > 1) b.part_dw = a256(static_cast<size_t>(b.dw.splits) * 2 * ft * 128 * kCG * D * 4);
-    return b;
+    struct Last {
+        int sms = 0;
+        int64_t T = 0, D = 0, F = 0;
+        BwdPlan plan{};
+    };
+    static thread_local Last last;
+    if (last.sms != sms || last.T != T || last.D != D || last.F != F) {
+        last.plan = make_plan(sms, T, D, F);
+        last.sms = sms, last.T = T, last.D = D, last.F = F;
+    }
+    return last.plan;
 }
 
+// Maps of the dual products: x, Wg and Wu.
 template <bool BF>
-int sum_parts(tz_ctx_t ctx, const float* part, void* o0, void* o1, int which, int splits, int m_pad, int rows, int cols, cudaStream_t s) {
-    const long long n8 = static_cast<long long>(rows) * cols / 8 * which;
-    const int blocks = static_cast<int>(n8 / 256 + 1 < ctx->sm_count * 8 ? n8 / 256 + 1 : ctx->sm_count * 8);
-    return launch_kernel(sum_parts_kernel<BF>, dim3(blocks), dim3(256), 0, s, false, part, o0, o1, which, splits, m_pad, rows, cols);
-}
-
-template <int MODE, bool BF>
-int launch_any(tz_ctx_t ctx, const Split& w, const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, const Mat& o0, const Mat& o1,
-               const MmParams& p, float* part, cudaStream_t s) {
-    if (w.bn == 384)
-        return p.splits > 1 ? launch_mm<kCG, 384, MODE, BF, true>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, part, s)
-                            : launch_mm<kCG, 384, MODE, BF, false>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, nullptr, s);
-    return p.splits > 1 ? launch_mm<kCG, kBN, MODE, BF, true>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, part, s)
-                        : launch_mm<kCG, kBN, MODE, BF, false>(ctx, a0, a1, b0, b1, o0, o1, nullptr, p, nullptr, s);
+int dual_maps(MmMaps* tm, const Mat& x, const Mat& wg, const Mat& wu, const Mat& o0, const Mat& o1) {
+    const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B, S64 = CU_TENSOR_MAP_SWIZZLE_64B;
+    int rc;
+    if ((rc = map16<BF>(&tm->a[0], x, 64, 128, S128)) || (rc = map16<BF>(&tm->b[0], wg, 64, kBN / 2, S128)) ||
+        (rc = map16<BF>(&tm->b[1], wu, 64, kBN / 2, S128)) || (rc = map16<BF>(&tm->o[0], o0, 32, 32, S64)))
+        return rc;
+    return o1.p ? map16<BF>(&tm->o[1], o1, 32, 32, S64) : TZ_OK;
 }
 
 template <int N, bool BF>
@@ -694,16 +725,17 @@ int forward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat&
         if (x.rows <= 16) return launch_rows<16, BF>(ctx, x, wg, wu, h, act, s);
         return launch_rows<32, BF>(ctx, x, wg, wu, h, act, s);
     }
+    MmMaps tm{};
+    int rc = dual_maps<BF>(&tm, x, wg, wu, h, Mat{});
+    if (rc) return rc;
     MmParams p{};
-    p.m_tiles = ceil_div(x.rows, 128 * kCG);
-    p.n_tiles = ceil_div(h.cols, kBN / 2);
-    p.which = p.splits = 1;
-    p.kblocks = p.kper = ceil_div(x.cols, 64);
+    const int kb = ceil_div(x.cols, 64);
+    p.g[0] = {ceil_div(x.rows, 128 * kCG), ceil_div(h.cols, kBN / 2), 1, 1, kb, kb, 0};
     p.cols = static_cast<int>(h.cols);
     p.act = act;
-    if (x.rows <= 128 && p.n_tiles > (ctx->sm_count - ctx->sm_reserve) / 2)  // half of a pair's rows would be empty
-        return launch_mm<1, kBN, MM_FWD, BF, false>(ctx, x, x, wg, wu, h, h, nullptr, p, nullptr, s);
-    return launch_mm<kCG, kBN, MM_FWD, BF, false>(ctx, x, x, wg, wu, h, h, nullptr, p, nullptr, s);
+    if (x.rows <= 128 && p.g[0].n_tiles > (ctx->sm_count - ctx->sm_reserve) / 2)  // half of a pair's rows would be empty
+        return launch_mm<1, kBN, MM_FWD, BF>(ctx, tm, p, s);
+    return launch_mm<kCG, kBN, MM_FWD, BF>(ctx, tm, p, s);
 }
 
 template <bool BF>
@@ -714,44 +746,50 @@ int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat
     const Mat dg{ws, T, F, F}, du{ws + b.dgdu, T, F, F};
     float* part_dx = reinterpret_cast<float*>(ws + 2 * b.dgdu);
     float* part_dw = reinterpret_cast<float*>(ws + 2 * b.dgdu + b.part_dx);
+    const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B, S64 = CU_TENSOR_MAP_SWIZZLE_64B;
+
+    MmMaps tm{};
+    int rc = dual_maps<BF>(&tm, x, wg, wu, dg, du);
+    if (rc || (rc = map16<BF>(&tm.dh, dh, 32, 32, S64))) return rc;
     MmParams p{};
-    p.m_tiles = ceil_div(T, 128 * kCG);
-    p.n_tiles = ceil_div(F, kBN / 2);
-    p.which = p.splits = 1;
-    p.kblocks = p.kper = ceil_div(D, 64);
+    const int mt = ceil_div(T, 128 * kCG), ft = ceil_div(F, 128 * kCG), nt = ceil_div(D, b.bn), kd = ceil_div(D, 64);
+    p.g[0] = {mt, ceil_div(F, kBN / 2), 1, 1, kd, kd, 0};
     p.cols = static_cast<int>(F);
     p.act = act;
-    int rc = launch_mm<kCG, kBN, MM_BWD, BF, false>(ctx, x, x, wg, wu, dg, du, &dh, p, nullptr, s);
-    if (rc) return rc;
+    if ((rc = launch_mm<kCG, kBN, MM_BWD, BF>(ctx, tm, p, s))) return rc;
 
+    MmMaps tg{};
+    if ((rc = map16<BF>(&tg.a[0], dg, 64, 128, S128)) || (rc = map16<BF>(&tg.a[1], du, 64, 128, S128)) ||
+        (rc = map16<BF>(&tg.a[2], dg, 64, 64, S128)) || (rc = map16<BF>(&tg.a[3], du, 64, 64, S128)) ||
+        (rc = map16<BF>(&tg.b[0], wg, 64, 64, S128)) || (rc = map16<BF>(&tg.b[1], wu, 64, 64, S128)) ||
+        (rc = map16<BF>(&tg.b[2], x, 64, 64, S128)))
+        return rc;
+    auto part_map = [&](CUtensorMap* m, const float* part, int64_t rows) {
+        return encode_tmap_2d_swz(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, D, rows, D * 4, 32, 32, S128);
+    };
     MmParams q{};
-    q.m_tiles = ceil_div(T, 128 * kCG);
-    q.n_tiles = ceil_div(D, b.dx.bn);
-    q.which = 1;
-    q.splits = b.dx.splits;
     q.half = ceil_div(F, 64);
-    q.kblocks = 2 * q.half;
-    q.kper = ceil_div(q.kblocks, q.splits);
-    q.m_pad = q.m_tiles * 128 * kCG;
+    q.g[0] = {mt, nt, 1, b.s_dx, 2 * q.half, ceil_div(2 * q.half, b.s_dx), mt * 128 * kCG};
+    const int kt = ceil_div(T, 64);
+    q.g[1] = {ft, nt, 2, b.s_dw, kt, ceil_div(kt, b.s_dw), ft * 128 * kCG};
     q.cols = static_cast<int>(D);
-    rc = launch_any<MM_DX, BF>(ctx, b.dx, dg, du, wg, wu, dx, dx, q, part_dx, s);
-    if (!rc && q.splits > 1)
-        rc = sum_parts<BF>(ctx, part_dx, const_cast<void*>(dx.p), nullptr, 1, q.splits, q.m_pad, static_cast<int>(T), q.cols, s);
+    rc = b.s_dx > 1 ? part_map(&tg.o[0], part_dx, static_cast<int64_t>(b.s_dx) * q.g[0].m_pad) : map16<BF>(&tg.o[0], dx, 32, 32, S64);
     if (rc) return rc;
+    if (b.s_dw > 1)
+        rc = part_map(&tg.o[1], part_dw, 2ll * b.s_dw * q.g[1].m_pad);
+    else if (!(rc = map16<BF>(&tg.o[1], dwg, 32, 32, S64)))
+        rc = map16<BF>(&tg.o[2], dwu, 32, 32, S64);
+    if (rc) return rc;
+    rc = b.bn == 384 ? launch_mm<kCG, 384, MM_GRAD, BF>(ctx, tg, q, s) : launch_mm<kCG, 256, MM_GRAD, BF>(ctx, tg, q, s);
+    if (rc || (b.s_dx == 1 && b.s_dw == 1)) return rc;
 
-    MmParams r{};
-    r.m_tiles = ceil_div(F, 128 * kCG);
-    r.n_tiles = ceil_div(D, b.dw.bn);
-    r.which = 2;
-    r.splits = b.dw.splits;
-    r.kblocks = ceil_div(T, 64);
-    r.kper = ceil_div(r.kblocks, r.splits);
-    r.m_pad = r.m_tiles * 128 * kCG;
-    r.cols = static_cast<int>(D);
-    rc = launch_any<MM_DW, BF>(ctx, b.dw, dg, du, x, x, dwg, dwu, r, part_dw, s);
-    if (!rc && r.splits > 1)
-        rc = sum_parts<BF>(ctx, part_dw, const_cast<void*>(dwg.p), const_cast<void*>(dwu.p), 2, r.splits, r.m_pad, static_cast<int>(F), r.cols, s);
-    return rc;
+    SumJob j0{}, j1{};
+    if (b.s_dx > 1) j0 = {part_dx, {const_cast<void*>(dx.p), nullptr}, 1, b.s_dx, q.g[0].m_pad, static_cast<int>(T)};
+    if (b.s_dw > 1) j1 = {part_dw, {const_cast<void*>(dwg.p), const_cast<void*>(dwu.p)}, 2, b.s_dw, q.g[1].m_pad, static_cast<int>(F)};
+    const long long n8 = (static_cast<long long>(j0.rows) * j0.which + static_cast<long long>(j1.rows) * j1.which) * (D / 8);
+    const long long blocks = n8 / 256 + 1, most = static_cast<long long>(ctx->sm_count) * 8;
+    return launch_kernel(sum_parts_kernel<BF>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, s, false, j0, j1,
+                         static_cast<int>(D));
 }
 
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
