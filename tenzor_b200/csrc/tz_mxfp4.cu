@@ -493,22 +493,22 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
             const int colt = n * BN + sl * 64;
             if (lane == 0) tzp::bulk_wait_read<0>();  // the previous tile's stores have read the boxes
             __syncwarp();
+            uint32_t va[32], vb[32];
+            tzp::tmem_ld32(td, va);
+            tzp::tmem_ld32(td + 32, vb);
+            tzp::tmem_ld_wait();
+            tzp::tc_fence_before();  // the accumulator is in registers: the MMAs may have it back
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2)
+                    tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
+                else
+                    tzp::mbar_arrive(&tempty[acc]);
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int col0 = colt + 32 * c;
-                uint32_t v[32];
-                tzp::tmem_ld32(td + 32 * c, v);
-                tzp::tmem_ld_wait();
-                if (c == 1) {  // the accumulator is in registers: the MMAs may have it back
-                    tzp::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if constexpr (CG == 2)
-                            tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
-                        else
-                            tzp::mbar_arrive(&tempty[acc]);
-                    }
-                }
+                uint32_t(&v)[32] = c ? vb : va;
                 if constexpr (GATED) {
                     uint32_t o[8];
 #define TZ_G(A) \
