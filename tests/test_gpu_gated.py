@@ -254,3 +254,48 @@ def test_refusals(ctx):
     assert Lb.tz_gated_linear(ctx.handle, p(x), 64, p(wg), p(wu), p(dh), 4, 64, 72, _lib.OP["exp"], 1, None) == _lib.TZ_EINVAL
     assert Lb.tz_gated_linear(ctx.handle, p(x), 64, p(wg), p(wu), p(dh), 4, 64, 72, _lib.OP["silu"], 7, None) == _lib.TZ_EINVAL
     assert Lb.tz_gated_linear(None, p(x), 64, p(wg), p(wu), p(dh), 4, 64, 72, _lib.OP["silu"], 1, None) == _lib.TZ_EINVAL
+
+
+@pytest.mark.parametrize("reserve", [100, 140, 146])
+def test_few_sms(reserve):
+    """Leaving SMs to other kernels cuts the grids: more tiles per CTA, other splits, the same results."""
+    from tenzor_b200.runtime import Context
+    c = Context(0)
+    c.set_sm_reserve(reserve)
+    for T, D, F in ((5, 384, 1536), (700, 384, 1544), (300, 520, 328)):
+        check(c, *make(T, D, F, "bf16", seed=T), "gelu")
+    c.close()
+
+
+def test_no_sm_left_is_refused():
+    from tenzor_b200 import TenzorError, ops
+    from tenzor_b200.runtime import Context
+    c = Context(0)
+    c.set_sm_reserve(147)
+    x, wg, wu, dh = make(300, 64, 72, "bf16")
+    with pytest.raises(TenzorError):
+        ops.gated_linear(c, x, wg, wu)
+    c.close()
+
+
+def test_more_than_2_to_31_elements(ctx):
+    """h, dg and du of 2.2e9 elements: the last rows against the 64-bit formulas, and the weights' gradients as the
+    sum of those of two halves of the tokens."""
+    from tenzor_b200 import ops
+    T, D, F = 530_001, 64, 4104
+    x, wg, wu, _ = make(T, D, F, "bf16", seed=1)
+    dh = torch.empty((T, F), device="cuda", dtype=torch.bfloat16).normal_(0, 0.1, generator=torch.Generator(device="cuda").manual_seed(2))
+    h = ops.gated_linear(ctx, x, wg, wu, "silu")
+    dx, dwg, dwu = ops.gated_linear_backward(ctx, x, wg, wu, dh, "silu")
+    for at in (slice(0, 200), slice(T - 200, T)):
+        (wh, wdx, _, _), (th, tdx, _, _) = reference(x[at], wg, wu, dh[at], "silu")
+        near(h[at], wh, th, "h")
+        near(dx[at], wdx, tdx, "dx")
+    del h, dx
+    half = 265_024
+    a = ops.gated_linear_backward(ctx, x[:half], wg, wu, dh[:half], "silu")
+    b = ops.gated_linear_backward(ctx, x[half:], wg, wu, dh[half:], "silu")
+    for whole, p, q in ((dwg, a[1], b[1]), (dwu, a[2], b[2])):
+        want = p.double() + q.double()
+        rms = want.square().mean().sqrt()  # rounding of the three results, and of sums of 530 k products in f32
+        assert ((whole.double() - want).abs() <= 3 * U["bf16"] * (want.abs() + rms)).all()

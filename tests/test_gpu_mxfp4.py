@@ -284,3 +284,46 @@ def test_example_trains_and_serves(ctx):
     # (x, the two weights, h and Wd in turn) leave an angle of about 0.2 to 0.25.
     assert float(cos.mean()) > 0.95
     assert same <= 2.0 ** -6  # the kernels of one token and of a batch round h to 16 bits, then to 4, from other sums
+
+
+@pytest.mark.parametrize("reserve", [100, 146])
+def test_few_sms(reserve):
+    from tenzor_b200 import ops
+    from tenzor_b200.runtime import Context
+    c = Context(0)
+    c.set_sm_reserve(reserve)
+    for M, K, N in ((3, 512, 1000), (700, 288, 1544)):
+        x, w = rand(M, K, "bf16", M), rand(N, K, "bf16", N)
+        y = ops.linear_mxfp4(c, x, ops.quantize_mxfp4(c, w))
+        want, err = product64(x, w)
+        near(y, want, err + U["bf16"] * (want.abs() + err))
+    c.close()
+
+
+def test_more_than_2_to_31_elements(ctx):
+    from tenzor_b200 import ops
+    rows, cols = 1_050_007, 2080
+    x = torch.empty((rows, cols), device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator(device="cuda").manual_seed(3))
+    q = ops.quantize_mxfp4(ctx, x)
+    y = ops.dequantize_mxfp4(ctx, q, torch.bfloat16)
+    for at in (slice(0, 64), slice(rows - 64, rows)):
+        assert np.array_equal(y[at].double().cpu().numpy(), quant64(x[at].float().cpu().numpy())[0])
+    del y, q
+    M, K, N = 530_001, 96, 4104
+    x, w = x.view(-1)[:M * K].view(M, K), rand(N, K, "bf16", 1)
+    y = ops.linear_mxfp4(ctx, x, ops.quantize_mxfp4(ctx, w))
+    for at in (slice(0, 64), slice(M - 64, M)):
+        want, err = product64(x[at], w)
+        near(y[at], want, err + U["bf16"] * (want.abs() + err))
+
+
+@pytest.mark.parametrize("M,K", [(16, 8192), (16, 8448), (17, 8192), (32, 12320), (3, 16384)])
+def test_long_rows(ctx, M, K):
+    """Row lengths at which x no longer fits the few-rows kernel's shared memory, or only in more splits."""
+    from tenzor_b200 import ops
+    x, w = rand(M, K, "f16", M, spread=False), (rand(40, K, "f16", 40, spread=False).float() * K ** -0.5).half()
+    want, err = product64(x, w)
+    tol = err + U["f16"] * (want.abs() + err) + TINY["f16"]
+    for times in (1, 500):  # the same 40 weight rows again and again
+        y = ops.linear_mxfp4(ctx, x, ops.quantize_mxfp4(ctx, w.repeat(times, 1)))
+        near(y, want.repeat(1, times), tol.repeat(1, times), (M, K, times))
