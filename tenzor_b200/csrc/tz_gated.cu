@@ -88,7 +88,8 @@ struct MmCfg {
     static constexpr int TCOLS = BN == 384 ? 512 : 2 * BN;
     static_assert(!kDual || BN == 256, "16 epilogue warps of 32 output columns");
     static_assert(!kBmn || BNC % 64 == 0, "MN-major B comes in blocks of 64");
-    static_assert(BN == 256 || (BN == 384 && kBmn && CG == 2), "384 columns: two MMAs of 256 and 128");
+    static_assert(BN == 256 || ((BN == 128 || BN == 384) && kBmn && CG == 2), "384 columns: two MMAs of 256 and 128");
+    static constexpr int MMA_N = BN == 384 ? 256 : BN;
 };
 
 // 16 gate / up pairs -> 8 words of 16-bit outputs.
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(MmCfg<CG, BN, MODE>::THREADS, 1)
         if (rank == 0) {
             // ---- MMA issuer (the whole warp; one lane issues) ----
             const bool issue = tzp::elect_one();
-            constexpr uint32_t idesc0 = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 256) | (C::kBmn ? 1u << 16 : 0u);
+            constexpr uint32_t idesc0 = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, C::MMA_N) | (C::kBmn ? 1u << 16 : 0u);
             constexpr uint32_t idesc0_b = tzp::make_idesc(1, BF ? 1 : 0, 128 * CG, 128) | (C::kBmn ? 1u << 16 : 0u);  // columns 256 .. 383
             constexpr uint32_t kBstep = C::kBmn ? 2048u >> 4 : 2u;
             int stage = 0, acc = 0;
@@ -640,7 +641,9 @@ struct BwdPlan {
 // By an estimate in clocks: every tile's K blocks at the rate its operands arrive at (256 columns: 32 KB per SM and
 // K block, 384: 40 KB), an epilogue per tile (with one accumulator, 384 columns, not hidden), the tiles dealt round
 // the pairs, and the partial sums' way out and back.  384 columns cover D = 384 in one tile: 18106 tokens, F = 1536
-// took 166 us with 256 columns and 148 us with 384.
+// took 166 us with 256 columns and 148 us with 384.  128 columns give a few tokens more tiles, often enough to do
+// without the partial sums and their launch: 77 tokens, D = 384, F = 1000 23.0 us
+// with the sums split, 20.7 without.
 BwdPlan make_plan(int sms, int64_t T, int64_t D, int64_t F) {
     const int64_t groups = sms / kCG > 0 ? sms / kCG : 1;
     const int64_t mt = ceil_div(T, 128 * kCG), ft = ceil_div(F, 128 * kCG);
@@ -648,15 +651,17 @@ BwdPlan make_plan(int sms, int64_t T, int64_t D, int64_t F) {
     auto splits_ok = [](int kb, int s) { return s == 1 || (kb / s >= 8 && ceil_div(kb, ceil_div(kb, s)) == s); };
     BwdPlan best{};
     double best_cost = 1e300;
-    for (int bn = 256; bn <= 384; bn += 128) {
+    for (int bn = 128; bn <= 384; bn += 128) {
         const int64_t nt = ceil_div(D, bn);
-        const double rate = bn == 256 ? 600.0 : 820.0, epi = bn == 256 ? 800.0 : 5000.0;
+        const double epi = bn == 384 ? 5000.0 : 800.0;
         for (int sx = 1; sx <= 16; ++sx) {
             const int64_t nx = mt * nt * sx;
             if (!splits_ok(kx, sx) || (sx > 1 && nx > groups)) continue;
             for (int sw = 1; sw <= 16; ++sw) {
                 const int64_t nw = 2 * ft * nt * sw;
                 if (!splits_ok(kw, sw) || (sw > 1 && nw > groups)) continue;
+                // 24 KB per SM and K block for 128 columns: below the MMA's time only while few SMs ask L2 for it
+                const double rate = bn == 384 ? 820.0 : bn == 256 ? 600.0 : nx + nw <= groups / 2 ? 330.0 : 450.0;
                 const double cx = ceil_div(kx, sx) * rate + epi, cw = ceil_div(kw, sw) * rate + epi;
                 double cost = 0;  // of the slowest pair: pair g has the tiles g, g + groups, ..., dx's first
                 const int64_t first[3] = {0, nx % groups, (nx + nw) % groups};  // where the counts step down
@@ -668,7 +673,7 @@ BwdPlan make_plan(int sms, int64_t T, int64_t D, int64_t F) {
                 }
                 cost += 3000.0;
                 if (sx > 1 || sw > 1)
-                    cost += 6000.0 + 8.0 * D * ((sx > 1 ? static_cast<double>(sx) * T : 0.0) + (sw > 1 ? 2.0 * sw * F : 0.0)) / 2500.0;
+                    cost += 10000.0 + 8.0 * D * ((sx > 1 ? static_cast<double>(sx) * T : 0.0) + (sw > 1 ? 2.0 * sw * F : 0.0)) / 2500.0;
                 if (cost < best_cost) {
                     best_cost = cost;
                     best.bn = bn, best.s_dx = sx, best.s_dw = sw;
@@ -791,7 +796,9 @@ int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat
     else if (!(rc = map16<BF>(&tg.o[1], dwg, 32, 32, S64)))
         rc = map16<BF>(&tg.o[2], dwu, 32, 32, S64);
     if (rc) return rc;
-    rc = b.bn == 384 ? launch_mm<kCG, 384, MM_GRAD, BF>(ctx, tg, q, s) : launch_mm<kCG, 256, MM_GRAD, BF>(ctx, tg, q, s);
+    rc = b.bn == 384   ? launch_mm<kCG, 384, MM_GRAD, BF>(ctx, tg, q, s)
+         : b.bn == 256 ? launch_mm<kCG, 256, MM_GRAD, BF>(ctx, tg, q, s)
+                       : launch_mm<kCG, 128, MM_GRAD, BF>(ctx, tg, q, s);
     if (rc || (b.s_dx == 1 && b.s_dw == 1)) return rc;
 
     SumJob j0{}, j1{};
