@@ -346,10 +346,10 @@ def gated_linear(ctx: Context, x, w_gate, w_up, act: str = "silu", out=None):
     _full("gated_linear", "w_gate", ctx, w_gate, (F, D), dtype)
     _full("gated_linear", "w_up", ctx, w_up, (F, D), dtype)
     if out is None:
-        out = x.new_empty((T, F))
+        out = x.new_empty(T, F)
     else:
         _full("gated_linear", "out", ctx, out, (T, F), dtype)
-    rc = L.lib().tz_gated_linear(ctx.handle, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), out.data_ptr(), T, D, F,
+    rc = L.lib().tz_gated_linear(ctx.ptr, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), out.data_ptr(), T, D, F,
                                  code, dt, _on("gated_linear", ctx))
     if rc:
         L.check(rc)
@@ -379,8 +379,8 @@ def gated_linear_backward(ctx: Context, x, w_gate, w_up, dh, act: str = "silu"):
     stream = _on(fn, ctx)
     size = _gated_workspace(ctx.sm_count - ctx.sm_reserve, T, D, F)
     ws = x.new_empty(size, dtype=torch.uint8)
-    dx, dwg, dwu = x.new_empty((T, D)), x.new_empty((F, D)), x.new_empty((F, D))
-    rc = L.lib().tz_gated_linear_backward(ctx.handle, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), dh.data_ptr(), lddh,
+    dx, dwg, dwu = torch.empty_like(x, memory_format=torch.contiguous_format), torch.empty_like(w_gate), torch.empty_like(w_up)
+    rc = L.lib().tz_gated_linear_backward(ctx.ptr, x.data_ptr(), ldx, w_gate.data_ptr(), w_up.data_ptr(), dh.data_ptr(), lddh,
                                           dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), ws.data_ptr(), size, T, D, F, code, dt,
                                           stream)
     if rc:
@@ -457,7 +457,7 @@ def quantize_mxfp4(ctx: Context, x) -> Mxfp4:
     ldx = _rows("quantize_mxfp4", "x", ctx, x, rows, cols, x.dtype)
     stream = _on("quantize_mxfp4", ctx)
     q = Mxfp4(rows, cols, x)
-    rc = L.lib().tz_quantize_mxfp4(ctx.handle, x.data_ptr(), ldx, dt, q.codes_ptr, q.scales_ptr, rows, cols, stream)
+    rc = L.lib().tz_quantize_mxfp4(ctx.ptr, x.data_ptr(), ldx, dt, q.codes_ptr, q.scales_ptr, rows, cols, stream)
     if rc:
         L.check(rc)
     return q
@@ -470,8 +470,8 @@ def dequantize_mxfp4(ctx: Context, q: Mxfp4, dtype=torch.float32):
     if q.gated:
         raise ValueError("dequantize_mxfp4: a gated pair's rows are interleaved; quantise the matrices one by one")
     stream = _on("dequantize_mxfp4", ctx)
-    out = q.buf.new_empty((q.rows, q.cols), dtype=dtype)
-    rc = L.lib().tz_dequantize_mxfp4(ctx.handle, q.codes_ptr, q.scales_ptr, out.data_ptr(), dt, q.rows, q.cols, stream)
+    out = q.buf.new_empty(q.rows, q.cols, dtype=dtype)
+    rc = L.lib().tz_dequantize_mxfp4(ctx.ptr, q.codes_ptr, q.scales_ptr, out.data_ptr(), dt, q.rows, q.cols, stream)
     if rc:
         L.check(rc)
     return out
@@ -489,7 +489,7 @@ def pack_gated_mxfp4(ctx: Context, w_gate, w_up) -> Mxfp4:
     _full(fn, "w_up", ctx, w_up, (F, D), w_gate.dtype)
     stream = _on(fn, ctx)
     q = Mxfp4(2 * F, D, w_gate, gated=True)
-    L.check(L.lib().tz_pack_gated_mxfp4(ctx.handle, w_gate.data_ptr(), w_up.data_ptr(), dt, q.codes_ptr, q.scales_ptr, F, D, stream))
+    L.check(L.lib().tz_pack_gated_mxfp4(ctx.ptr, w_gate.data_ptr(), w_up.data_ptr(), dt, q.codes_ptr, q.scales_ptr, F, D, stream))
     return q
 
 
@@ -520,18 +520,18 @@ def linear_mxfp4(ctx: Context, x, w: Mxfp4, bias=None, out_dtype=None, out=None)
         bias = bias.data_ptr()
     stream = _on(fn, ctx)
     if out is None:
-        out = w.buf.new_empty((M, N), dtype=out_dtype)
+        out = w.buf.new_empty(M, N, dtype=out_dtype) if given or x.dtype is not out_dtype else x.new_empty(M, N)
     else:
         _full(fn, "out", ctx, out, (M, N), out_dtype)
     if given:
         _mx(fn, "x", ctx, x)
-        rc = L.lib().tz_gemm_mxfp4(ctx.handle, x.codes_ptr, x.scales_ptr, w.codes_ptr, w.scales_ptr, bias, out.data_ptr(), ydt,
+        rc = L.lib().tz_gemm_mxfp4(ctx.ptr, x.codes_ptr, x.scales_ptr, w.codes_ptr, w.scales_ptr, bias, out.data_ptr(), ydt,
                                    M, K, N, stream)
     else:
         ldx = _rows(fn, "x", ctx, x, M, K, x.dtype)
         size = _mx_workspace(M, K, N)
         ws = x.new_empty(size, dtype=torch.uint8) if size else None
-        rc = L.lib().tz_linear_mxfp4(ctx.handle, x.data_ptr(), ldx, _dtype_f(fn, x.dtype), w.codes_ptr, w.scales_ptr, bias,
+        rc = L.lib().tz_linear_mxfp4(ctx.ptr, x.data_ptr(), ldx, _dtype_f(fn, x.dtype), w.codes_ptr, w.scales_ptr, bias,
                                      out.data_ptr(), ydt, ws.data_ptr() if size else None, size, M, K, N, stream)
     if rc:
         L.check(rc)
@@ -555,12 +555,12 @@ def gated_linear_mxfp4(ctx: Context, x, w: Mxfp4, act: str = "silu", out=None):
     ldx = _rows(fn, "x", ctx, x, T, D, dtype)
     stream = _on(fn, ctx)
     if out is None:
-        out = x.new_empty((T, F))
+        out = x.new_empty(T, F)
     else:
         _full(fn, "out", ctx, out, (T, F), dtype)
     size = _mx_workspace(T, D, 2 * F)
     ws = x.new_empty(size, dtype=torch.uint8) if size else None
-    rc = L.lib().tz_gated_linear_mxfp4(ctx.handle, x.data_ptr(), ldx, _DTF[dtype], w.codes_ptr, w.scales_ptr, out.data_ptr(), code,
+    rc = L.lib().tz_gated_linear_mxfp4(ctx.ptr, x.data_ptr(), ldx, _DTF[dtype], w.codes_ptr, w.scales_ptr, out.data_ptr(), code,
                                        ws.data_ptr() if size else None, size, T, D, F, stream)
     if rc:
         L.check(rc)

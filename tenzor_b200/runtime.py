@@ -15,6 +15,7 @@ class Context:
         h = C.c_void_p()
         L.check(L.lib().tz_cuda_create(device, C.byref(h)))
         self.handle = h
+        self.ptr = h.value  # the handle as a plain address: what the small, frequent calls pass
         self.device = device
         self.sm_count = L.lib().tz_cuda_sm_count(h)
         self.sm_reserve = 0
@@ -40,7 +41,7 @@ class Context:
             for obj in list(self._owned):
                 obj.close()
             L.lib().tz_cuda_destroy(self.handle)
-            self.handle = None
+            self.handle = self.ptr = None
 
     def __del__(self):
         try:
