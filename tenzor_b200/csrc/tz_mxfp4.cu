@@ -251,17 +251,22 @@ struct MxParams {
     int act;
 };
 
-template <int CG>
+template <int CG, bool GATED>
 struct MxCfg {
     static constexpr int BN = 192;
-    static constexpr int EPI = 12;  // 4 TMEM lane quarters x 3 slices of 64 columns
+    // A group of 12 epilogue warps reads an accumulator: 4 TMEM lane quarters x 3 slices of 64 columns.  The gated
+    // form, bound by its exponentials, has a group for each of the two accumulators, so that one group's loads and
+    // stores run under the other's arithmetic.
+    static constexpr int GROUPS = GATED ? 2 : 1;
+    static constexpr int EPI = 12 * GROUPS;
     static constexpr int THREADS = 64 + 32 * EPI;
     static constexpr int BNC = BN / CG;
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int B_BYTES = BNC * 128;
     static constexpr int SF_BYTES = 3072;  // A: 2 chunks; B: 2 row blocks x 2 chunks
     static constexpr int STAGE = A_BYTES + B_BYTES + SF_BYTES;
-    static constexpr int STAGING = EPI * 4096;
+    static constexpr int BOX = GATED ? 2048 : 4096;  // staging of one epilogue warp
+    static constexpr int STAGING = EPI * BOX;
     static constexpr int STAGES = CG == 2 ? 5 : 4;
     static constexpr int SF_COLS = 24;
     static constexpr int SF0 = 2 * BN;
@@ -306,10 +311,10 @@ __device__ __forceinline__ void sf_copy(uint32_t taddr, uint32_t smem_addr) {
 }
 
 template <int CG, int OUT, bool GATED>
-__global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
+__global__ void __launch_bounds__(MxCfg<CG, GATED>::THREADS, 1)
     mxfp4_mm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO,
                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const MxParams p, int* status) {
-    using C = MxCfg<CG>;
+    using C = MxCfg<CG, GATED>;
     constexpr int STAGES = C::STAGES, BN = C::BN;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = tzp::smem_u32(smem_raw);
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
         }
         for (int a = 0; a < 2; ++a) {
             tzp::mbar_init(&tfull[a], 1);
-            tzp::mbar_init(&tempty[a], C::EPI * CG);
+            tzp::mbar_init(&tempty[a], 12 * CG);
         }
         tzp::mbar_init(drain, 1);
         *abort_flag = 0;
@@ -483,15 +488,15 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
         }
     } else {
         // ---- epilogue: TMEM lane quarter (warp % 4), 64 of the columns ----
-        const int e = warp - 2, q4 = warp & 3, sl = e >> 2;
-        const uint32_t box = tzp::smem_u32(staging) + static_cast<uint32_t>(e * 4096);
-        uint8_t* boxp = staging + e * 4096;
-        int acc = 0;
+        const int e = warp - 2, q4 = warp & 3, grp = e / 12, sl = (e - grp * 12) >> 2;
+        const uint32_t box = tzp::smem_u32(staging) + static_cast<uint32_t>(e * C::BOX);
+        uint8_t* boxp = staging + e * C::BOX;
+        int acc = grp;  // two groups: each keeps to its accumulator and takes every other tile
         uint32_t acc_phase = 0;
-        for (int t = t0; t < num_tiles; t += tstep) {
+        for (int t = t0 + grp * tstep; t < num_tiles; t += C::GROUPS * tstep) {
             int m, n;
             tile_of(t, m, n);
-            if (t + tstep >= num_tiles) tzp::pdl_trigger();
+            if (t + C::GROUPS * tstep >= num_tiles) tzp::pdl_trigger();
             if (!tzp::warp_wait(&tfull[acc], acc_phase, status, abort_flag)) break;
             tzp::tc_fence_after();
             const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) + static_cast<uint32_t>(acc * BN + sl * 64);
@@ -499,22 +504,22 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
             const int colt = n * BN + sl * 64;
             if (lane == 0) tzp::bulk_wait_read<0>();  // the previous tile's stores have read the boxes
             __syncwarp();
-            uint32_t va[32], vb[32];
-            tzp::tmem_ld32(td, va);
-            tzp::tmem_ld32(td + 32, vb);
-            tzp::tmem_ld_wait();
-            tzp::tc_fence_before();  // the accumulator is in registers: the MMAs may have it back
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (CG == 2)
-                    tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
-                else
-                    tzp::mbar_arrive(&tempty[acc]);
-            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int col0 = colt + 32 * c;
-                uint32_t(&v)[32] = c ? vb : va;
+                uint32_t v[32];
+                tzp::tmem_ld32(td + 32 * c, v);
+                tzp::tmem_ld_wait();
+                if (c == 1) {  // the accumulator is in registers: the MMAs may have it back
+                    tzp::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (CG == 2)
+                            tzp::mbar_arrive_cluster(tzp::mapa(&tempty[acc], 0));
+                        else
+                            tzp::mbar_arrive(&tempty[acc]);
+                    }
+                }
                 if constexpr (GATED) {
                     uint32_t o[8];
 #define TZ_G(A) \
@@ -574,11 +579,14 @@ __global__ void __launch_bounds__(MxCfg<CG>::THREADS, 1)
                     tzp::bulk_commit();
                 }
             }
-            if (++acc == 2) {
+            if (C::GROUPS == 2) {
+                acc_phase ^= 1u;
+            } else if (++acc == 2) {
                 acc = 0;
                 acc_phase ^= 1u;
             }
         }
+        tzp::pdl_trigger();  // a group without a tile
         if (lane == 0) tzp::bulk_wait_all();
     }
 
@@ -861,7 +869,7 @@ struct Q4 {
 
 template <int CG, int OUT, bool GATED>
 int launch_mx_cg(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, void* y, int act, cudaStream_t s) {
-    using C = MxCfg<CG>;
+    using C = MxCfg<CG, GATED>;
     auto kern = mxfp4_mm_kernel<CG, OUT, GATED>;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::SMEM, done);
@@ -899,7 +907,7 @@ int launch_mx_cg(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bia
 // one round of pairs single CTAs take them (64 rows, D = 4096, 2 F = 16384: 14.8 us instead of 18.6).
 template <int OUT, bool GATED>
 int launch_mx(tz_ctx_t ctx, const Q4& a, const Q4& b, int k, const float* bias, void* y, int act, cudaStream_t s) {
-    if (a.rows <= 128 && ceil_div(b.rows, MxCfg<1>::BN) > (ctx->sm_count - ctx->sm_reserve) / 2) return launch_mx_cg<1, OUT, GATED>(ctx, a, b, k, bias, y, act, s);
+    if (a.rows <= 128 && ceil_div(b.rows, MxCfg<1, GATED>::BN) > (ctx->sm_count - ctx->sm_reserve) / 2) return launch_mx_cg<1, OUT, GATED>(ctx, a, b, k, bias, y, act, s);
     return launch_mx_cg<kCG, OUT, GATED>(ctx, a, b, k, bias, y, act, s);
 }
 
