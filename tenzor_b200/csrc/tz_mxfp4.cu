@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(256) dequantize_mxfp4_kernel(const uint8_t* co
 // for 384 clocks of MMAs, is the bound), about 240 us in a loop under the power cap.  The issue of a K block's six
 // scale copies and four MMAs is serial: with a branch on the lane number around it (operands moved to uniform
 // registers one by one) a K block took 1050 clocks and the product 355 us.  The encoder batch's gated form (T 18106,
-// D 384, F 1536) takes 31 us: two K blocks a tile, bound by the epilogue (special-function unit 54 %).
+// D 384, F 1536) takes 26 us: two K blocks a tile, bound by the epilogue (special-function
+// unit 61 %; 31 us with one group of epilogue warps for both accumulators).
 constexpr int GROUP = 16;
 
 struct MxParams {
@@ -614,9 +615,9 @@ __global__ void __launch_bounds__(MxCfg<CG, GATED>::THREADS, 1)
 // CTA needs its K slice only, so the work (0.5 us for 16 rows of 4096) hides behind the first weight copies and the
 // separate quantiser launch goes away.  With GATED a warp's 32 TMEM lanes are 16 gate rows and their 16 up rows.
 //
-// Measured (weights from L2): D 4096, 2 F 16384 gated 9.5 us for one row, 10.2 for 16; K 4096, N 8192 6.1 and 7.6.
-// What is left over the weights' own time (5.4 and 2.7 us from HBM) is the launch and the first copies (about 3 us)
-// and the serial issue per K block, which two CTAs per SM overlap (one per SM took 13.1 us for 16 rows).
+// Measured (weights from HBM): D 4096, 2 F 16384 gated 9.2 us for one row, 9.9 for 16, 13.4 for 32; K 4096, N 8192 6.0,
+// 7.2 and 9.6.  What is left over the weights' own time (5.4 and 2.7 us) is the launch and the first copies (about 3 us)
+// and, from 16 rows on, the quantising.
 struct MxRowsParams {
     const void* x;
     long long ldx;
@@ -629,13 +630,13 @@ struct MxRowsParams {
 
 template <int N>
 struct MxRowsCfg {
-    static constexpr int QWARPS = 8;
-    static constexpr int THREADS = 64 + 32 * QWARPS;
+    static constexpr int QWARPS = N == 32 ? 16 : 8;  // two rows of a K block each
+    static constexpr int THREADS = 96 + 32 * QWARPS;
     static constexpr int STAGE = 16384 + 1024;
-    static constexpr int STAGES = 4;             // two CTAs fit an SM: the MMA issue of one K block (about 700 clocks) is serial
+    static constexpr int STAGES = 4;             // even: a stage's K blocks belong to one MMA issuer
     static constexpr int SF_COLS = 16;           // per stage: A 2 x 4, B 2 x 4
-    static constexpr int SF0 = 32;
-    static constexpr int TCOLS = 128;            // 32 + 4 * 16
+    static constexpr int SF0 = 64;
+    static constexpr int TCOLS = 128;            // two accumulators of 32, 4 * 16 columns of scales
     static constexpr int B_KB = N * 128 + 1024;  // one K block of x: codes and two scale chunks
     static constexpr int PART = 128 * N * 4;
     static constexpr int MAX_SPLIT = 1 + STAGES * STAGE / PART;
@@ -644,7 +645,7 @@ struct MxRowsCfg {
 };
 
 template <int N, int XDT, int OUT, bool GATED>
-__global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 2)
+__global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
     mxfp4_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW, const MxRowsParams p, int* status) {
     using C = MxRowsCfg<N>;
     constexpr int STAGES = C::STAGES;
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 2)
             tzp::mbar_init(&full[s], 1);
             tzp::mbar_init(&empty[s], 1);
         }
-        tzp::mbar_init(done, 1);
+        tzp::mbar_init(done, 2);
         for (int i = 0; i < 32; ++i) tzp::mbar_init(&xready[i], C::QWARPS);
         *abort_flag = 0;
         tzp::fence_mbar_init();
@@ -705,11 +706,15 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 2)
             for (int s = 0; s < STAGES; ++s)  // every copy has landed before the stages are used again (bounded)
                 if (armed & (1u << s)) tzp::mbar_wait(&full[s], (armed_par >> s) & 1u, status, nullptr);
         }
-    } else if (warp == 1) {
-        {  // the whole warp; one lane issues
+    } else if (warp == 1 || warp == 2 + C::QWARPS) {
+        // Two MMA issuers (whole warps; one lane issues) take the K blocks in turn, each with an accumulator of its own:
+        // the issue of a K block's scale copies and MMAs is serial, and the tensor core idles for most of it.
+        {
             const bool issue = tzp::elect_one();
+            const int mi = warp == 1 ? 0 : 1;
+            const uint32_t d = tmem_base + 32u * mi;
             constexpr uint32_t idesc0 = mx_idesc(128, N, 0), idesc2 = mx_idesc(128, N, 2);
-            for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+            for (int kb = kb0 + mi, i = mi; kb < kb1; kb += 2, i += 2) {
                 const int s = i % STAGES;
                 if (!tzp::warp_wait(&xready[i], 0, status, abort_flag)) break;
                 if (!tzp::warp_wait(&full[s], (i / STAGES) & 1, status, abort_flag)) break;
@@ -728,8 +733,8 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 2)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         if (k == 0 || left > 64 * k)
-                            mx_mma<1>(tmem_base, ad + 2u * k, bd + 2u * k, (k & 1) ? idesc2 : idesc0, tsf + 4 * (k >> 1), tsf + 8 + 4 * (k >> 1),
-                                      (i | k) != 0 ? 1u : 0u);
+                            mx_mma<1>(d, ad + 2u * k, bd + 2u * k, (k & 1) ? idesc2 : idesc0, tsf + 4 * (k >> 1), tsf + 8 + 4 * (k >> 1),
+                                      (i > mi || k != 0) ? 1u : 0u);
                     tzp::umma_commit(&empty[s]);
                 }
                 __syncwarp();
@@ -740,7 +745,7 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 2)
         }
     } else {
         // ---- quantise this CTA's K slice of x, one K block (256 values of N rows) after the other; a warp takes
-        // N / 8 rows of the block, a lane 8 values of each.  Rows past the last one are zeros with the smallest scale.
+        // two rows of the block, a lane 8 values of each.  Rows past the last one are zeros with the smallest scale.
         // The next block's values are on their way while a block is quantised. ----
         constexpr int R = N / C::QWARPS;
         Raw8<XDT> v[R];
@@ -789,14 +794,22 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 2)
     const int q4 = warp & 3, row = q4 * 32 + lane;  // weight row n0 + row
     float* part = reinterpret_cast<float*>(smem);   // [rank - 1][N][128]
     const uint32_t td = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16);
-    const bool epi = warp >= 2 && warp < 6;
+    const bool epi = warp >= 2 && warp < 6, two = kb1 - kb0 > 1;
+    auto sums = [&](int c, uint32_t (&v)[16]) {  // 16 columns of both accumulators
+        uint32_t w[16];
+        tzp::tmem_ld16(td + c, v);
+        tzp::tmem_ld16(td + 32 + c, w);
+        tzp::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (two) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(w[j]));
+    };
     if (rank > 0 && epi) {
         const uint32_t dst = tzp::mapa(part + (rank - 1) * N * 128 + row, 0);
 #pragma unroll 1
         for (int c = 0; c < N; c += 16) {
             uint32_t v[16];
-            tzp::tmem_ld16(td + c, v);
-            tzp::tmem_ld_wait();
+            sums(c, v);
 #pragma unroll
             for (int j = 0; j < 16; ++j) st_cluster_f32(dst + (c + j) * 512, __uint_as_float(v[j]));
         }
@@ -809,8 +822,7 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 2)
         for (int c = 0; c < N; c += 16) {
             if (c >= p.rows) break;
             uint32_t v[16];
-            tzp::tmem_ld16(td + c, v);
-            tzp::tmem_ld_wait();
+            sums(c, v);
             for (int r = 1; r < ranks; ++r) {
                 const float* src = part + (r - 1) * N * 128 + row;
 #pragma unroll
@@ -920,15 +932,15 @@ int launch_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int rows, const Q4&
     const int tiles = ceil_div(w.rows, 128), kblocks = ceil_div(k, 256);
     *ran = false;
     if (tiles > 65535) return TZ_OK;  // the grid's second extent
-    // With room for 32 rows quantising x costs each CTA more than the large kernel's tiles cost once there is more
-    // than one CTA per SM: 32 rows, D = 4096, 2 F = 32768 take 30.6 us here, 27.0 there; 2 F = 16384 16.0 and 19.5.
-    if (N > 16 && tiles > ctx->sm_count) return TZ_OK;
+    // With room for 32 rows every CTA's quantising of x weighs more, and from the third wave of CTAs on the large
+    // kernel is faster: 17 / 32 rows take 22.8 / 25.2 us here and 25.3 / 25.0 there at 256 tiles (D = 4096), 28.6 / 31.3
+    // and 23.1 / 22.2 us at 512 tiles (D = 2048).
+    if (N > 16 && tiles > 2 * ctx->sm_count) return TZ_OK;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::smem(C::MAX_KB), done);
     if (rc) return rc;
     int splits = 1;
-    const int ctas = 2 * (ctx->sm_count - ctx->sm_reserve);
-    if ((rc = rows_splits<N * 100 + XDT * 20 + OUT * 4 + GATED + 1>(kern, C::THREADS, C::smem, ctas, tiles, kblocks, C::MAX_SPLIT, &splits)))
+    if ((rc = rows_splits<N * 100 + XDT * 20 + OUT * 4 + GATED + 1>(kern, C::THREADS, C::smem, ctx->sm_count - ctx->sm_reserve, tiles, kblocks, C::MAX_SPLIT, &splits)))
         return rc;
     MxRowsParams p{};
     p.kblocks = kblocks;
