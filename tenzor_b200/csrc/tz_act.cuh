@@ -81,6 +81,18 @@ __device__ __forceinline__ uint32_t gated_pair(uint32_t g0, uint32_t g1, uint32_
     return tzp::pack16x2<BF>(h.x, h.y);
 }
 
+// Two gate / up pairs and their outputs' gradients to packed 16-bit dg = dh u act'(g) and du = dh act(g).
+template <int ACT, bool BF>
+__device__ __forceinline__ void gated_pair_grad(uint32_t g0, uint32_t g1, uint32_t u0, uint32_t u1, float2 dh, uint32_t& dg, uint32_t& du) {
+    uint64_t d;
+    const uint64_t h2 = tzp::f2_pack(dh.x, dh.y);
+    const uint64_t a = gated_act2<ACT, true>(tzp::f2_pack(__uint_as_float(g0), __uint_as_float(g1)), d);
+    const float2 p = tzp::f2_unpack(tzp::f2_mul(tzp::f2_mul(h2, tzp::f2_pack(__uint_as_float(u0), __uint_as_float(u1))), d));
+    const float2 q = tzp::f2_unpack(tzp::f2_mul(h2, a));
+    dg = tzp::pack16x2<BF>(p.x, p.y);
+    du = tzp::pack16x2<BF>(q.x, q.y);
+}
+
 #define TZ_ACT_SWITCH(act, CALL)                          \
     switch (act) {                                        \
         case TZ_OP_SILU: CALL(TZ_OP_SILU); break;         \

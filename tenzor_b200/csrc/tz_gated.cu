@@ -102,18 +102,7 @@ template <int ACT, bool BF>
 __device__ __forceinline__ void bwd_math(const uint32_t (&g)[16], const uint32_t (&u)[16], const uint32_t* dh, uint32_t* dg, uint32_t* du) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        float2 h;
-        if constexpr (BF)
-            h = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&dh[j]));
-        else
-            h = __half22float2(*reinterpret_cast<const __half2*>(&dh[j]));
-        uint64_t d;
-        const uint64_t h2 = tzp::f2_pack(h.x, h.y);
-        const uint64_t a = gated_act2<ACT, true>(tzp::f2_pack(__uint_as_float(g[2 * j]), __uint_as_float(g[2 * j + 1])), d);
-        const float2 p = tzp::f2_unpack(tzp::f2_mul(tzp::f2_mul(h2, tzp::f2_pack(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]))), d));
-        const float2 q = tzp::f2_unpack(tzp::f2_mul(h2, a));
-        dg[j] = tzp::pack16x2<BF>(p.x, p.y);
-        du[j] = tzp::pack16x2<BF>(q.x, q.y);
+        gated_pair_grad<ACT, BF>(g[2 * j], g[2 * j + 1], u[2 * j], u[2 * j + 1], widen2<BF>(dh[j]), dg[j], du[j]);
     }
 }
 
@@ -639,7 +628,7 @@ struct BwdPlan {
 };
 
 // By an estimate in clocks: every tile's K blocks at the rate its operands arrive at (256 columns: 32 KB per SM and
-// K block, 384: 40 KB), an epilogue per tile (with one accumulator, 384 columns, not hidden), the tiles dealt round
+// K block, 384: 40 KB), the epilogue (beside it, or with one accumulator, 384 columns, after it), the tiles dealt round
 // the pairs, and the partial sums' way out and back.  384 columns cover D = 384 in one tile: 18106 tokens, F = 1536
 // took 166 us with 256 columns and 148 us with 384.  128 columns give a few tokens more tiles, often enough to do
 // without the partial sums and their launch: 77 tokens, D = 384, F = 1000 23.0 us
@@ -653,7 +642,7 @@ BwdPlan make_plan(int sms, int64_t T, int64_t D, int64_t F) {
     double best_cost = 1e300;
     for (int bn = 128; bn <= 384; bn += 128) {
         const int64_t nt = ceil_div(D, bn);
-        const double epi = bn == 384 ? 5000.0 : 800.0;
+        const double epi = bn == 384 ? 5000.0 : bn == 256 ? 3000.0 : 1700.0;  // an epilogue's own time
         for (int sx = 1; sx <= 16; ++sx) {
             const int64_t nx = mt * nt * sx;
             if (!splits_ok(kx, sx) || (sx > 1 && nx > groups)) continue;
@@ -662,7 +651,11 @@ BwdPlan make_plan(int sms, int64_t T, int64_t D, int64_t F) {
                 if (!splits_ok(kw, sw) || (sw > 1 && nw > groups)) continue;
                 // 24 KB per SM and K block for 128 columns: below the MMA's time only while few SMs ask L2 for it
                 const double rate = bn == 384 ? 820.0 : bn == 256 ? 600.0 : nx + nw <= groups / 2 ? 330.0 : 450.0;
-                const double cx = ceil_div(kx, sx) * rate + epi, cw = ceil_div(kw, sw) * rate + epi;
+                auto tile = [&](int kb) {  // with two accumulators the longer of MMAs and epilogue
+                    const double c = kb * rate + 500.0;
+                    return bn == 384 ? c + epi : c > epi ? c : epi;
+                };
+                const double cx = tile(ceil_div(kx, sx)), cw = tile(ceil_div(kw, sw));
                 double cost = 0;  // of the slowest pair: pair g has the tiles g, g + groups, ..., dx's first
                 const int64_t first[3] = {0, nx % groups, (nx + nw) % groups};  // where the counts step down
                 for (int64_t g : first) {
@@ -712,10 +705,10 @@ int dual_maps(MmMaps* tm, const Mat& x, const Mat& wg, const Mat& wu, const Mat&
     return o1.p ? map16<BF>(&tm->o[1], o1, 32, 32, S64) : TZ_OK;
 }
 
-template <int N, bool BF>
-int launch_rows(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& h, int act, cudaStream_t s) {
+template <int N, bool BF, bool GRAD>
+int launch_rows(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& o0, const Mat& o1, const Mat& dh, int act, cudaStream_t s) {
     using C = RowsCfg<N>;
-    auto kern = gated_rows_kernel<N, BF>;
+    auto kern = gated_rows_kernel<N, BF, GRAD>;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::SMEM, done);
     if (rc) return rc;
@@ -723,27 +716,40 @@ int launch_rows(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const 
     const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B;
     if ((rc = map16<BF>(&mx, x, 64, N, S128)) || (rc = map16<BF>(&mg, wg, 64, 128, S128)) || (rc = map16<BF>(&mu, wu, 64, 128, S128))) return rc;
     RowsParams p{};
-    const int tiles = ceil_div(h.cols, 128);
+    const int tiles = ceil_div(o0.cols, 128);
     p.kblocks = ceil_div(x.cols, 64);
     int splits = 1;
-    if ((rc = rows_splits<N>(kern, C::THREADS, [](int) { return C::SMEM; }, ctx->sm_count - ctx->sm_reserve, tiles, p.kblocks, C::MAX_SPLIT, &splits))) return rc;
+    if ((rc = rows_splits<N + GRAD>(kern, C::THREADS, [](int) { return C::SMEM; }, ctx->sm_count - ctx->sm_reserve, tiles, p.kblocks, C::MAX_SPLIT,
+                                    &splits)))
+        return rc;
     p.kper = ceil_div(p.kblocks, splits);
     p.t = static_cast<int>(x.rows);
-    p.f = static_cast<int>(h.cols);
+    p.f = static_cast<int>(o0.cols);
     p.act = act;
-    p.h = const_cast<void*>(h.p);
+    p.h = const_cast<void*>(o0.p);
+    p.du = const_cast<void*>(o1.p);
+    p.dh = dh.p;
+    p.lddh = dh.ld;
     return launch_cluster(kern, splits, dim3(splits, tiles), dim3(C::THREADS), C::SMEM, s, true, mx, mg, mu, p, ctx->d_status);
+}
+
+// The few-token kernel; *ran says whether the sizes are its own.
+template <bool BF, bool GRAD>
+int try_rows(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& o0, const Mat& o1, const Mat& dh, int act, cudaStream_t s,
+             bool* ran) {
+    *ran = x.rows <= kRowsMax && o0.cols <= 128 * 65535;  // the grid's second extent
+    if (!*ran) return TZ_OK;
+    return x.rows <= 16 ? launch_rows<16, BF, GRAD>(ctx, x, wg, wu, o0, o1, dh, act, s)
+                        : launch_rows<32, BF, GRAD>(ctx, x, wg, wu, o0, o1, dh, act, s);
 }
 
 template <bool BF>
 int forward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat& h, int act, cudaStream_t s) {
-    if (x.rows <= kRowsMax && h.cols <= 128 * 65535) {  // the grid's second extent
-        if (x.rows <= 16) return launch_rows<16, BF>(ctx, x, wg, wu, h, act, s);
-        return launch_rows<32, BF>(ctx, x, wg, wu, h, act, s);
-    }
+    bool ran = false;
+    int rc = try_rows<BF, false>(ctx, x, wg, wu, h, Mat{}, Mat{}, act, s, &ran);
+    if (rc || ran) return rc;
     MmMaps tm{};
-    int rc = dual_maps<BF>(&tm, x, wg, wu, h, Mat{});
-    if (rc) return rc;
+    if ((rc = dual_maps<BF>(&tm, x, wg, wu, h, Mat{}))) return rc;
     MmParams p{};
     const int kb = ceil_div(x.cols, 64);
     p.g[0] = {ceil_div(x.rows, 128 * kCG), ceil_div(h.cols, kBN / 2), 1, 1, kb, kb, 0};
@@ -764,15 +770,19 @@ int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat
     float* part_dw = reinterpret_cast<float*>(ws + 2 * b.dgdu + b.part_dx);
     const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B, S64 = CU_TENSOR_MAP_SWIZZLE_64B;
 
-    MmMaps tm{};
-    int rc = dual_maps<BF>(&tm, x, wg, wu, dg, du);
-    if (rc || (rc = map16<BF>(&tm.dh, dh, 32, 32, S64))) return rc;
-    MmParams p{};
     const int mt = ceil_div(T, 128 * kCG), ft = ceil_div(F, 128 * kCG), nt = ceil_div(D, b.bn), kd = ceil_div(D, 64);
-    p.g[0] = {mt, ceil_div(F, kBN / 2), 1, 1, kd, kd, 0};
-    p.cols = static_cast<int>(F);
-    p.act = act;
-    if ((rc = launch_mm<kCG, kBN, MM_BWD, BF>(ctx, tm, p, s))) return rc;
+    bool ran = false;
+    int rc = try_rows<BF, true>(ctx, x, wg, wu, dg, du, dh, act, s, &ran);
+    if (rc) return rc;
+    if (!ran) {
+        MmMaps tm{};
+        if ((rc = dual_maps<BF>(&tm, x, wg, wu, dg, du)) || (rc = map16<BF>(&tm.dh, dh, 32, 32, S64))) return rc;
+        MmParams p{};
+        p.g[0] = {mt, ceil_div(F, kBN / 2), 1, 1, kd, kd, 0};
+        p.cols = static_cast<int>(F);
+        p.act = act;
+        if ((rc = launch_mm<kCG, kBN, MM_BWD, BF>(ctx, tm, p, s))) return rc;
+    }
 
     MmMaps tg{};
     if ((rc = map16<BF>(&tg.a[0], dg, 64, 128, S128)) || (rc = map16<BF>(&tg.a[1], du, 64, 128, S128)) ||

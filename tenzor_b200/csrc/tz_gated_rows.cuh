@@ -1,5 +1,5 @@
 // tz_gated_rows.cuh -- the gated block for few tokens (serving, one token at a time): bound by reading the two
-// weight matrices once.
+// weight matrices once.  GRAD is the backward pass's first kernel for few tokens: dg and du from the same products.
 //
 // The tensor core's roles are swapped: 128 rows of Wg and of Wu are the two A tiles (M = 128 output features)
 // and up to 32 tokens the B tile (N), so no lane works on padding that costs bandwidth.  The K blocks of a
@@ -22,10 +22,22 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// A packed 16-bit pair as f32.
+template <bool BF>
+__device__ __forceinline__ float2 widen2(uint32_t w) {
+    if constexpr (BF)
+        return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+    else
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
 struct RowsParams {
     int kblocks, kper;  // K blocks of 64, and of one cluster rank
     int t, f, act;
-    void* h;
+    void* h;         // GRAD: dg
+    void* du;        // GRAD
+    const void* dh;  // GRAD: [t, f], row stride lddh
+    long long lddh;
 };
 
 template <int N>
@@ -39,7 +51,7 @@ struct RowsCfg {
     static constexpr int MAX_SPLIT = 1 + STAGES * STAGE / PART;
 };
 
-template <int N, bool BF>
+template <int N, bool BF, bool GRAD>
 __global__ void __launch_bounds__(RowsCfg<N>::THREADS, 1)
     gated_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmU,
                       const RowsParams p, int* status) {
@@ -151,6 +163,7 @@ __global__ void __launch_bounds__(RowsCfg<N>::THREADS, 1)
     if (rank == 0 && warp >= 2) {
         const int ranks = (p.kblocks + p.kper - 1) / p.kper;
         uint16_t* out = reinterpret_cast<uint16_t*>(p.h) + f0 + row;
+        uint16_t* out2 = reinterpret_cast<uint16_t*>(p.du) + f0 + row;
 #pragma unroll 1
         for (int c = 0; c < N; c += 16) {
             if (c >= p.t) break;
@@ -166,15 +179,33 @@ __global__ void __launch_bounds__(RowsCfg<N>::THREADS, 1)
                     u[j] = __float_as_uint(__uint_as_float(u[j]) + src[(N + c + j) * 128]);
                 }
             }
-            uint32_t o[8];
+            uint32_t o[8], o2[8];
+            if constexpr (GRAD) {
+                const uint16_t* src = reinterpret_cast<const uint16_t*>(p.dh) + f0 + row;
+                uint32_t dh[8];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const uint32_t v = f0 + row < p.f && c + j < p.t ? __ldg(src + (c + j) * p.lddh) : 0;
+                    dh[j / 2] = j & 1 ? dh[j / 2] | v << 16 : v;
+                }
+#define TZ_ROWS(A) \
+    for (int j = 0; j < 8; ++j) gated_pair_grad<A, BF>(g[2 * j], g[2 * j + 1], u[2 * j], u[2 * j + 1], widen2<BF>(dh[j]), o[j], o2[j])
+                TZ_ACT_SWITCH(p.act, _Pragma("unroll") TZ_ROWS)
+#undef TZ_ROWS
+            } else {
 #define TZ_ROWS(A) \
     for (int j = 0; j < 8; ++j) o[j] = gated_pair<A, BF>(g[2 * j], g[2 * j + 1], u[2 * j], u[2 * j + 1])
-            TZ_ACT_SWITCH(p.act, _Pragma("unroll") TZ_ROWS)
+                TZ_ACT_SWITCH(p.act, _Pragma("unroll") TZ_ROWS)
 #undef TZ_ROWS
+            }
             if (f0 + row < p.f) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (c + j < p.t) out[static_cast<long long>(c + j) * p.f] = static_cast<uint16_t>(o[j / 2] >> (16 * (j & 1)));
+                for (int j = 0; j < 16; ++j) {
+                    if (c + j >= p.t) break;
+                    const long long at = static_cast<long long>(c + j) * p.f;
+                    out[at] = static_cast<uint16_t>(o[j / 2] >> (16 * (j & 1)));
+                    if constexpr (GRAD) out2[at] = static_cast<uint16_t>(o2[j / 2] >> (16 * (j & 1)));
+                }
             }
         }
     }
