@@ -233,6 +233,7 @@ int rows_splits(K kern, int threads, Smem smem, int max_ctas, int tiles, int kbl
         if (kblocks < 4 * s || static_cast<int64_t>(tiles) * s > max_ctas) continue;
         const int per = (kblocks + s - 1) / s;
         if ((kblocks + per - 1) / per != s) continue;  // every rank has work
+        if (smem(per < 32 ? per : 32) > 227 * 1024) continue;
         std::atomic<int>& slot = fit[dev & 15][s][per < 32 ? per : 32];
         int n = slot.load(std::memory_order_relaxed);
         if (n == 0) {

@@ -230,17 +230,18 @@ __global__ void __launch_bounds__(256) dequantize_mxfp4_kernel(const uint8_t* co
 // y = q(x) q(W)^T (+ bias), or with GATED the gated form of interleaved weights: W rows come as 16 gate rows,
 // 16 up rows, and so on, so a 32-column chunk of the accumulator holds the gate and the up values of 16 outputs.
 //
-// The structure of the 16-bit gated kernel (persistent, TMA producer, MMA issuer, 12 epilogue warps, two
-// accumulators, CTA pairs).  A K block is 128 bytes = 256 values: four MMAs of 64.  Its scales are two
-// chunks for the CTA's 128 rows of A and four for the columns' rows of W (both CTAs of a pair keep all of them) and go to TMEM by tcgen05.cp, each stage to its own 24 columns: a stage's scales are only
-// replaced once its MMAs have completed.  BN = 192 leaves TMEM for that: 2 x 192 + 24 x stages <= 512 columns.
+// The structure of the 16-bit gated kernel (persistent, TMA producer, MMA issuer, epilogue warps in groups of 12, two
+// accumulators, CTA pairs).  A K block is 128 bytes = 256 values: four MMAs of 64.  Its scales are two chunks for the
+// CTA's 128 rows of A and four for the columns' rows of W (both CTAs of a pair keep all of them).  They go to TMEM by
+// tcgen05.cp, each stage to its own 24 columns: a stage's scales are only replaced once its MMAs have completed.
+// BN = 192 leaves TMEM for that: 2 x 192 + 24 x stages <= 512 columns.
 //
 // Measured: 8192 x 8192 x 8192 f16 196 us alone (5.6 PFLOP/s, tensor pipe 77 % active; the feed from L2, 31 KB per SM
 // for 384 clocks of MMAs, is the bound), about 240 us in a loop under the power cap.  The issue of a K block's six
 // scale copies and four MMAs is serial: with a branch on the lane number around it (operands moved to uniform
 // registers one by one) a K block took 1050 clocks and the product 355 us.  The encoder batch's gated form (T 18106,
-// D 384, F 1536) takes 26 us: two K blocks a tile, bound by the epilogue (special-function
-// unit 61 %; 31 us with one group of epilogue warps for both accumulators).
+// D 384, F 1536) takes 26 us: two K blocks a tile, bound by the epilogue (special-function unit 61 %; 31 us with one
+// group of epilogue warps for both accumulators).
 constexpr int GROUP = 16;
 
 struct MxParams {

@@ -327,3 +327,19 @@ def test_long_rows(ctx, M, K):
     for times in (1, 500):  # the same 40 weight rows again and again
         y = ops.linear_mxfp4(ctx, x, ops.quantize_mxfp4(ctx, w.repeat(times, 1)))
         near(y, want.repeat(1, times), tol.repeat(1, times), (M, K, times))
+
+
+@pytest.mark.parametrize("reserve,M,K,N", [(146, 32, 16384, 128), (146, 17, 15872, 800), (130, 20, 16384, 1000), (130, 32, 16640, 1000),
+                                           (146, 16, 16384, 128), (146, 2, 32768, 120)])
+def test_long_rows_and_few_sms(reserve, M, K, N):
+    """So few SMs that a cluster of two would give each CTA more of x than its shared memory holds, or just as much."""
+    from tenzor_b200 import ops
+    from tenzor_b200.runtime import Context
+    c = Context(0)
+    c.set_sm_reserve(reserve)
+    x, w = rand(M, K, "f16", M, spread=False), (rand(N, K, "f16", N, spread=False).float() * K ** -0.5).half()
+    y = ops.linear_mxfp4(c, x, ops.quantize_mxfp4(c, w))
+    want, err = product64(x, w)
+    near(y, want, err + U["f16"] * (want.abs() + err) + TINY["f16"])
+    c.check_status()
+    c.close()
