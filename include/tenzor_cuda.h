@@ -56,8 +56,8 @@ int tz_cuda_synchronize(tz_ctx_t ctx);
  * check fired (bit 1) since the last call.  Reading clears it. */
 int tz_cuda_check_status(tz_ctx_t ctx);
 int tz_cuda_sm_count(tz_ctx_t ctx);
-/* Persistent GEMM grids of this context (the model's projections and the op-level GEMMs) use at most
- * SMs - n CTAs, so that n SMs stay free for kernels that run concurrently on another stream -- the
+/* Persistent GEMM grids of this context (the model's projections and the op-level GEMMs, the gated block's and
+ * the MXFP4 products among them, the kernels for few rows too) use at most SMs - n CTAs, so that n SMs stay free for kernels that run concurrently on another stream -- the
  * collective of a multi-GPU pipeline (e.g. NCCL limited to n CTAs with NCCL_MAX_CTAS), which would
  * otherwise hold SMs the one-CTA-per-SM grids wait for.  0 (the default) uses every SM. */
 int tz_cuda_set_sm_reserve(tz_ctx_t ctx, int n);

@@ -730,7 +730,10 @@ int launch_rows(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const 
     p.du = const_cast<void*>(o1.p);
     p.dh = dh.p;
     p.lddh = dh.ld;
-    return launch_cluster(kern, splits, dim3(splits, tiles), dim3(C::THREADS), C::SMEM, s, true, mx, mg, mu, p, ctx->d_status);
+    return rows_launches(ctx, tiles, splits, [&](int t0, int n, bool pdl) {
+        p.tile0 = t0;
+        return launch_cluster(kern, splits, dim3(splits, n), dim3(C::THREADS), C::SMEM, s, pdl, mx, mg, mu, p, ctx->d_status);
+    });
 }
 
 // The few-token kernel; *ran says whether the sizes are its own.

@@ -33,6 +33,7 @@ __device__ __forceinline__ float2 widen2(uint32_t w) {
 
 struct RowsParams {
     int kblocks, kper;  // K blocks of 64, and of one cluster rank
+    int tile0;          // the launch's first feature tile
     int t, f, act;
     void* h;         // GRAD: dg
     void* du;        // GRAD
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(RowsCfg<N>::THREADS, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(tzp::cluster_ctarank());
-    const int f0 = static_cast<int>(blockIdx.y) * 128;
+    const int f0 = (p.tile0 + static_cast<int>(blockIdx.y)) * 128;
     const int kb0 = rank * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
 
     if (threadIdx.x == 0) {
@@ -255,6 +256,20 @@ int rows_splits(K kern, int threads, Smem smem, int max_ctas, int tiles, int kbl
             *out = s;
             return TZ_OK;
         }
+    }
+    return TZ_OK;
+}
+
+// The launches of a few-row kernel's feature tiles, launch(first tile, tiles, pdl): one for all of them, or, where SMs
+// are reserved and the tiles are more than the CTAs that the others hold at a time, one for as many tiles as there are
+// SMs left, and so on, each after the one before is done.  (rows_splits gives no cluster to tiles that do not fit.)
+template <typename Launch>
+int rows_launches(tz_ctx_t ctx, int tiles, int splits, Launch launch) {
+    const int at_once = (ctx->sm_count - ctx->sm_reserve) / splits;
+    const int step = ctx->sm_reserve > 0 && tiles > at_once ? at_once : tiles;
+    for (int t = 0; t < tiles; t += step) {
+        const int rc = launch(t, tiles - t < step ? tiles - t : step, t == 0);
+        if (rc) return rc;
     }
     return TZ_OK;
 }

@@ -626,6 +626,7 @@ struct MxRowsParams {
     const float* bias;
     int rows, k, n;      // of x, of a row, weight rows
     int k_chunks, kblocks, kper;
+    int tile0;           // the launch's first tile of weight rows
     int act;
 };
 
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(tzp::cluster_ctarank());
-    const int n0 = static_cast<int>(blockIdx.y) * 128;
+    const int tile = p.tile0 + static_cast<int>(blockIdx.y), n0 = tile * 128;
     const int kb0 = rank * p.kper, kb1 = min(p.kblocks, kb0 + p.kper);
 
     if (threadIdx.x == 0) {
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(MxRowsCfg<N>::THREADS, 1)
                 if (issue) {
                     tzp::mbar_arrive_expect_tx(&full[s], C::STAGE);
                     tzp::tma_load_2d(a, &tmW, kb * 128, n0, &full[s]);
-                    tzp::tma_load_2d(a + 16384, &tmSW, 0, static_cast<int>(blockIdx.y) * p.k_chunks + 2 * kb, &full[s]);
+                    tzp::tma_load_2d(a + 16384, &tmSW, 0, tile * p.k_chunks + 2 * kb, &full[s]);
                 }
                 __syncwarp();
             }
@@ -936,7 +937,7 @@ int launch_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int rows, const Q4&
     // With room for 32 rows every CTA's quantising of x weighs more, and from the third wave of CTAs on the large
     // kernel is faster: 17 / 32 rows take 22.8 / 25.2 us here and 25.3 / 25.0 there at 256 tiles (D = 4096), 28.6 / 31.3
     // and 23.1 / 22.2 us at 512 tiles (D = 2048).
-    if (N > 16 && tiles > 2 * ctx->sm_count) return TZ_OK;
+    if (N > 16 && tiles > 2 * (ctx->sm_count - ctx->sm_reserve)) return TZ_OK;
     static std::atomic<unsigned> done{0};
     int rc = ensure_smem(kern, C::smem(C::MAX_KB), done);
     if (rc) return rc;
@@ -962,7 +963,10 @@ int launch_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int rows, const Q4&
                                  CU_TENSOR_MAP_SWIZZLE_NONE)))
         return rc;
     *ran = true;
-    return launch_cluster(kern, splits, dim3(splits, tiles), dim3(C::THREADS), C::smem(p.kper), s, true, mw, msw, p, ctx->d_status);
+    return rows_launches(ctx, tiles, splits, [&](int t0, int n, bool pdl) {
+        p.tile0 = t0;
+        return launch_cluster(kern, splits, dim3(splits, n), dim3(C::THREADS), C::smem(p.kper), s, pdl, mw, msw, p, ctx->d_status);
+    });
 }
 template <int XDT, int OUT, bool GATED>
 int try_mx_rows(tz_ctx_t ctx, const void* x, int64_t ldx, int64_t rows, const Q4& w, int k, const float* bias, void* y, int act, cudaStream_t s,

@@ -267,6 +267,59 @@ def test_few_sms(reserve):
     c.close()
 
 
+class _KernelNode(C.Structure):  # CUDA_KERNEL_NODE_PARAMS of the driver API
+    _fields_ = [("func", C.c_void_p), *((n, C.c_uint) for n in ("gx", "gy", "gz", "bx", "by", "bz", "smem")), ("params", C.c_void_p),
+                ("extra", C.c_void_p), ("kern", C.c_void_p), ("ctx", C.c_void_p)]
+
+
+def captured_grids(fn):
+    """(blocks, dynamic shared memory) of every kernel that fn launches."""
+    cu = C.CDLL("libcuda.so.1")
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        keep = fn()
+    graph, n = C.c_void_p(g.raw_cuda_graph()), C.c_size_t()
+    assert cu.cuGraphGetNodes(graph, None, C.byref(n)) == 0
+    nodes = (C.c_void_p * n.value)()
+    assert cu.cuGraphGetNodes(graph, nodes, C.byref(n)) == 0
+    got = []
+    for node in nodes:
+        kind, k = C.c_int(), _KernelNode()
+        assert cu.cuGraphNodeGetType(C.c_void_p(node), C.byref(kind)) == 0
+        if kind.value == 0:  # a kernel
+            assert cu.cuGraphKernelNodeGetParams_v2(C.c_void_p(node), C.byref(k)) == 0
+            got.append((k.gx * k.gy * k.gz, k.smem))
+    del keep
+    return got
+
+
+@pytest.mark.parametrize("reserve", [0, 16, 100, 146])
+@pytest.mark.parametrize("T", [1, 16, 20, 32, 100, 300])
+def test_reserved_sms_stay_free(reserve, T):
+    """No product kernel (all of them use shared memory for their operands) launches more CTAs than there are SMs left;
+    more feature tiles than that are taken one lot after the other, with the same result."""
+    from tenzor_b200 import ops
+    from tenzor_b200.runtime import Context
+    c = Context(0)
+    x, wg, wu, dh = make(T, 64, 151 * 128 - 40, "bf16", seed=T)
+    want = (ops.gated_linear(c, x, wg, wu), *ops.gated_linear_backward(c, x, wg, wu, dh))
+    c.set_sm_reserve(reserve)
+
+    def call():
+        return ops.gated_linear(c, x, wg, wu), *ops.gated_linear_backward(c, x, wg, wu, dh)
+
+    grids = [blocks for blocks, smem in captured_grids(call) if smem > 0]
+    assert len(grids) >= 3 and (reserve == 0 or max(grids) <= c.sm_count - reserve), grids
+    got = call()
+    torch.cuda.synchronize()
+    c.check_status()
+    assert torch.equal(got[0], want[0])  # h: one sum over all of D, whatever the grid
+    _, tol = reference(x, wg, wu, dh, "silu")
+    for g, w, t in zip(got[1:], want[1:], tol[1:]):  # the gradients' sums are split by the SMs in use
+        near(g, w.double(), 2 * t, (T, reserve))
+    c.close()
+
+
 def test_no_sm_left_is_refused():
     from tenzor_b200 import TenzorError, ops
     from tenzor_b200.runtime import Context

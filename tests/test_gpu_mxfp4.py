@@ -300,6 +300,44 @@ def test_few_sms(reserve):
     c.close()
 
 
+def gated64(x, wg, wu, act):
+    """The gated block on quantised operands in 64 bits, and the bound of a 16-bit result."""
+    from test_gpu_gated import act64
+    dt = {v: k for k, v in DT.items()}[x.dtype]
+    (g, eg), (u, eu) = product64(x, wg), product64(x, wu)
+    a = act64(act, g)
+    ea = 1.13 * eg + 2.0 ** -19 * (1 + g.abs())  # |act'| <= 1.13; the fast exponential
+    err = u.abs() * ea + a.abs() * eu + ea * eu
+    return a * u, err + U[dt] * ((a * u).abs() + err) + TINY[dt]
+
+
+@pytest.mark.parametrize("reserve", [0, 16, 100, 146])
+@pytest.mark.parametrize("M", [1, 16, 20, 32, 100, 300])
+def test_reserved_sms_stay_free(reserve, M):
+    """No product kernel (all of them use shared memory for their operands) launches more CTAs than there are SMs left."""
+    from test_gpu_gated import captured_grids
+    from tenzor_b200 import ops
+    from tenzor_b200.runtime import Context
+    c = Context(0)
+    x, w = rand(M, 160, "bf16", M), rand(151 * 128 - 40, 160, "bf16", 1)
+    wg, wu = (0.08 * rand(151 * 64 - 32, 160, "bf16", k) for k in (2, 3))
+    wq, wp = ops.quantize_mxfp4(c, w), ops.pack_gated_mxfp4(c, wg, wu)
+    c.set_sm_reserve(reserve)
+
+    def call():
+        return ops.linear_mxfp4(c, x, wq), ops.gated_linear_mxfp4(c, x, wp, "gelu")
+
+    grids = [blocks for blocks, smem in captured_grids(call) if smem > 0]
+    assert len(grids) >= 2 and (reserve == 0 or max(grids) <= c.sm_count - reserve), grids
+    y, h = call()
+    torch.cuda.synchronize()
+    c.check_status()
+    want, err = product64(x, w)
+    near(y, want, err + U["bf16"] * (want.abs() + err))
+    near(h, *gated64(x, wg, wu, "gelu"))
+    c.close()
+
+
 def test_more_than_2_to_31_elements(ctx):
     from tenzor_b200 import ops
     rows, cols = 1_050_007, 2080
