@@ -349,7 +349,7 @@ int tz_reduce(tz_ctx_t ctx, int reduce_op, const int* pre_ops, int n_pre, const 
  * the 16-bit type `dtype` (tz_gemm_prec: TZ_PREC_F16 or TZ_PREC_BF16), 16-byte aligned; d, f and the row
  * strides multiples of 8, any t >= 0.  act: TZ_OP_SILU, TZ_OP_GELU (tanh form), TZ_OP_GELU_ERF,
  * TZ_OP_RELU or TZ_OP_SIGMOID.  Products accumulate in f32, activation and product are f32, and h is
- * rounded once. */
+ * rounded once.  Here and below an output or workspace that overlaps an input or another output is refused. */
 int tz_gated_linear(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate, const void* w_up, void* h,
                     int64_t t, int d, int f, int act, int dtype, tz_stream_t stream);
 /* Bytes of device workspace one tz_gated_linear_backward call of these sizes needs on a context with `sms`

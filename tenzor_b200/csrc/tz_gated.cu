@@ -824,6 +824,7 @@ int backward(tz_ctx_t ctx, const Mat& x, const Mat& wg, const Mat& wu, const Mat
 }
 
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+Span span16(const void* p, int64_t rows, int64_t cols, int64_t ld) { return {p, rows, static_cast<size_t>(cols) * 2, static_cast<size_t>(ld) * 2}; }
 
 int check_shape(const char* fn, int64_t T, int D, int F, int dtype, int act) {
     TZ_CHECK(dtype == TZ_PREC_F16 || dtype == TZ_PREC_BF16, TZ_EINVAL, "%s: dtype %d is neither f16 nor bf16", fn, dtype);
@@ -850,6 +851,9 @@ int tz_gated_linear(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate
     TZ_CHECK(x && w_gate && w_up && h, TZ_EINVAL, "tz_gated_linear: null pointer");
     TZ_CHECK(ldx >= d && ldx % 8 == 0, TZ_EINVAL, "tz_gated_linear: row stride %lld of x (at least D, a multiple of 8)", static_cast<long long>(ldx));
     TZ_CHECK(al16(x) && al16(w_gate) && al16(w_up) && al16(h), TZ_EINVAL, "tz_gated_linear: pointers must be 16-byte aligned");
+    const size_t wbytes = static_cast<size_t>(d) * f * 2;
+    if ((rc = check_apart("tz_gated_linear", "h", h, static_cast<size_t>(t) * f * 2, {span16(x, t, d, ldx), flat(w_gate, wbytes), flat(w_up, wbytes)})))
+        return rc;
     cudaStream_t s = pick_stream(ctx, stream);
     const Mat mx{x, t, d, ldx}, mg{w_gate, f, d, d}, mu{w_up, f, d, d}, mh{h, t, f, f};
     return dtype == TZ_PREC_BF16 ? forward<true>(ctx, mx, mg, mu, mh, act, s) : forward<false>(ctx, mx, mg, mu, mh, act, s);
@@ -871,8 +875,8 @@ int tz_gated_linear_backward(tz_ctx_t ctx, const void* x, int64_t ldx, const voi
     int rc = check_shape("tz_gated_linear_backward", t, d, f, dtype, act);
     if (rc) return rc;
     TZ_CHECK(w_gate && w_up && dw_gate && dw_up && (t == 0 || (x && dh && dx && workspace)), TZ_EINVAL, "tz_gated_linear_backward: null pointer");
-    cudaStream_t s = pick_stream(ctx, stream);
     if (t == 0) {  // an empty sum
+        cudaStream_t s = pick_stream(ctx, stream);
         TZ_CUDA(cudaMemsetAsync(dw_gate, 0, static_cast<size_t>(d) * f * 2, s));
         TZ_CUDA(cudaMemsetAsync(dw_up, 0, static_cast<size_t>(d) * f * 2, s));
         return TZ_OK;
@@ -885,6 +889,15 @@ int tz_gated_linear_backward(tz_ctx_t ctx, const void* x, int64_t ldx, const voi
     size_t need = 0;
     if ((rc = tz_gated_linear_backward_workspace(ctx->sm_count - ctx->sm_reserve, t, d, f, &need))) return rc;
     TZ_CHECK(workspace_bytes >= need, TZ_EINVAL, "tz_gated_linear_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    const size_t xbytes = static_cast<size_t>(t) * d * 2, wbytes = static_cast<size_t>(d) * f * 2;
+    const Span ix = span16(x, t, d, ldx), idh = span16(dh, t, f, lddh), ig = flat(w_gate, wbytes), iu = flat(w_up, wbytes);
+    const Span ox = flat(dx, xbytes), og = flat(dw_gate, wbytes), ou = flat(dw_up, wbytes);
+    if ((rc = check_apart("tz_gated_linear_backward", "dx", dx, xbytes, {ix, idh, ig, iu})) ||
+        (rc = check_apart("tz_gated_linear_backward", "dw_gate", dw_gate, wbytes, {ix, idh, ig, iu, ox})) ||
+        (rc = check_apart("tz_gated_linear_backward", "dw_up", dw_up, wbytes, {ix, idh, ig, iu, ox, og})) ||
+        (rc = check_apart("tz_gated_linear_backward", "the workspace", workspace, need, {ix, idh, ig, iu, ox, og, ou})))
+        return rc;
+    cudaStream_t s = pick_stream(ctx, stream);
     const Mat mx{x, t, d, ldx}, mg{w_gate, f, d, d}, mu{w_up, f, d, d}, mdh{dh, t, f, lddh}, mdx{dx, t, d, d}, mwg{dw_gate, f, d, d},
         mwu{dw_up, f, d, d};
     char* ws = static_cast<char*>(workspace);

@@ -5,6 +5,7 @@
 
 #include <cstdarg>
 #include <cstdint>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <utility>
@@ -29,6 +30,28 @@ void clear_error();
     do {                                                           \
         if (!(cond)) return ::tz::fail((code), __VA_ARGS__);       \
     } while (0)
+
+// Memory that a call reads: rows of `width` bytes, `pitch` (at least `width`) bytes apart.
+struct Span {
+    const void* p;
+    int64_t rows;
+    size_t width, pitch;
+};
+inline Span flat(const void* p, size_t bytes) { return {p, 1, bytes, bytes}; }
+// Whether the `bytes` at `out` share one with the span (the gaps between its rows do not count).
+inline bool overlaps(const void* out, size_t bytes, const Span& in) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in.p);
+    if (!a || !b || bytes == 0 || in.rows <= 0 || in.width == 0) return false;
+    if (a < b) return b - a < bytes;
+    const size_t row = (a - b) / in.pitch, at = (a - b) % in.pitch;
+    if (row >= static_cast<size_t>(in.rows)) return false;
+    return at < in.width || (row + 1 < static_cast<size_t>(in.rows) && in.pitch - at < bytes);
+}
+// Refuses an output that overlaps what the call still reads: its kernels write while other CTAs read.
+inline int check_apart(const char* fn, const char* name, const void* out, size_t bytes, std::initializer_list<Span> others) {
+    for (const Span& s : others) TZ_CHECK(!overlaps(out, bytes, s), TZ_EINVAL, "%s: %s overlaps an input or another output", fn, name);
+    return TZ_OK;
+}
 
 // A growable device scratch arena owned by a context (op-level calls that need temporaries).
 struct Scratch {

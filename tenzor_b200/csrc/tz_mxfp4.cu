@@ -1006,7 +1006,9 @@ int quant_any(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, void* codes, 
 size_t a256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 size_t code_bytes(int64_t rows, int cols) { return static_cast<size_t>(rows) * (cols / 2); }
 size_t scale_bytes(int64_t rows, int cols) { return static_cast<size_t>((rows + 127) / 128) * ((cols + 127) / 128) * 512; }
+size_t value_bytes(int64_t rows, int64_t cols, int dtype) { return static_cast<size_t>(rows) * cols * (dtype == DT_F32 ? 4 : 2); }
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+Span span_of(const void* x, int64_t rows, int cols, int64_t ldx, int dtype) { return {x, rows, value_bytes(1, cols, dtype), value_bytes(1, ldx, dtype)}; }
 
 int check_dims(const char* fn, int64_t rows, int cols) {
     TZ_CHECK(rows >= 0 && rows <= (1 << 30) && cols > 0 && cols <= (1 << 24), TZ_EINVAL, "%s: bad sizes (%lld rows, %d values)", fn,
@@ -1052,6 +1054,10 @@ int tz_quantize_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, void*
     TZ_CHECK(x && codes && scales, TZ_EINVAL, "%s: null pointer", fn);
     if ((rc = check_rows(fn, x, ldx, cols, dtype))) return rc;
     TZ_CHECK(al16(codes) && al16(scales), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    const Span ix = span_of(x, rows, cols, ldx, dtype);
+    if ((rc = check_apart(fn, "codes", codes, code_bytes(rows, cols), {ix})) ||
+        (rc = check_apart(fn, "scales", scales, scale_bytes(rows, cols), {ix, flat(codes, code_bytes(rows, cols))})))
+        return rc;
     return quant_any<0>(ctx, x, ldx, dtype, codes, scales, rows, cols, 0, pick_stream(ctx, stream));
 }
 
@@ -1063,6 +1069,8 @@ int tz_dequantize_mxfp4(tz_ctx_t ctx, const void* codes, const void* scales, voi
     if (rows == 0) return TZ_OK;
     TZ_CHECK(codes && scales && out, TZ_EINVAL, "%s: null pointer", fn);
     TZ_CHECK(al16(codes) && al16(scales) && al16(out), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    if ((rc = check_apart(fn, "out", out, value_bytes(rows, cols, dtype), {flat(codes, code_bytes(rows, cols)), flat(scales, scale_bytes(rows, cols))})))
+        return rc;
     auto* kern = dtype == DT_F32 ? dequantize_mxfp4_kernel<DT_F32> : dtype == DT_F16 ? dequantize_mxfp4_kernel<DT_F16> : dequantize_mxfp4_kernel<DT_BF16>;
     return launch_kernel(kern, row_grid(rows, cols), dim3(256), 0, pick_stream(ctx, stream), false, static_cast<const uint8_t*>(codes),
                          static_cast<const uint8_t*>(scales), out, static_cast<long long>(rows), cols);
@@ -1076,6 +1084,10 @@ int tz_pack_gated_mxfp4(tz_ctx_t ctx, const void* w_gate, const void* w_up, int 
     TZ_CHECK(f > 0 && f % GROUP == 0 && f <= (1 << 24), TZ_EINVAL, "%s: f must be a positive multiple of 16 (%d)", fn, f);
     if ((rc = check_rows(fn, w_gate, d, d, dtype)) || (rc = check_rows(fn, w_up, d, d, dtype))) return rc;
     TZ_CHECK(al16(codes) && al16(scales), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
+    const Span ig = flat(w_gate, value_bytes(f, d, dtype)), iu = flat(w_up, value_bytes(f, d, dtype));
+    if ((rc = check_apart(fn, "codes", codes, code_bytes(2ll * f, d), {ig, iu})) ||
+        (rc = check_apart(fn, "scales", scales, scale_bytes(2ll * f, d), {ig, iu, flat(codes, code_bytes(2ll * f, d))})))
+        return rc;
     cudaStream_t s = pick_stream(ctx, stream);
     if ((rc = quant_any<GROUP>(ctx, w_gate, d, dtype, codes, scales, f, d, 0, s))) return rc;
     return quant_any<GROUP>(ctx, w_up, d, dtype, codes, scales, f, d, GROUP, s);
@@ -1090,6 +1102,10 @@ int tz_gemm_mxfp4(tz_ctx_t ctx, const void* a_codes, const void* a_scales, const
     TZ_CHECK(n > 0, TZ_EINVAL, "%s: n must be positive", fn);
     if (m == 0) return TZ_OK;
     TZ_CHECK(a_codes && a_scales && w_codes && w_scales && y, TZ_EINVAL, "%s: null pointer", fn);
+    if ((rc = check_apart(fn, "y", y, value_bytes(m, n, y_dtype),
+                          {flat(a_codes, code_bytes(m, k)), flat(a_scales, scale_bytes(m, k)), flat(w_codes, code_bytes(n, k)),
+                           flat(w_scales, scale_bytes(n, k)), flat(bias, bias ? 4ull * n : 0)})))
+        return rc;
     return product(ctx, fn, {static_cast<const uint8_t*>(a_codes), static_cast<const uint8_t*>(a_scales), m},
                    {static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), n}, k, bias, y, y_dtype, pick_stream(ctx, stream));
 }
@@ -1104,12 +1120,16 @@ int tz_linear_mxfp4_workspace(int64_t m, int k, int n, size_t* bytes) {
     return TZ_OK;
 }
 
-static int check_workspace(const char* fn, const void* ws, size_t ws_bytes, int64_t m, int k, int n) {
+// The workspace's size, and that output (`ybytes`) and workspace share no memory with the inputs or each other.
+static int check_workspace(const char* fn, const void* ws, size_t ws_bytes, int64_t m, int k, int n, const Span& x, const void* w_codes,
+                           const void* w_scales, const float* bias, const char* yname, const void* y, size_t ybytes) {
     size_t need = 0;
     int rc = tz_linear_mxfp4_workspace(m, k, n, &need);
     if (rc) return rc;
     TZ_CHECK(need == 0 || (ws && al16(ws) && ws_bytes >= need), TZ_EINVAL, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", fn, ws_bytes, need);
-    return TZ_OK;
+    const Span wc = flat(w_codes, code_bytes(n, k)), sc = flat(w_scales, scale_bytes(n, k)), b = flat(bias, bias ? 4ull * n : 0);
+    if ((rc = check_apart(fn, yname, y, ybytes, {x, wc, sc, b}))) return rc;
+    return check_apart(fn, "the workspace", ws, need, {x, wc, sc, b, flat(y, ybytes)});
 }
 static int quantize_input(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, void* ws, int64_t m, int k, cudaStream_t s, Q4* out) {
     uint8_t* codes = static_cast<uint8_t*>(ws);
@@ -1129,7 +1149,9 @@ int tz_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int x_dtype, const
     TZ_CHECK(x && w_codes && w_scales && y, TZ_EINVAL, "%s: null pointer", fn);
     if ((rc = check_rows(fn, x, ldx, k, x_dtype))) return rc;
     TZ_CHECK(al16(w_codes) && al16(w_scales) && al16(bias) && al16(y), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
-    if ((rc = check_workspace(fn, workspace, workspace_bytes, m, k, n))) return rc;
+    if ((rc = check_workspace(fn, workspace, workspace_bytes, m, k, n, span_of(x, m, k, ldx, x_dtype), w_codes, w_scales, bias, "y", y,
+                              value_bytes(m, n, y_dtype))))
+        return rc;
     cudaStream_t s = pick_stream(ctx, stream);
     const Q4 w{static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), n};
     bool ran = false;
@@ -1154,7 +1176,9 @@ int tz_gated_linear_mxfp4(tz_ctx_t ctx, const void* x, int64_t ldx, int dtype, c
     TZ_CHECK(x && w_codes && w_scales && h, TZ_EINVAL, "%s: null pointer", fn);
     TZ_CHECK(al16(w_codes) && al16(w_scales) && al16(h), TZ_EINVAL, "%s: pointers must be 16-byte aligned", fn);
     if ((rc = check_rows(fn, x, ldx, d, dtype))) return rc;
-    if ((rc = check_workspace(fn, workspace, workspace_bytes, t, d, 2 * f))) return rc;
+    if ((rc = check_workspace(fn, workspace, workspace_bytes, t, d, 2 * f, span_of(x, t, d, ldx, dtype), w_codes, w_scales, nullptr, "h", h,
+                              value_bytes(t, f, dtype))))
+        return rc;
     cudaStream_t s = pick_stream(ctx, stream);
     const Q4 w{static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), 2ll * f};
     bool ran = false;

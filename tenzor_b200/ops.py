@@ -335,7 +335,8 @@ def _two(fn, x, w):
 
 def gated_linear(ctx: Context, x, w_gate, w_up, act: str = "silu", out=None):
     """act(x @ w_gate.T) * (x @ w_up.T) in one kernel: x [T, D] (rows may be strided), w_gate and w_up [F, D],
-    all float16 or all bfloat16, D and F multiples of 8; returns [T, F].  act: one of GATED_ACTS."""
+    all float16 or all bfloat16, D and F multiples of 8; returns [T, F].  act: one of GATED_ACTS.  `out` shares no
+    memory with the inputs."""
     dtype = x.dtype
     dt = _dtype16("gated_linear", dtype)
     code = _act_code("gated_linear", act)
@@ -502,7 +503,8 @@ def _mx_workspace(m, k, n):
 
 def linear_mxfp4(ctx: Context, x, w: Mxfp4, bias=None, out_dtype=None, out=None):
     """q(x) @ w.T (+ bias f32 [N]): x [M, K] (float32, float16 or bfloat16, quantised in the call) or an Mxfp4;
-    returns [M, N] of `out_dtype` (x's type; float32 for an Mxfp4).  N is a multiple of 8."""
+    returns [M, N] of `out_dtype` (x's type; float32 for an Mxfp4).  N is a multiple of 8.  `out` shares no memory with
+    the inputs."""
     fn = "linear_mxfp4"
     _mx(fn, "w", ctx, w)
     given = isinstance(x, Mxfp4)
@@ -540,7 +542,7 @@ def linear_mxfp4(ctx: Context, x, w: Mxfp4, bias=None, out_dtype=None, out=None)
 
 def gated_linear_mxfp4(ctx: Context, x, w: Mxfp4, act: str = "silu", out=None):
     """act(q(x) @ wg.T) * (q(x) @ wu.T) with the weights of pack_gated_mxfp4: x [T, D] float16 or bfloat16;
-    returns [T, F]."""
+    returns [T, F].  `out` shares no memory with the inputs."""
     fn = "gated_linear_mxfp4"
     dtype = x.dtype
     _dtype16(fn, dtype)

@@ -267,6 +267,45 @@ def test_few_sms(reserve):
     c.close()
 
 
+@pytest.mark.parametrize("T", [1, 6, 40, 300])
+def test_outputs_that_overlap_are_refused(ctx, T):
+    """Other CTAs still read what an overlapping output would overwrite."""
+    from tenzor_b200 import TenzorError, _lib, ops
+    x, wg, wu, dh = make(T, 64, 64, "bf16")
+    buf = torch.zeros(T * 64 + 64 * 64 + T * 64, device="cuda", dtype=x.dtype)
+    at = lambda n, rows: buf[n:n + rows * 64].view(rows, 64)  # noqa: E731
+    for a, gate, up, out in ((x, wg, wu, x), (at(8, T), wg, wu, at(0, T)), (at(0, T), wg, wu, at(T * 64 - 8, T)),
+                             (x, at(T * 64, 64), wu, at(8 + 64, T)), (x, wg, at(0, 64), at(64 * 64 - 8, T))):
+        with pytest.raises(TenzorError) as e:
+            ops.gated_linear(ctx, a, gate, up, out=out)
+        assert e.value.code == _lib.TZ_EINVAL and "overlaps" in str(e.value)
+    # touching, or in the gap between two rows, is no overlap
+    assert torch.equal(ops.gated_linear(ctx, at(0, T), wg, wu, out=at(T * 64, T)), torch.zeros_like(x))
+    wide = torch.zeros(2, 64 + 128 + 8, device="cuda", dtype=x.dtype)
+    wide[:, :64] = x[0]
+    gap = wide.view(-1)[64:192].view(2, 64)
+    assert torch.equal(ops.gated_linear(ctx, wide[:, :64], wg, wu, out=gap), ops.gated_linear(ctx, x[:1].repeat(2, 1), wg, wu))
+    with pytest.raises(TenzorError):
+        ops.gated_linear(ctx, wide[:, :64], wg, wu, out=wide.view(-1)[80:208].view(2, 64))
+
+    Lb, p = _lib.lib(), (lambda t: C.c_void_p(t.data_ptr()))
+    need = C.c_size_t()
+    assert Lb.tz_gated_linear_backward_workspace(ctx.sm_count, T, 64, 64, C.byref(need)) == 0
+    ws = torch.zeros(need.value, device="cuda", dtype=torch.uint8)
+    good = {"dx": torch.empty_like(x), "dw_gate": torch.empty_like(wg), "dw_up": torch.empty_like(wu), "ws": ws}
+
+    def call(**other):
+        o = {**good, **other}
+        return Lb.tz_gated_linear_backward(ctx.handle, p(x), 64, p(wg), p(wu), p(dh), 64, p(o["dx"]), p(o["dw_gate"]), p(o["dw_up"]), p(o["ws"]),
+                                           need.value, T, 64, 64, _lib.OP["silu"], 1, None)
+
+    for bad in ({"dx": x}, {"dx": dh}, {"dx": wg}, {"dw_gate": wg}, {"dw_up": wg}, {"dw_up": good["dw_gate"]}, {"dw_gate": good["dx"]}, {"ws": x},
+                {"ws": good["dw_up"]}, {"dx": ws}):
+        assert call(**bad) == _lib.TZ_EINVAL and "overlaps" in Lb.tz_get_last_error().decode(), bad
+    assert call() == 0
+    torch.cuda.synchronize()
+
+
 class _KernelNode(C.Structure):  # CUDA_KERNEL_NODE_PARAMS of the driver API
     _fields_ = [("func", C.c_void_p), *((n, C.c_uint) for n in ("gx", "gy", "gz", "bx", "by", "bz", "smem")), ("params", C.c_void_p),
                 ("extra", C.c_void_p), ("kern", C.c_void_p), ("ctx", C.c_void_p)]

@@ -300,6 +300,46 @@ def test_few_sms(reserve):
     c.close()
 
 
+@pytest.mark.parametrize("M", [1, 20, 40, 300])
+def test_outputs_that_overlap_are_refused(ctx, M):
+    from tenzor_b200 import TenzorError, _lib, ops
+    x, w = rand(M, 64, "bf16", 1), ops.quantize_mxfp4(ctx, rand(64, 64, "bf16", 2))
+    wp = ops.pack_gated_mxfp4(ctx, rand(64, 64, "bf16", 1), rand(64, 64, "bf16", 2))
+    bias = torch.zeros(64 + 64 * M, device="cuda")
+    calls = [lambda: ops.linear_mxfp4(ctx, x, w, out=x), lambda: ops.gated_linear_mxfp4(ctx, x, wp, out=x),
+             lambda: ops.linear_mxfp4(ctx, x, w, bias=bias[:64], out_dtype=torch.float32, out=bias[60:60 + 64 * M].view(M, 64))]
+    if M <= 20:  # outputs inside the weights' codes and scales
+        for q, f in ((w, ops.linear_mxfp4), (wp, ops.gated_linear_mxfp4)):
+            for end in (M * 128, q.buf.numel()):
+                calls.append(lambda q=q, f=f, end=end: f(ctx, x, q, out=q.buf[end - M * 128:end].view(torch.bfloat16).view(M, 64)))
+    for call in calls:
+        with pytest.raises(TenzorError) as e:
+            call()
+        assert e.value.code == _lib.TZ_EINVAL and "overlaps" in str(e.value)
+    Lb = _lib.lib()
+    v = torch.zeros(8 * M * 64, device="cuda")
+    a = v.data_ptr()
+    n = M * 64 * 4
+    for codes, scales in ((a, a + n), (a + 16, a + n), (a + n, a + n), (a + n, a), (a + n - 16, a + 2 * n)):
+        assert Lb.tz_quantize_mxfp4(ctx.handle, a, 64, 0, codes, scales, M, 64, None) == _lib.TZ_EINVAL
+        assert "overlaps" in Lb.tz_get_last_error().decode()
+    for out in (w.codes_ptr, w.scales_ptr):
+        assert Lb.tz_dequantize_mxfp4(ctx.handle, w.codes_ptr, w.scales_ptr, out, 2, 64, 64, None) == _lib.TZ_EINVAL
+    assert Lb.tz_gemm_mxfp4(ctx.handle, w.codes_ptr, w.scales_ptr, w.codes_ptr, w.scales_ptr, None, w.codes_ptr, 2, 64, 64, 64, None) == _lib.TZ_EINVAL
+    g = torch.zeros(64, 64, device="cuda", dtype=torch.bfloat16)
+    assert Lb.tz_pack_gated_mxfp4(ctx.handle, g.data_ptr(), g.data_ptr(), 2, g.data_ptr(), wp.scales_ptr, 64, 64, None) == _lib.TZ_EINVAL
+    need = C.c_size_t()
+    assert Lb.tz_linear_mxfp4_workspace(M, 64, 64, C.byref(need)) == 0
+    if need.value:
+        big = torch.zeros(need.value + M * 128, device="cuda", dtype=torch.uint8)
+        y = torch.empty_like(x)
+        for ws in (big.data_ptr(), w.codes_ptr, x.data_ptr()):
+            out = big.data_ptr() if ws == big.data_ptr() else y.data_ptr()
+            assert Lb.tz_linear_mxfp4(ctx.handle, x.data_ptr(), 64, 2, w.codes_ptr, w.scales_ptr, None, out, 2, ws, need.value, M, 64, 64,
+                                      None) == _lib.TZ_EINVAL
+            assert "overlaps" in Lb.tz_get_last_error().decode()
+
+
 def gated64(x, wg, wu, act):
     """The gated block on quantised operands in 64 bits, and the bound of a 16-bit result."""
     from test_gpu_gated import act64
