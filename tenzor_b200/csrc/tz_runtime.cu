@@ -193,6 +193,8 @@ int tz_cuda_set_sm_reserve(tz_ctx_t ctx, int n) {
     return TZ_OK;
 }
 
+int tz_cuda_sm_reserve(tz_ctx_t ctx) { return ctx ? ctx->sm_reserve : 0; }
+
 int tz_cuda_selftest_wait(tz_ctx_t ctx) {
     TZ_CHECK(ctx, TZ_EINVAL, "null context");
     TZ_CUDA(cudaSetDevice(ctx->device));

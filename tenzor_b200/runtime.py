@@ -18,7 +18,6 @@ class Context:
         self.ptr = h.value  # the handle as a plain address: what the small, frequent calls pass
         self.device = device
         self.sm_count = L.lib().tz_cuda_sm_count(h)
-        self.sm_reserve = 0
         self._owned = weakref.WeakSet()  # models on this context: closed before the context
 
     def _adopt(self, obj):
@@ -27,7 +26,10 @@ class Context:
     def set_sm_reserve(self, n: int):
         """Leave n SMs free in the persistent GEMM grids (for a collective running concurrently)."""
         L.check(L.lib().tz_cuda_set_sm_reserve(self.handle, int(n)))
-        self.sm_reserve = int(n)
+
+    @property
+    def sm_reserve(self) -> int:
+        return L.lib().tz_cuda_sm_reserve(self.ptr)
 
     def synchronize(self):
         L.check(L.lib().tz_cuda_synchronize(self.handle))

@@ -359,6 +359,21 @@ def test_reserved_sms_stay_free(reserve, T):
     c.close()
 
 
+def test_reserve_set_through_the_c_abi():
+    """The backward call sizes its workspace for the SMs that the library uses, however the reserve was set."""
+    from tenzor_b200 import _lib
+    from tenzor_b200.runtime import Context
+    c = Context(0)
+    a = make(3000, 384, 264, "bf16", seed=1)
+    c.set_sm_reserve(140)
+    check(c, *a, "silu")
+    for reserve in (0, 116):  # more SMs, more splits: more partial sums than for the reserve above
+        assert _lib.lib().tz_cuda_set_sm_reserve(c.handle, reserve) == 0
+        check(c, *a, "silu")
+        assert c.sm_reserve == reserve
+    c.close()
+
+
 def test_no_sm_left_is_refused():
     from tenzor_b200 import TenzorError, ops
     from tenzor_b200.runtime import Context
