@@ -358,9 +358,11 @@ int tz_gated_linear(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate
 int tz_gated_linear_backward_workspace(int sms, int64_t t, int d, int f, size_t* bytes);
 /* dx [t, d], dw_gate and dw_up [f, d] from dh [t, f] (row stride lddh).  Nothing of the forward pass is
  * kept: gate and up are computed again in f32.  Their gradients are rounded once to `dtype` as operands of
- * the next products (an f16 value beyond 65504 there becomes an infinity); every sum is f32, and the order
- * of summation depends on the sizes alone.  The caller owns the workspace (16-byte aligned) until the
- * stream has passed the call.  t = 0 zeroes the weights' gradients. */
+ * the next products (an f16 value beyond 65504 there becomes an infinity).  Every sum is f32, in an order that
+ * the sizes and the SMs in use (count minus reserve) determine: equal calls repeat bit for bit, a reserve set in
+ * between can change last bits (here, and in all calls of up to 32 rows, whose sums are split by the SMs too).
+ * The caller owns the workspace (16-byte aligned) until the stream has passed the call.  t = 0 zeroes the
+ * weights' gradients. */
 int tz_gated_linear_backward(tz_ctx_t ctx, const void* x, int64_t ldx, const void* w_gate, const void* w_up,
                              const void* dh, int64_t lddh, void* dx, void* dw_gate, void* dw_up, void* workspace,
                              size_t workspace_bytes, int64_t t, int d, int f, int act, int dtype,

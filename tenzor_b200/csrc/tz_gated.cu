@@ -12,10 +12,10 @@
 //   GRAD dx and both weights' gradients in one launch (the two kinds of tiles fill each other's last round):
 //        dx = [dg | du] [Wg ; Wu] is one accumulation over both halves, the weights read MN-major in place;
 //        dWg = dg^T x and dWu = du^T x read both operands MN-major in place (the sum runs over tokens).
-//        Where the tiles do not fill the GPU their sums are split and the f32 partial sums added in a fixed
-//        order by a second kernel
+//        Where the tiles do not fill the SMs in use their sums are split and the f32 partial sums added
+//        in a fixed order by a second kernel
 //
-// Per CTA (64 + 32 * EPI warps): warp 0 TMA producer, warp 1 allocates TMEM and issues the MMAs, the others
+// Per CTA (64 + 32 * EPI threads): warp 0 TMA producer, warp 1 allocates TMEM and issues the MMAs, the others
 // read the accumulators (two buffers: the epilogue of a tile runs under the next tile's MMAs) and store boxes
 // of 32 x 32 outputs through swizzled shared memory and TMA, which clips ragged edges.  TMA fills reads
 // outside the operands with zeros, so any T works; D and F are multiples of 8 (16-byte rows).
