@@ -375,7 +375,10 @@ int tz_gated_linear_backward(tz_ctx_t ctx, const void* x, int64_t ldx, const voi
  *   codes   [rows, cols / 2] bytes, the even column in the low half
  *   scales  tz_mxfp4_scale_bytes(rows, cols) bytes: chunks of 512 bytes for 128 rows x 4 blocks, chunk
  *           (r / 128, b / 4) at ((r / 128) * ceil(cols / 128) + b / 4) * 512, byte
- *           (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 inside it; bytes of absent rows are not written
+ *           (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 inside it; bytes of absent rows are neither written nor
+ *           used.  The bytes of a present row's last chunk for blocks past `cols` are written as 0, and a caller
+ *           that builds scales itself must not leave 255 there: the tensor core multiplies 64 values at a time,
+ *           and past an odd multiple of 32 it would make NaN of that row's (or column's) results.
  * cols is a multiple of 32, all pointers are 16-byte aligned, row strides keep rows 16-byte aligned.
  * dtype, x_dtype, y_dtype: TZ_DT_F32, TZ_DT_F16 or TZ_DT_BF16. */
 int64_t tz_mxfp4_scale_bytes(int64_t rows, int cols);

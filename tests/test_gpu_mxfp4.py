@@ -378,6 +378,41 @@ def test_reserved_sms_stay_free(reserve, M):
     c.close()
 
 
+def quantise_into_ones(ctx, x, other=None):
+    """quantize_mxfp4(x), or pack_gated_mxfp4(x, other), into memory that is all ones: scale code 255, a NaN, wherever
+    nothing is written."""
+    from tenzor_b200 import _lib, ops
+    q = ops.Mxfp4(x.shape[0] * (1 if other is None else 2), x.shape[1], x, gated=other is not None)
+    q.buf.fill_(255)
+    dt, stream = ops._DTF[x.dtype], ops.CUDA_STREAM_LEGACY
+    if other is None:
+        rc = _lib.lib().tz_quantize_mxfp4(ctx.ptr, x.data_ptr(), q.cols, dt, q.codes_ptr, q.scales_ptr, q.rows, q.cols, stream)
+    else:
+        rc = _lib.lib().tz_pack_gated_mxfp4(ctx.ptr, x.data_ptr(), other.data_ptr(), dt, q.codes_ptr, q.scales_ptr, x.shape[0], q.cols, stream)
+    assert rc == 0
+    return q
+
+
+@pytest.mark.parametrize("K", [32, 64, 96, 160, 224, 288, 1056, 1312])
+@pytest.mark.parametrize("M", [3, 20, 40, 300])
+def test_scales_past_the_rows_end_and_of_absent_rows(ctx, M, K):
+    """Scale bytes of blocks past a row's end are written as 0 (an MMA of 64 values reads one of them where K is an odd
+    multiple of 32), and what the scales of absent rows hold reaches no result."""
+    from tenzor_b200 import ops
+    x, w = rand(M, K, "bf16", M), rand(72, K, "bf16", K)
+    wg, wu = (rand(80, K, "bf16", k) * 0.04 for k in (1, 2))
+    xq, wq, wp = quantise_into_ones(ctx, x), quantise_into_ones(ctx, w), quantise_into_ones(ctx, wg, wu)
+    for q in (xq, wq, wp):
+        raw = q.scales.cpu().numpy().reshape(-(-q.rows // 128), -1, 32, 4, 4)  # row block, chunk, row % 32, row / 32, block
+        rows = raw.transpose(0, 3, 2, 1, 4).reshape(raw.shape[0] * 128, -1)
+        assert (rows[:q.rows, K // 32:] == 0).all() and (rows[q.rows:] == 255).all()
+    want, err = product64(x, w)
+    for dt in ("f32", "bf16"):
+        for a in (x, xq):
+            near(ops.linear_mxfp4(ctx, a, wq, out_dtype=DT[dt]), want, err + U[dt] * (want.abs() + err) + TINY[dt])
+    near(ops.gated_linear_mxfp4(ctx, x, wp, "silu"), *gated64(x, wg, wu, "silu"))
+
+
 def test_more_than_2_to_31_elements(ctx):
     from tenzor_b200 import ops
     rows, cols = 1_050_007, 2080
