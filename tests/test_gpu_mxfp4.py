@@ -378,6 +378,71 @@ def test_reserved_sms_stay_free(reserve, M):
     c.close()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu_erf", "relu"])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("T,D,F", [(17, 160, 112), (17, 32, 16), (20, 4096, 1024), (24, 288, 80), (31, 512, 208), (32, 2080, 208), (32, 256, 4016)])
+def test_gated_17_to_32_tokens(ctx, T, D, F, dt, act):
+    """The few-row kernel's form for 32 rows: both of its column passes, both MMA issuers, splits, partial tiles."""
+    from tenzor_b200 import ops
+    x, wg, wu = rand(T, D, dt, T), rand(F, D, dt, 1), rand(F, D, dt, 2)
+    wg, wu = (wg.float() * 0.5 * D ** -0.5).to(DT[dt]), (wu.float() * 0.5 * D ** -0.5).to(DT[dt])
+    h = ops.gated_linear_mxfp4(ctx, x, ops.pack_gated_mxfp4(ctx, wg, wu), act)
+    torch.cuda.synchronize()
+    ctx.check_status()
+    near(h, *gated64(x, wg, wu, act))
+
+
+@pytest.mark.parametrize("waves", [2, 3])
+@pytest.mark.parametrize("M", [16, 17, 32])
+def test_few_rows_of_many_weights(ctx, M, waves):
+    """From the third wave of 128-row weight tiles on, 17 to 32 rows take the persistent kernel; up to 16 stay."""
+    from test_gpu_gated import captured_grids
+    from tenzor_b200 import ops
+    tiles = 2 * ctx.sm_count + (waves - 2) * 3
+    x, w = rand(M, 96, "bf16", M), rand(tiles * 128 - 32, 96, "bf16", 1)
+    wg, wu = (rand(tiles * 64 - 16, 96, "bf16", k) * 0.1 for k in (2, 3))
+    wq, wp = ops.quantize_mxfp4(ctx, w), ops.pack_gated_mxfp4(ctx, wg, wu)
+    grids = [blocks for blocks, smem in captured_grids(lambda: (ops.linear_mxfp4(ctx, x, wq), ops.gated_linear_mxfp4(ctx, x, wp))) if smem > 0]
+    assert len(grids) == 2
+    if M <= 16 or waves == 2:
+        assert grids == [tiles, tiles]
+    else:
+        assert max(grids) <= ctx.sm_count
+    want, err = product64(x, w)
+    near(ops.linear_mxfp4(ctx, x, wq), want, err + U["bf16"] * (want.abs() + err))
+    near(ops.gated_linear_mxfp4(ctx, x, wp), *gated64(x, wg, wu, "silu"))
+    ctx.check_status()
+
+
+@pytest.mark.parametrize("reserve", [100, 140, 146])
+@pytest.mark.parametrize("T,D,F", [(3, 512, 496), (16, 2048, 1040), (20, 288, 400), (32, 1056, 1040), (100, 96, 208), (700, 288, 768)])
+def test_gated_few_sms(reserve, T, D, F):
+    from tenzor_b200 import ops
+    from tenzor_b200.runtime import Context
+    c = Context(0)
+    c.set_sm_reserve(reserve)
+    x, wg, wu = rand(T, D, "f16", T), rand(F, D, "f16", 1), rand(F, D, "f16", 2)
+    wg, wu = (wg.float() * 0.5 * D ** -0.5).half(), (wu.float() * 0.5 * D ** -0.5).half()
+    h = ops.gated_linear_mxfp4(c, x, ops.pack_gated_mxfp4(c, wg, wu), "gelu")
+    torch.cuda.synchronize()
+    c.check_status()
+    near(h, *gated64(x, wg, wu, "gelu"))
+    c.close()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("F,D", [(16, 32), (48, 160), (144, 96), (80, 1056)])
+def test_packed_pair_layout(ctx, F, D, dt):
+    """16 rows of the gate's codes and scales, then 16 of the up projection's, and so on."""
+    from tenzor_b200 import ops
+    wg, wu = rand(F, D, dt, 1), rand(F, D, dt, 2)
+    q = ops.pack_gated_mxfp4(ctx, wg, wu)
+    assert q.gated and q.shape == (2 * F, D)
+    (_, cg, sg), (_, cu, su) = (quant64(w.float().cpu().numpy()) for w in (wg, wu))
+    mixed = lambda a, b: np.stack([a.reshape(F // 16, 16, -1), b.reshape(F // 16, 16, -1)], axis=1).reshape(2 * F, -1)  # noqa: E731
+    assert np.array_equal(element_codes(q), mixed(cg, cu)) and np.array_equal(scale_codes(q), mixed(sg, su))
+
+
 def quantise_into_ones(ctx, x, other=None):
     """quantize_mxfp4(x), or pack_gated_mxfp4(x, other), into memory that is all ones: scale code 255, a NaN, wherever
     nothing is written."""
