@@ -128,11 +128,20 @@ namespace tz {
 
 // launch_kernel with a cluster of `cg` CTAs (grid.x a multiple of cg).
 //
-// Programmatic launches and progress: CTAs that wait in griddepcontrol.wait hold their SM's threads and
-// registers.  If small CTAs of a later kernel got there while clusters of the awaited kernel were still to be
-// placed, they could take every slot that such a cluster needs, and both would wait for good.  So the cluster
-// kernels call launch_dependents only at a CTA's last tile, when every cluster of the grid has long been placed,
-// and the small kernels around them (quantisers, partial sums) are launched without the attribute.
+// Programmatic launches and progress.  A dependent grid is scheduled once every CTA of the grid before it has issued
+// launch_dependents or ended, so all clusters of that grid are placed by then.  The cluster kernels issue it at a CTA's
+// last tile (the few-row kernels at its end), long after their TMEM is allocated, so that no dependent holds threads,
+// shared memory or TMEM for the length of a grid, or takes TMEM that the awaited grid has still to ask for; the small
+// kernels around them (quantisers, partial sums) are launched without the attribute.  Waits on an mbarrier are bounded.
+// The three others end because
+//   griddepcontrol.wait  waits for grids earlier in the stream, whose CTAs have all started (above) and which end by
+//                        the same reasons;
+//   tcgen05.alloc        waits for columns of CTAs on the same SM.  A CTA of a tile kernel or of the 16-bit few-row
+//                        kernel (204 KB of shared memory or more) leaves no room for another that uses TMEM; 4-bit
+//                        few-row CTAs (73 KB or more: three to an SM) take 128 of the 512 columns each, so they never
+//                        wait for one another; and the other kernels that use TMEM have no clusters, so a CTA of
+//                        theirs that holds columns ends without any CTA that waits for them;
+//   barrier.cluster      the CTAs of a cluster are placed together, and each arrives after waits of the kinds above.
 template <typename... KArgs, typename... Args>
 int launch_cluster(void (*kern)(KArgs...), int cg, dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl,
                    Args&&... args) {
