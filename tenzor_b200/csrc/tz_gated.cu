@@ -21,14 +21,14 @@
 // outside the operands with zeros, so any T works; D and F are multiples of 8 (16-byte rows).
 //
 // Bounds and measurements (B200; "alone": one launch with idle clocks before it, "in a loop": under the board's power
-// cap, which the large shapes reach at 1.3 to 1.5 GHz):
+// cap, which holds the large shapes at 1.1 to 1.5 GHz):
 //   T 8192, D 4096, F 8192, bf16   FWD 680 us alone (1.62 PFLOP/s, tensor pipe 98.5 % active), 0.80 ms in a loop;
 //                                  BWD 0.70 ms and GRAD 1.51 ms alone (98.7 %), 2.4 to 2.6 ms together in a loop.
 //                                  Single CTAs (128 x 256 tiles, cta_group::1) took 0.97 and 2.97 ms in a loop: a pair
 //                                  reads each B tile once for 256 rows.
-//   T 18106, D 384, F 1536         FWD 35 us alone, 31 us back to back, 40 us in a loop: six K blocks a tile, so the
-//                                  operand feed from L2 and the epilogue (special-function unit 52 %) come close to
-//                                  the MMAs (73 %).  8 epilogue warps took 53 us alone, B tiles loaded for every tile
+//   T 18106, D 384, F 1536         FWD 36 us alone; a call 33 us in a burst of 21, 42 us sustained at 1.3 GHz (power
+//                                  cap).  Six K blocks a tile, so the operand feed from L2 and the epilogue
+//                                  (special-function unit 52 %) come close to the MMAs (73 %).  8 epilogue warps took 53 us alone, B tiles loaded for every tile
 //                                  48 us in a loop.  BWD 49 us (writes dg and du, 111 MB), GRAD 65 us, sums 8 us.
 #include <cuda.h>
 #include <cuda_bf16.h>

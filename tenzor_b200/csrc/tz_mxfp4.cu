@@ -616,9 +616,10 @@ __global__ void __launch_bounds__(MxCfg<CG, GATED>::THREADS, 1)
 // CTA needs its K slice only, so the work (0.5 us for 16 rows of 4096) hides behind the first weight copies and the
 // separate quantiser launch goes away.  With GATED a warp's 32 TMEM lanes are 16 gate rows and their 16 up rows.
 //
-// Measured (weights from HBM): D 4096, 2 F 16384 gated 9.2 us for one row, 9.9 for 16, 13.4 for 32; K 4096, N 8192 6.0,
-// 7.2 and 9.6.  What is left over the weights' own time (5.4 and 2.7 us) is the launch and the first copies (about 3 us)
-// and, from 16 rows on, the quantising.
+// Measured (a call of a graph, bf16; weights from HBM: 12 sets of them in turn, 213 MB or more / from L2: one set): D 4096,
+// 2 F 16384 gated 11.0 / 6.9 us for one row, 12.4 / 8.8 for 16, 15.2 / 12.2 for 32; K 4096, N 8192 8.0 us from HBM for one
+// row, 8.5 / 6.6 for 16, 10.2 / 8.8 for 32.  What is left over the weights' own time from HBM (5.4 and 2.7 us) is the
+// launch and the first copies (about 4 us) and, from 16 rows on, the quantising.
 struct MxRowsParams {
     const void* x;
     long long ldx;
